@@ -1,6 +1,7 @@
 """gswarp_b200 -- B200-native (sm_100a) 3DGS training hot path behind
 gswarp's drop-in API: GaussianRasterizationSettings / GaussianRasterizer,
-fused_ssim and distCUDA2."""
+fused_ssim and distCUDA2; beside them the shared attribute rows of compressed
+scenes (codebook_lookup)."""
 
 __version__ = "0.1.0"
 
@@ -25,3 +26,4 @@ from .rasterizer import (  # noqa: F401
 from ._runtime import get_tuned_block_dim, register_kernel_class, get_canonical_device  # noqa: F401
 from .fused_ssim import fused_ssim  # noqa: F401
 from .knn import distCUDA2  # noqa: F401
+from .codebook import codebook_lookup  # noqa: F401

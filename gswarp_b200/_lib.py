@@ -24,7 +24,7 @@ GSB_ERR_OVERFLOW = -2
 GSB_ERR_CUDA = -3
 GSB_ERR_TIMEOUT = -4
 
-ABI_VERSION = 16
+ABI_VERSION = 17
 RECORD_FLOATS = 12
 GRAD_FLOATS = 12
 
@@ -167,6 +167,18 @@ class KNNArgs(ctypes.Structure):
     ]
 
 
+class CodebookArgs(ctypes.Structure):
+    _fields_ = [
+        ("P", c_ll), ("K", c_ll), ("D", c_int), ("dtype", c_int), ("codes64", c_int), ("scale", c_float),
+        ("table", vp), ("codes", vp), ("gain", vp), ("out", vp),
+        ("grad_out", vp), ("grad_table", vp), ("grad_gain", vp), ("error_word", vp),
+        ("workspace", vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+# GSB_TYPE_* of the operators that take 16-bit tensors beside fp32
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
 _lib = None
 _lib_lock = threading.Lock()
 
@@ -178,6 +190,7 @@ EXPORTED = (
     "gsb_knn", "gsb_selftest_threshold_log", "gsb_ssim_fwd_noalloc", "gsb_photo_loss_fwd",
     "gsb_photo_loss_bwd", "gsb_adam_step", "gsb_densify_stats", "gsb_sh_colors_views",
     "gsb_sh_backward_views", "gsb_block_dim", "gsb_peak_fp32", "gsb_peak_ex2", "gsb_peak_work",
+    "gsb_codebook_fwd", "gsb_codebook_bwd_workspace_bytes", "gsb_codebook_bwd",
 )
 
 
@@ -214,6 +227,9 @@ def _declare(L) -> None:
     fn("gsb_sh_backward_views", c_int, [P(SHViewsArgs), vp])
     fn("gsb_knn_workspace_bytes", ctypes.c_size_t, [c_int])
     fn("gsb_knn", c_int, [P(KNNArgs), vp])
+    fn("gsb_codebook_fwd", c_int, [P(CodebookArgs), vp])
+    fn("gsb_codebook_bwd_workspace_bytes", ctypes.c_size_t, [c_ll, c_ll, c_int])
+    fn("gsb_codebook_bwd", c_int, [P(CodebookArgs), vp])
     fn("gsb_selftest_threshold_log", c_int, [vp, vp, c_ll, vp])
 
 

@@ -61,8 +61,10 @@ def sticky_error_word(device: torch.device) -> torch.Tensor:
 
 
 def _device_error(bits: int) -> RuntimeError:
-    return RuntimeError(f"gswarp_b200 device error word {int(bits):#x} "
-                        "(bounded wait timed out or binning mismatch)")
+    what = [] if not int(bits) & 3 else ["bounded wait timed out or binning mismatch"]
+    what += [text for bit, text in ((4, "codebook code out of range"), (8, "class label out of range"))
+             if int(bits) & bit]
+    return RuntimeError(f"gswarp_b200 device error word {int(bits):#x} ({', '.join(what)})")
 
 
 def raise_device_errors(device: torch.device) -> None:

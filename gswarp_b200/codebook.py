@@ -1,0 +1,124 @@
+"""Shared attribute rows: ``codebook_lookup(table, codes, scale)`` and its gradients.
+
+A compressed scene keeps one code per Gaussian and a codebook of attribute
+rows (SH rows, DC colours, feature rows).  The lookup expands the rows the
+rasterizer takes (``dc``, ``shs``, ``colors_precomp``); backward sums the
+rows' gradients by sorted code, without atomics, so it gives the same bits on
+every call.  ``scale`` is one factor, or a gain per Gaussian (shape-gain
+codebooks), which gets a gradient too.
+"""
+
+from __future__ import annotations
+
+import math
+from numbers import Real
+
+import torch
+
+from . import _lib, _pipeline
+
+__all__ = ["codebook_lookup"]
+
+
+def _validate(table, codes, scale) -> None:
+    if not isinstance(table, torch.Tensor) or not isinstance(codes, torch.Tensor):
+        raise ValueError("table and codes must be torch.Tensor instances")
+    if table.ndim < 2:
+        raise ValueError(f"table must have shape (K, ...) with at least two dimensions, got {tuple(table.shape)}")
+    if table.dtype not in _lib.DTYPES:
+        raise ValueError(f"table must have dtype float32, bfloat16 or float16, got {table.dtype}")
+    if codes.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"codes must have dtype int32 or int64, got {codes.dtype}")
+    if not table.is_cuda or codes.device != table.device:
+        raise ValueError("table and codes must be on the same CUDA device")
+    row = math.prod(table.shape[1:])
+    if row < 1 or row > 1 << 24:
+        raise ValueError(f"table rows must have 1 to {1 << 24} elements, got {row}")
+    if table.shape[0] >= (1 << 31) - 1 or codes.numel() >= (1 << 31) - 4096:
+        raise ValueError("table and codes must have fewer than 2**31 - 4096 rows")
+    if isinstance(scale, torch.Tensor):
+        if scale.dtype != torch.float32 or scale.shape != codes.shape or scale.device != codes.device:
+            raise ValueError("a scale tensor must be float32 with the shape and device of codes")
+    elif not isinstance(scale, Real) or isinstance(scale, bool):
+        raise ValueError("scale must be a number or a float32 tensor")
+
+
+def _args(table, codes, scale, gain) -> _lib.CodebookArgs:
+    a = _lib.CodebookArgs()
+    a.P, a.K, a.D = codes.numel(), table.shape[0], math.prod(table.shape[1:])
+    a.dtype = _lib.DTYPES[table.dtype]
+    a.codes64 = int(codes.dtype == torch.int64)
+    a.scale = scale
+    a.table, a.codes, a.gain = _lib.ptr(table), _lib.ptr(codes), _lib.ptr(gain)
+    a.error_word = _lib.ptr(_pipeline.sticky_error_word(table.device))
+    return a
+
+
+def lookup_forward(table: torch.Tensor, codes: torch.Tensor, scale: float = 1.0,
+                   gain: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``scale * gain * table[codes]`` of contiguous tensors, into ``out`` if given."""
+    if out is None:
+        out = torch.empty(codes.shape + table.shape[1:], dtype=table.dtype, device=table.device)
+    a = _args(table, codes, scale, gain)
+    a.out = _lib.ptr(out)
+    with torch.cuda.device(table.device), _pipeline._stage_timer("codebook_fwd", {"rows": codes.numel(),
+                                                                                  "kernels": 1}):
+        _lib.call("gsb_codebook_fwd", a, _lib.stream_handle(table.device))
+    return out
+
+
+def lookup_backward(table: torch.Tensor, codes: torch.Tensor, scale: float, gain: torch.Tensor | None,
+                    grad_out: torch.Tensor, want_table: bool = True, want_gain: bool = False,
+                    out: torch.Tensor | None = None):
+    """``(grad_table, grad_gain)`` of contiguous tensors; ``grad_table`` into ``out`` if given."""
+    L = _lib.load()
+    a = _args(table, codes, scale, gain)
+    grad_table = grad_gain = None
+    a.grad_out = _lib.ptr(grad_out)
+    if want_table:
+        grad_table = torch.empty_like(table) if out is None else out
+        a.grad_table = _lib.ptr(grad_table)
+        ws_bytes = int(L.gsb_codebook_bwd_workspace_bytes(a.P, a.K, a.D))
+        ws = _pipeline._workspace(ws_bytes, table.device)
+        a.workspace, a.workspace_bytes = _lib.ptr(ws), ws_bytes
+    if want_gain:
+        grad_gain = torch.empty_like(gain)
+        a.grad_gain = _lib.ptr(grad_gain)
+    with torch.cuda.device(table.device), _pipeline._stage_timer("codebook_bwd", {"rows": codes.numel()}):
+        _lib.call("gsb_codebook_bwd", a, _lib.stream_handle(table.device))
+    return grad_table, grad_gain
+
+
+class _CodebookLookup(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, codes, scale, gain):
+        t = table.detach().contiguous()
+        c = codes.contiguous()
+        g = gain.detach().contiguous() if gain is not None else None
+        ctx.scale = scale
+        ctx.save_for_backward(t, c, g)
+        return lookup_forward(t, c, scale, g)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        t, c, g = ctx.saved_tensors
+        want_table, want_gain = ctx.needs_input_grad[0], ctx.needs_input_grad[3]
+        if not (want_table or want_gain):
+            return None, None, None, None
+        grad_table, grad_gain = lookup_backward(t, c, ctx.scale, g, grad.contiguous(), want_table, want_gain)
+        return grad_table, None, None, grad_gain
+
+
+def codebook_lookup(table, codes, scale=1.0):
+    """``scale * table[codes]``: rows of a codebook ``(K, ...)`` (float32, bfloat16 or float16) for ``codes`` of
+    any shape (int32 or int64), of shape ``codes.shape + table.shape[1:]`` and the table's type.
+
+    ``scale`` is a number, or a float32 tensor of ``codes``' shape (one gain per row).  Products are taken in
+    float32 and rounded once.  Code -1 gives a zero row and no gradient; any other code outside ``[0, K)`` does
+    the same and is reported by the device error word (a ``RuntimeError`` at the next call that reads it).
+    Differentiable in ``table`` and in a tensor ``scale``.
+    """
+    _validate(table, codes, scale)
+    gain = scale if isinstance(scale, torch.Tensor) else None
+    return _CodebookLookup.apply(table, codes, 1.0 if gain is not None else float(scale), gain)

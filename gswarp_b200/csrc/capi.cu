@@ -67,6 +67,7 @@ GSB_EXPORT int gsb_block_dim(const char* kernel_class) {
       {"knn_box_dist", KNN},
       {"knn_search", KNN},
       {"adam", ADAM},
+      {"codebook", CODEBOOK},
   };
   if (!kernel_class) return 0;
   for (const Entry& e : table)

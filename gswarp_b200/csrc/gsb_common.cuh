@@ -22,6 +22,8 @@ constexpr int TILE_PIXELS = BLOCK_X * BLOCK_Y;
 // Error bits OR-ed into the device error word.
 constexpr long long ERR_LOOKBACK_TIMEOUT = 1ll << 0;
 constexpr long long ERR_EMIT_MISMATCH = 1ll << 1;
+constexpr long long ERR_BAD_CODE = 1ll << 2;
+constexpr long long ERR_BAD_LABEL = 1ll << 3;
 
 // Bound for every device-side spin (decoupled look-back).  A predecessor
 // tile's CTA is always resident when a successor spins on it (tiles are

@@ -20,6 +20,7 @@ constexpr int SH_BACKWARD_VIEWS = 128;   // sh_backward_views_kernel
 constexpr int SSIM = 256;                // ssim_fwd_kernel, ssim_bwd_kernel (fused H+V passes)
 constexpr int KNN = 256;                 // morton, gather/leaf boxes, box reductions, search (a warp per leaf)
 constexpr int ADAM = 256;                // adam_kernel, densify_stats_kernel
+constexpr int CODEBOOK = 256;            // codebook gather, code keys, segment sums, gain dot products
 
 }  // namespace launch
 }  // namespace gsb

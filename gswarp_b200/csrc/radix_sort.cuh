@@ -14,7 +14,8 @@
 // The caller states how many low key bits are significant: every pass takes
 // 8 of them except the last, which takes what is left (a 13-bit tile id
 // sorts in an 8-bit and a 5-bit pass), and the last pass writes only the
-// values (and the key ranges) -- no caller reads the sorted keys.
+// values (and the key ranges), and the sorted keys for the one caller that
+// reads them (the codebook gradient).
 // Tiles are claimed in launch order, so every tile a CTA waits on belongs to
 // a CTA that is already running; each look-back spin is nevertheless bounded
 // (SPIN_LIMIT) and reports ERR_LOOKBACK_TIMEOUT instead of hanging.
@@ -362,14 +363,14 @@ __host__ inline void launch_pass(int tiles, cudaStream_t stream, const unsigned*
 // ignored).  Buffers ping-pong: pass 0 reads (k[0],v[0]) and writes
 // (k[1],v[1]), pass 1 the reverse, ...  Returns the index (0/1) of the
 // buffer pair that holds the sorted values; the last pass does not write
-// keys, so the sorted keys are not kept.  With n_dev non-null the count is read on
+// keys, so the sorted keys are not kept, unless keep_keys asks for them.  With n_dev non-null the count is read on
 // the device (at most n, which sizes the grids and the scratch).
 // With `ranges` (and n_dev null) the last pass also writes, for every key
 // value below range_keys, its [start, end) in the sorted output into the
 // zero-initialised int2 array `ranges` ((0, 0) for absent keys).
 __host__ inline int sort_pairs(unsigned* k[2], unsigned* v[2], long long n, const int* n_dev, int key_bits,
                                void* scratch, long long* err, cudaStream_t stream, int* ranges = nullptr,
-                               int range_keys = 0) {
+                               int range_keys = 0, bool keep_keys = false) {
   const int passes = passes_for_bits(key_bits);
   if ((n <= 1 && !n_dev) || n <= 0 || passes == 0) return 0;
   const int last_bits = key_bits - RADIX_BITS * (passes - 1);
@@ -385,7 +386,7 @@ __host__ inline int sort_pairs(unsigned* k[2], unsigned* v[2], long long n, cons
     unsigned long long* lb = s.lookback + (size_t)p * tiles * RADIX;
     const bool last = p == passes - 1;
     int* rg = (last && !n_dev) ? ranges : nullptr;
-    unsigned* ko = last ? nullptr : k[cur ^ 1];
+    unsigned* ko = last && !keep_keys ? nullptr : k[cur ^ 1];
     const unsigned* vi = v[cur];
     unsigned* vo = v[cur ^ 1];
     const int bits = last ? last_bits : RADIX_BITS;

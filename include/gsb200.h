@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define GSB_ABI_VERSION 16
+#define GSB_ABI_VERSION 17
 
 #define GSB_OK 0
 #define GSB_ERR_INVALID (-1)  /* bad argument: ValueError in Python          */
@@ -441,6 +441,40 @@ typedef struct {
 
 size_t gsb_knn_workspace_bytes(int P);
 int gsb_knn(const gsb_knn_args* a, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Codebook rows (B200 addition; compressed scenes share attribute rows).    */
+/* out[p] = scale * gain[p] * table[codes[p]], a zero row for code -1; codes */
+/* outside [-1, K) give a zero row and set an error bit.  Backward sums the  */
+/* rows' gradients by code: codes sorted with the library's radix sort, runs */
+/* summed in fp32 in a fixed order (the same bits on every call).            */
+/* ------------------------------------------------------------------------ */
+#define GSB_TYPE_FP32 0
+#define GSB_TYPE_BF16 1
+#define GSB_TYPE_FP16 2
+
+typedef struct {
+  long long P;            /* rows, < 2^31 - 4096 */
+  long long K;            /* codebook rows, < 2^31 - 1 */
+  int D;                  /* elements per row */
+  int dtype;              /* GSB_TYPE_* of table, out, grad_out, grad_table */
+  int codes64;            /* codes are int64 (else int32) */
+  float scale;
+  const void* table;      /* (K,D) contiguous */
+  const void* codes;      /* (P) */
+  const float* gain;      /* (P) or NULL */
+  void* out;              /* forward: (P,D) */
+  const void* grad_out;   /* backward: (P,D) contiguous */
+  void* grad_table;       /* backward: (K,D) or NULL */
+  float* grad_gain;       /* backward: (P) or NULL (needs gain) */
+  long long* error_word;  /* device word */
+  void* workspace;        /* backward, with grad_table */
+  size_t workspace_bytes;
+} gsb_codebook_args;
+
+int gsb_codebook_fwd(const gsb_codebook_args* a, void* stream);
+size_t gsb_codebook_bwd_workspace_bytes(long long P, long long K, int D);
+int gsb_codebook_bwd(const gsb_codebook_args* a, void* stream);
 
 /* Correctly rounded binary32 log of every input (the AccuTile threshold   */
 /* primitive); exported so tests can pin device and host bit for bit.       */
