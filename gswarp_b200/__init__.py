@@ -1,7 +1,8 @@
 """gswarp_b200 -- B200-native (sm_100a) 3DGS training hot path behind
 gswarp's drop-in API: GaussianRasterizationSettings / GaussianRasterizer,
 fused_ssim and distCUDA2; beside them the shared attribute rows of compressed
-scenes (codebook_lookup)."""
+scenes (codebook_lookup) and the class loss of rendered feature maps
+(class_cross_entropy)."""
 
 __version__ = "0.1.0"
 
@@ -27,3 +28,4 @@ from ._runtime import get_tuned_block_dim, register_kernel_class, get_canonical_
 from .fused_ssim import fused_ssim  # noqa: F401
 from .knn import distCUDA2  # noqa: F401
 from .codebook import codebook_lookup  # noqa: F401
+from .class_loss import class_cross_entropy  # noqa: F401

@@ -1,0 +1,188 @@
+"""Class loss of a rendered feature map: ``class_cross_entropy(features, weight, labels, bias)``.
+
+The softmax cross entropy of every pixel's (or row's) label through a linear
+classifier ``z = weight @ f + bias``, as identity and language fields are
+trained: the scene's per-Gaussian features are rendered to a (C,H,W) map and
+each pixel is classified.  The V logits of a pixel are never stored (at
+1920x1080 and 256 classes they would be 2.1 GB): forward streams the classes
+past the pixels with a running maximum and sum, backward recomputes them tile
+by tile and accumulates the gradients of the map, the classifier and its bias.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib, _pipeline
+
+__all__ = ["class_cross_entropy"]
+
+_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+MAX_CHANNELS = 256
+MAX_CHANNELS_FP32 = 128
+TILE = 128
+
+
+def _validate(features, weight, labels, bias, ignore_index, reduction, train) -> None:
+    if not all(isinstance(t, torch.Tensor) for t in (features, weight, labels)):
+        raise ValueError("features, weight and labels must be torch.Tensor instances")
+    if features.ndim not in (2, 3, 4):
+        raise ValueError("features must have shape (N, C), (C, H, W) or (B, C, H, W)")
+    channels = features.shape[0] if features.ndim == 3 else features.shape[1]
+    shape = {2: features.shape[:1], 3: features.shape[1:],
+             4: features.shape[:1] + features.shape[2:]}[features.ndim]
+    if labels.shape != shape:
+        raise ValueError(f"labels must have shape {tuple(shape)}, got {tuple(labels.shape)}")
+    if weight.ndim != 2 or weight.shape[1] != channels or weight.shape[0] < 1:
+        raise ValueError(f"weight must have shape (V, {channels}) with V >= 1, got {tuple(weight.shape)}")
+    if features.dtype not in _lib.DTYPES or weight.dtype != features.dtype:
+        raise ValueError("features and weight must share one dtype of float32, bfloat16 and float16, "
+                         f"got {features.dtype} and {weight.dtype}")
+    if labels.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"labels must have dtype int32 or int64, got {labels.dtype}")
+    limit = MAX_CHANNELS_FP32 if features.dtype == torch.float32 else MAX_CHANNELS
+    if not 1 <= channels <= limit:
+        raise ValueError(f"{features.dtype} features must have 1 to {limit} channels, got {channels}")
+    if labels.numel() >= (1 << 31) - TILE or weight.shape[0] >= (1 << 31) - TILE:
+        raise ValueError("rows and classes must be fewer than 2**31 - 128")
+    if bias is not None:
+        if not isinstance(bias, torch.Tensor) or bias.shape != weight.shape[:1] or bias.dtype != torch.float32:
+            raise ValueError(f"bias must be a float32 tensor of shape ({weight.shape[0]},)")
+    if not features.is_cuda or any(t is not None and t.device != features.device for t in (weight, labels, bias)):
+        raise ValueError("features, weight, labels and bias must be on the same CUDA device")
+    if not isinstance(ignore_index, int) or isinstance(ignore_index, bool):
+        raise ValueError("ignore_index must be an int")
+    if not -(1 << 63) <= ignore_index < 1 << 63:
+        raise ValueError("ignore_index must fit 64 bits")
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction must be one of {tuple(_REDUCTIONS)}, got {reduction!r}")
+    if not isinstance(train, bool):
+        raise ValueError("train must be a bool")
+
+
+def _rows(features):
+    """(B, S, C, strides of b, c and s): rows n = b * S + s of a map or a matrix.  A map whose pixels have
+    no single stride is made contiguous first."""
+    x = features.detach()
+    if x.ndim == 2:
+        x = x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
+        # stride_c = 1 marks rows of channels: the gradient is written (N, C)
+        return x, 1, x.shape[0], x.shape[1], (0, 1, x.stride(0))
+    B, C, H, W = (1, *x.shape) if x.ndim == 3 else x.shape
+    sb, sc, sh, sw = (0, *x.stride()) if x.ndim == 3 else x.stride()
+    if (H > 1 and sh != W * sw) or (sc == 1 and C > 1):
+        x = x.contiguous()
+        sb, sc, sw = C * H * W, H * W, 1
+    return x, B, H * W, C, (sb, max(sc, 2) if C == 1 else sc, sw)
+
+
+def _forward(features, weight, labels, bias, ignore_index, reduction):
+    """``(loss, args, kept)``: the argument block with its sizes, and the tensors backward reads."""
+    x, B, S, C, (sb, sc, ss) = _rows(features)
+    dev = x.device
+    L = _lib.load()
+    N, V = B * S, weight.shape[0]
+
+    def empty(n, dtype):
+        return torch.empty(max(n, 1), dtype=dtype, device=dev)
+
+    def whole_tiles(n):
+        return -(-n // TILE) * TILE
+
+    a = _lib.ClassLossArgs()
+    a.B, a.S, a.V, a.C = B, S, V, C
+    a.dtype, a.reduction = _lib.DTYPES[x.dtype], _REDUCTIONS[reduction]
+    a.labels64 = int(labels.dtype == torch.int64)
+    a.stride_b, a.stride_c, a.stride_s = sb, sc, ss
+    a.ignore_index = ignore_index
+    w = weight.detach().contiguous()
+    b = bias.detach().contiguous() if bias is not None else None
+    y = labels.contiguous()
+    a.features, a.weight, a.bias, a.labels = _lib.ptr(x), _lib.ptr(w), _lib.ptr(b), _lib.ptr(y)
+    kept = (empty(int(L.gsb_class_loss_packed_bytes(N, C, a.dtype)), torch.uint8),
+            empty(int(L.gsb_class_loss_packed_bytes(V, C, a.dtype)), torch.uint8),
+            empty(whole_tiles(V), torch.float32), empty(whole_tiles(N), torch.float32),
+            empty(whole_tiles(N), torch.int32), empty(1, torch.float32))
+    _point_at(a, kept)
+    loss = empty(N if reduction == "none" else 1, torch.float32)
+    a.loss = _lib.ptr(loss)
+    with torch.cuda.device(dev), _pipeline._stage_timer("class_loss_fwd", {"rows": N}):
+        ws = _workspace(a, 0, dev)
+        _lib.call("gsb_class_loss_fwd", a, _lib.stream_handle(dev))
+    del ws
+    return loss[:N].view(labels.shape) if reduction == "none" else loss.view(()), a, kept
+
+
+def _point_at(a, kept) -> None:
+    packed_x, packed_w, bias2, lse2, row_y, inv_count = kept
+    a.packed_x, a.packed_w = _lib.ptr(packed_x), _lib.ptr(packed_w)
+    a.class_bias2, a.row_lse2, a.row_y = _lib.ptr(bias2), _lib.ptr(lse2), _lib.ptr(row_y)
+    a.inv_count = _lib.ptr(inv_count)
+    a.error_word = _lib.ptr(_pipeline.sticky_error_word(packed_x.device))
+
+
+def _workspace(a, backward, device):
+    n = int(_lib.load().gsb_class_loss_workspace_bytes(a, backward))
+    ws = _pipeline._workspace(n, device)
+    a.workspace, a.workspace_bytes = _lib.ptr(ws), n
+    return ws
+
+
+def _backward(args, kept, upstream, features_shape, dtype, want_features, want_weight, want_bias):
+    dev = upstream.device
+    a = _lib.ClassLossArgs.from_buffer_copy(args)
+    a.features = a.weight = a.bias = a.labels = a.loss = None  # not kept, not read
+    _point_at(a, kept)
+    up = upstream.detach().to(torch.float32).reshape(-1).contiguous()
+    a.upstream = _lib.ptr(up)
+    gx = torch.empty(features_shape, dtype=dtype, device=dev) if want_features else None
+    gw = torch.empty((a.V, a.C), dtype=dtype, device=dev) if want_weight else None
+    gb = torch.empty(a.V, dtype=torch.float32, device=dev) if want_bias else None
+    a.grad_features, a.grad_weight, a.grad_bias = _lib.ptr(gx), _lib.ptr(gw), _lib.ptr(gb)
+    with torch.cuda.device(dev), _pipeline._stage_timer("class_loss_bwd", {"rows": a.B * a.S}):
+        ws = _workspace(a, 1, dev)
+        _lib.call("gsb_class_loss_bwd", a, _lib.stream_handle(dev))
+    del ws
+    return gx, gw, gb
+
+
+class _ClassCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, features, weight, labels, bias, ignore_index, reduction, train):
+        loss, args, kept = _forward(features, weight, labels, bias, ignore_index, reduction)
+        ctx.train = train
+        if train:
+            ctx.args, ctx.shape, ctx.dtype = args, features.shape, features.dtype
+            ctx.save_for_backward(*kept)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        want = ctx.needs_input_grad
+        if not ctx.train or not (want[0] or want[1] or want[3]):
+            return (None,) * 7
+        gx, gw, gb = _backward(ctx.args, ctx.saved_tensors, grad, ctx.shape, ctx.dtype, want[0], want[1], want[3])
+        return gx, gw, None, gb, None, None, None
+
+
+def class_cross_entropy(features, weight, labels, bias=None, ignore_index=-100, reduction="mean", train=True):
+    """Softmax cross entropy of ``labels`` under the logits ``weight @ f + bias`` of every pixel or row ``f``.
+
+    ``features`` is a map (C, H, W) or (B, C, H, W), or rows (N, C); ``labels`` (int32 or int64) has its shape
+    without C.  ``weight`` (V, C) shares the features' type: float32 with up to 128 channels, bfloat16 or float16
+    with up to 256.  ``bias`` (V,) is float32.  Logits, softmax and sums are float32 and gradients are rounded
+    once to their input's type; for 16-bit inputs the softmax's probabilities are rounded to bfloat16 (bfloat16
+    inputs) or to 16 bits of precision (float16) before the gradients' products.
+
+    Returns a float32 scalar ("mean" over the rows that count, "sum") or the rows' losses in ``labels``' shape
+    ("none").  Rows labelled ``ignore_index`` have loss 0 and no gradient, whatever their features hold; with no
+    row left the mean is 0.  Labels outside [0, V) count as ignored and are reported by the device error word (a
+    ``RuntimeError`` at the next call that reads it).  A class whose bias is -inf takes no part (its weight row is
+    not read); a row labelled with it has the loss +inf and no gradient.
+
+    With ``train`` the loss is differentiable in ``features``, ``weight`` and ``bias``; the call then keeps a
+    packed copy of the features and the classifier instead of the tensors themselves.
+    """
+    _validate(features, weight, labels, bias, ignore_index, reduction, train)
+    return _ClassCrossEntropy.apply(features, weight, labels, bias, ignore_index, reduction, train)

@@ -68,6 +68,7 @@ GSB_EXPORT int gsb_block_dim(const char* kernel_class) {
       {"knn_search", KNN},
       {"adam", ADAM},
       {"codebook", CODEBOOK},
+      {"class_loss", CLASS_LOSS},
   };
   if (!kernel_class) return 0;
   for (const Entry& e : table)

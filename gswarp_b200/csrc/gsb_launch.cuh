@@ -21,6 +21,7 @@ constexpr int SSIM = 256;                // ssim_fwd_kernel, ssim_bwd_kernel (fu
 constexpr int KNN = 256;                 // morton, gather/leaf boxes, box reductions, search (a warp per leaf)
 constexpr int ADAM = 256;                // adam_kernel, densify_stats_kernel
 constexpr int CODEBOOK = 256;            // codebook gather, code keys, segment sums, gain dot products
+constexpr int CLASS_LOSS = 256;          // class loss: packing, joins, streaming passes
 
 }  // namespace launch
 }  // namespace gsb

@@ -476,6 +476,57 @@ int gsb_codebook_fwd(const gsb_codebook_args* a, void* stream);
 size_t gsb_codebook_bwd_workspace_bytes(long long P, long long K, int D);
 int gsb_codebook_bwd(const gsb_codebook_args* a, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* Class loss (B200 addition): softmax cross entropy of a feature map        */
+/* against a label map through a linear classifier, z = W x + b, with the    */
+/* gradients of the map, the classifier and its bias.  The logits are never  */
+/* stored.  Rows are n = b * S + s, B * S of them; element (n, c) of the     */
+/* features is at b * stride_b + c * stride_c + s * stride_s.  Rows whose    */
+/* label is ignore_index have loss 0 and no gradient, labels outside [0, V)  */
+/* too and set an error bit; a mean divides by the number of the other rows  */
+/* (at least 1).  A class whose bias is -inf takes no part; a row labelled   */
+/* with it has the loss +inf and no gradient.                                */
+/* ------------------------------------------------------------------------ */
+#define GSB_REDUCE_NONE 0
+#define GSB_REDUCE_SUM 1
+#define GSB_REDUCE_MEAN 2
+#define GSB_CLASS_LOSS_MAX_C 256      /* 16-bit features */
+#define GSB_CLASS_LOSS_MAX_C_FP32 128 /* fp32 features */
+
+typedef struct {
+  long long B, S, V;      /* B * S and V < 2^31 - 128 */
+  int C, dtype;           /* channels; GSB_TYPE_* of features, weight and their gradients */
+  int reduction, labels64;
+  long long stride_b, stride_c, stride_s;
+  long long ignore_index;
+  const void* features;
+  const void* weight;     /* (V,C) contiguous */
+  const float* bias;      /* (V) or NULL */
+  const void* labels;     /* (B * S) int64, or int32 if labels64 is 0 */
+  float* loss;            /* 1, or B * S with GSB_REDUCE_NONE */
+  /* kept from forward for backward: */
+  void* packed_x;         /* gsb_class_loss_packed_bytes(B * S, C, dtype), 16-byte aligned */
+  void* packed_w;         /* gsb_class_loss_packed_bytes(V, C, dtype), 16-byte aligned */
+  float* class_bias2;     /* V rounded up to 128 */
+  float* row_lse2;        /* B * S rounded up to 128 */
+  int* row_y;             /* B * S rounded up to 128 */
+  float* inv_count;       /* 1 */
+  /* backward: */
+  const float* upstream;  /* device, like loss */
+  void* grad_features;    /* (B,S,C) if stride_c is 1, else (B,C,S), contiguous; or NULL */
+  void* grad_weight;      /* (V,C) or NULL */
+  float* grad_bias;       /* (V) or NULL */
+  long long* error_word;  /* device word */
+  void* workspace;        /* gsb_class_loss_workspace_bytes() */
+  size_t workspace_bytes;
+} gsb_class_loss_args;
+
+size_t gsb_class_loss_packed_bytes(long long rows, int C, int dtype);
+/* reads the sizes, dtype and reduction of the arguments only */
+size_t gsb_class_loss_workspace_bytes(const gsb_class_loss_args* a, int backward);
+int gsb_class_loss_fwd(const gsb_class_loss_args* a, void* stream);
+int gsb_class_loss_bwd(const gsb_class_loss_args* a, void* stream);
+
 /* Correctly rounded binary32 log of every input (the AccuTile threshold   */
 /* primitive); exported so tests can pin device and host bit for bit.       */
 int gsb_selftest_threshold_log(const float* in, float* out, long long n, void* stream);
