@@ -24,6 +24,7 @@
 #include <algorithm>
 
 #include "gsb_common.cuh"
+#include "gsb_tcgen05.cuh"
 
 namespace gsb {
 namespace {
@@ -135,10 +136,22 @@ __global__ void __launch_bounds__(THREADS) pack_classes_kernel(const gsb_class_l
 }
 
 // ---------------------------------------------------------------------------
-// The streaming pass: a CTA holds 128 rows and walks its range of the other
-// operand's tiles on the fp32 pipes.
+// The streaming pass: one persistent CTA per SM.  A work unit is a resident
+// tile of 128 rows and a range of the streamed operand's tiles of TN rows
+// (columns of z).  Warp 8 loads, warp 9 issues the matrix instructions, two
+// groups of four warps take the tiles of z in turn, and in the gradient
+// passes four more warps store finished accumulators while the next unit
+// runs.  A thread owns one row of z (a lane of tensor memory):
+//   z tile (TMEM) -> registers -> P, rounded to bf16 planes -> TMEM, over z
+//   accumulator (TMEM) += P (TMEM) x streamed tile (shared, as K x channels).
+// The streamed tile is read twice, K-major for z and MN-major for the second
+// product, from one copy: without a swizzle, its 8 x 8 core matrices serve
+// both.
 // ---------------------------------------------------------------------------
 enum { FWD = 0, DX = 1, DW = 2 };
+
+constexpr int MAX_STAGES = 6;
+constexpr int TMEM_COLUMNS = 512;
 
 struct StreamArgs {
   const uint4* a;          // resident operand, packed
@@ -147,133 +160,437 @@ struct StreamArgs {
   const float* lse2;       // rows (DX, DW)
   const int* y;            // rows
   const float* row_u;      // per-row upstream (DW, reduction none) or NULL
-  int a_tiles, b_tiles, splits, planes, D8;
-  float* part_m;           // FWD: [split][row]
+  int a_tiles, b_tiles, splits, D8;
+  int a_slots, stages, acc_slots;
+  float* part_m;           // FWD: [split][group][row]
   float* part_s;
   float* t_label;          // FWD: [row]
   float* part_acc;         // DX, DW: [split][row][D8 * 8]
-  float* part_bias;        // DW: [split][row]
+  float* part_bias;        // DW: [split][group][row]
+  long long* error_word;
 };
 
-__device__ __forceinline__ float plane_sum(const uint4* tile, int planes, int D8, int d8, int row, int k) {
-  float x = 0.f;
-  for (int p = planes - 1; p >= 0; --p) {
-    const __nv_bfloat16* e = reinterpret_cast<const __nv_bfloat16*>(tile + ((size_t)p * D8 + d8) * TILE + row);
-    x += __bfloat162float(e[k]);
-  }
-  return x;
-}
+struct Barriers {
+  uint64_t a_full[2], a_empty[2], b_full[MAX_STAGES], b_empty[MAX_STAGES];
+  uint64_t s_full[2], s_free[2], p_full[2], acc_full[2], acc_empty[2], drained;
+  uint32_t tmem;
+  int stop;
+};
 
 template <int MODE>
-__global__ void __launch_bounds__(THREADS) stream_kernel(const StreamArgs g) {
-  extern __shared__ float smem[];
-  float* sA = smem;                       // [8][TILE]
-  float* sB = sA + 8 * TILE;              // [8][TILE]
-  float* sS = sB + 8 * TILE;              // [TILE][TILE + 1]
-  float* sAcc = sS + TILE * (TILE + 1);   // [TILE][D + 1] (DX, DW)
-  const int D = g.D8 * 8;
-  const int tid = threadIdx.x;
-  const int tile = blockIdx.x, split = blockIdx.y;
-  const size_t tile_u4 = (size_t)g.planes * g.D8 * TILE;
-  const uint4* A = g.a + (size_t)tile * tile_u4;
-  const long long row0 = (long long)tile * TILE;
-  const int lo = (int)((long long)g.b_tiles * split / g.splits), hi = (int)((long long)g.b_tiles * (split + 1) / g.splits);
-  float m = -INFINITY, s = 0.f, bias_sum = 0.f;
-  if (MODE != FWD)
-    for (int i = tid; i < TILE * (D + 1); i += THREADS) sAcc[i] = 0.f;
+__host__ __device__ constexpr int meta_floats(int tn) { return MODE == DW ? 3 * tn : tn; }
+template <int MODE>
+__host__ __device__ constexpr int stream_threads() { return MODE == FWD ? 320 : 448; }
 
-  const int ty = tid / 16, tx = tid % 16;
-  for (int bt = lo; bt < hi; ++bt) {
-    const uint4* Bt = g.b + (size_t)bt * tile_u4;
-    const long long col0 = (long long)bt * TILE;
-    float acc[8][8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) acc[i][j] = 0.f;
-    for (int d8 = 0; d8 < g.D8; ++d8) {
-      __syncthreads();
-      for (int i = tid; i < 8 * TILE; i += THREADS) {
-        sA[i] = plane_sum(A, g.planes, g.D8, d8, i % TILE, i / TILE);
-        sB[i] = plane_sum(Bt, g.planes, g.D8, d8, i % TILE, i / TILE);
-      }
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        float x[8], w[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = sA[k * TILE + ty * 8 + i];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = sB[k * TILE + tx + 16 * j];
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) acc[i][j] += x[i] * w[j];
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) sS[(ty * 8 + i) * (TILE + 1) + tx + 16 * j] = acc[i][j];
-    __syncthreads();
-    if (tid < TILE) {
-      float* srow = sS + tid * (TILE + 1);
-      const long long r = row0 + tid;
-      if (MODE == FWD) {
-        const int y = g.y[r];
-        float mx = m;
-        for (int c = 0; c < TILE; ++c) {
-          const float t = fmaf(srow[c], LOG2E, g.b2[col0 + c]);
-          srow[c] = t;
-          mx = fmaxf(mx, t);
-          if (y == col0 + c) g.t_label[r] = t;
-        }
-        const float base = mx == -INFINITY ? 0.f : mx;
-        float sum = s * ex2(m - base);
-        for (int c = 0; c < TILE; ++c) sum += ex2(srow[c] - base);
-        m = mx;
-        s = sum;
-      } else if (MODE == DX) {
-        const int y = g.y[r];
-        const float l = g.lse2[r];
-        for (int c = 0; c < TILE; ++c) {
-          const float t = fmaf(srow[c], LOG2E, g.b2[col0 + c]);
-          srow[c] = ex2(t - l) - (y == col0 + c ? 1.f : 0.f);
-        }
-      } else {
-        const float b = g.b2[r];
-        for (int c = 0; c < TILE; ++c) {
-          const float t = fmaf(srow[c], LOG2E, b);
-          float p = ex2(t - g.lse2[col0 + c]) - (g.y[col0 + c] == r ? 1.f : 0.f);
-          if (g.row_u) p *= g.row_u[col0 + c];
-          srow[c] = p;
-          bias_sum += p;
-        }
-      }
-    }
-    __syncthreads();
-    if (MODE != FWD) {
-      const int row = tid % TILE;
-      for (int d8 = 0; d8 < g.D8; ++d8)
-        for (int k = tid / TILE; k < 8; k += THREADS / TILE) {
-          float sum = 0.f;
-          for (int c = 0; c < TILE; ++c) sum += sS[row * (TILE + 1) + c] * plane_sum(Bt, g.planes, g.D8, d8, c, k);
-          sAcc[row * (D + 1) + d8 * 8 + k] += sum;
-        }
+// A position in a ring of buffers and the parity of its current round.
+struct Ring {
+  int i = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int n) {
+    if (++i == n) {
+      i = 0;
+      phase ^= 1;
     }
   }
+};
+
+struct Range {
+  int tile, split, lo, hi;
+};
+__device__ __forceinline__ Range unit_range(const StreamArgs& g, int unit) {
+  Range r;
+  r.split = unit / g.a_tiles;
+  r.tile = unit - r.split * g.a_tiles;
+  r.lo = (int)((long long)g.b_tiles * r.split / g.splits);
+  r.hi = (int)((long long)g.b_tiles * (r.split + 1) / g.splits);
+  return r;
+}
+
+// Packed pairs of fp32 (sm_100a issues both halves at once).
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+
+// Products of planes whose sum is the fp32 (fp16) product: from the smallest
+// up; what is left out is below 2^-25 of the product.
+// One hex digit per product, the first one lowest.
+__host__ __device__ constexpr int plane_products(int np) { return np == 3 ? 6 : np == 2 ? 4 : 1; }
+__host__ __device__ constexpr int plane_of_a(int np, int q) {
+  return (np == 3 ? 0x001102 : np == 2 ? 0x0011 : 0) >> (4 * q) & 15;
+}
+__host__ __device__ constexpr int plane_of_b(int np, int q) {
+  return (np == 3 ? 0x010120 : np == 2 ? 0x0101 : 0) >> (4 * q) & 15;
+}
+
+// Splits 32 values into bf16 planes and stores them over z's chunk.
+template <int NP, int TN>
+__device__ __forceinline__ void store_p(uint32_t buffer, int chunk, const float2 (&p)[16]) {
+  float2 rest[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) rest[i] = p[i];
+#pragma unroll
+  for (int k = 0; k < NP; ++k) {
+    uint32_t h[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const __nv_bfloat162 v = __floats2bfloat162_rn(rest[i].x, rest[i].y);
+      h[i] = *reinterpret_cast<const uint32_t*>(&v);
+      if (k + 1 < NP) {
+        const float2 f = make_float2(__uint_as_float(h[i] << 16), __uint_as_float(h[i] & 0xffff0000u));
+        rest[i] = add2(rest[i], make_float2(-f.x, -f.y));
+      }
+    }
+    tc::tmem_store16(buffer + (k < 2 ? 32 * chunk + 16 * k : TN + 16 * chunk), h);
+  }
+}
+
+template <int MODE, int NP, int TN>
+__global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const StreamArgs g) {
+  using namespace tc;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int D8 = g.D8, D = D8 * 8;
+  const uint32_t a_bytes = (uint32_t)NP * D8 * 2048, b_bytes = (uint32_t)NP * D8 * TN * 16;
+  constexpr uint32_t META = (uint32_t)meta_floats<MODE>(TN);
+  uint8_t* const sA = smem;
+  uint8_t* const sB = sA + (size_t)g.a_slots * a_bytes;
+  float* const sMeta = reinterpret_cast<float*>(sB + (size_t)g.stages * b_bytes);
+  Barriers* const bar = reinterpret_cast<Barriers*>(sMeta + (size_t)g.stages * META);
+  volatile int* const stop = &bar->stop;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int units = g.a_tiles * g.splits;
+  constexpr int SBUF = TN * (NP == 3 ? 3 : 2) / 2;  // columns of one z (and P) buffer
+  const int group = warp >> 2;                      // consumer groups 0 and 1
+
+  if (threadIdx.x == 0) {
+    bar->stop = 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar->a_full[i], 1);
+      mbar_init(&bar->a_empty[i], 1);
+      mbar_init(&bar->s_full[i], 1);
+      mbar_init(&bar->s_free[i], MODE == FWD ? 4 : 1);
+      mbar_init(&bar->p_full[i], 4);
+      mbar_init(&bar->acc_full[i], 1);
+      mbar_init(&bar->acc_empty[i], 4);
+    }
+    for (int i = 0; i < MAX_STAGES; ++i) {
+      mbar_init(&bar->b_full[i], 1);
+      mbar_init(&bar->b_empty[i], 1 + 4);  // the last product, and the group's warps (bias, sums, labels)
+    }
+    mbar_init(&bar->drained, 1);
+    mbar_init_fence();
+  }
+  if (warp == 9) tmem_alloc(&bar->tmem, TMEM_COLUMNS);
+  fence_before();
   __syncthreads();
-  const long long rows = (long long)g.a_tiles * TILE;
-  if (MODE == FWD) {
-    if (tid < TILE) {
-      g.part_m[split * rows + row0 + tid] = m;
-      g.part_s[split * rows + row0 + tid] = s;
+  fence_after();
+  const uint32_t tmem = bar->tmem;
+  const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's quarter of the 128 lanes
+
+  if (warp == 8) {
+    // ---- loads ----
+    Ring as, bs;
+    bool ok = true;
+    for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+      const Range r = unit_range(g, u);
+      ok = __all_sync(0xffffffffu, mbar_wait(&bar->a_empty[as.i], as.phase ^ 1, stop));
+      if (!ok) break;
+      if (lane == 0) mbar_expect(&bar->a_full[as.i], a_bytes);
+      __syncwarp();
+      {
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(g.a) + (size_t)r.tile * a_bytes;
+        for (int k = lane; k < NP * D8; k += 32)
+          bulk_load(sA + (size_t)as.i * a_bytes + k * 2048, src + (size_t)k * 2048, 2048, &bar->a_full[as.i]);
+      }
+      as.next(g.a_slots);
+      for (int bt = r.lo; bt < r.hi; ++bt) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&bar->b_empty[bs.i], bs.phase ^ 1, stop));
+        if (!ok) break;
+        uint64_t* full = &bar->b_full[bs.i];
+        const bool with_u = MODE == DW && g.row_u;
+        const uint32_t metas = MODE == DW ? (with_u ? 3 : 2) : 1;
+        if (lane == 0) mbar_expect(full, b_bytes + metas * TN * 4);
+        __syncwarp();
+        const long long col0 = (long long)bt * TN;
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(g.b) + (size_t)(col0 / TILE) * NP * D8 * 2048 +
+                             (size_t)(col0 % TILE) * 16;
+        for (int k = lane; k < NP * D8; k += 32)
+          bulk_load(sB + (size_t)bs.i * b_bytes + (size_t)k * TN * 16, src + (size_t)k * 2048, TN * 16, full);
+        float* meta = sMeta + bs.i * META;
+        if (lane == 0) bulk_load(meta, (MODE == DW ? g.lse2 : g.b2) + col0, TN * 4, full);
+        if (MODE == DW && lane == 1) bulk_load(meta + TN, g.y + col0, TN * 4, full);
+        if (with_u && lane == 2) bulk_load(meta + 2 * TN, g.row_u + col0, TN * 4, full);
+        bs.next(g.stages);
+      }
+    }
+    if (!ok) {
+      // copies still in flight end before the CTA does
+      int never = 0;
+      for (int i = 0; i < g.stages; ++i)
+        mbar_wait(&bar->b_full[i], i < bs.i ? bs.phase : bs.phase ^ 1, &never);
+      for (int i = 0; i < g.a_slots; ++i)
+        mbar_wait(&bar->a_full[i], i < as.i ? as.phase : as.phase ^ 1, &never);
+    }
+  } else if (warp == 9) {
+    // ---- matrix instructions ----
+    if (lane == 0) {
+      const uint32_t idesc1 = instr_desc(TN, false), idesc2 = instr_desc(D, true);
+      const uint32_t a0 = smem_u32(sA), b0 = smem_u32(sB);
+      Ring as, bs, acc;
+      uint32_t t = 0;
+      bool ok = true, pending = false, p_first = false, p_last = false;
+      int p_stage = 0, p_acc = 0;
+      uint32_t p_t = 0, p_acc_phase = 0;
+
+      auto second_product = [&]() {
+        const uint32_t b = p_t & 1;
+        if (!mbar_wait(&bar->p_full[b], (p_t >> 1) & 1, stop)) return false;
+        if (p_first && !mbar_wait(&bar->acc_empty[p_acc], p_acc_phase ^ 1, stop)) return false;
+        fence_after();
+        const uint32_t dst = tmem + 2 * SBUF + p_acc * D;
+        const uint32_t src = b0 + p_stage * b_bytes;
+        bool accumulate = !p_first;
+#pragma unroll
+        for (int q = 0; q < plane_products(NP); ++q)
+#pragma unroll
+          for (int k = 0; k < TN / 16; ++k) {
+            const int pa = plane_of_a(NP, q);
+            const uint32_t a = tmem + b * SBUF + (pa < 2 ? 32 * (k / 2) + 16 * pa : TN + 16 * (k / 2)) + 8 * (k & 1);
+            mma_ts(dst, a, smem_desc(src + plane_of_b(NP, q) * D8 * TN * 16 + k * 256, 128, TN * 16), idesc2, accumulate);
+            accumulate = true;
+          }
+        mma_commit(&bar->b_empty[p_stage]);
+        mma_commit(&bar->s_free[b]);
+        if (p_last) mma_commit(&bar->acc_full[p_acc]);
+        return true;
+      };
+
+      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        const Range r = unit_range(g, u);
+        ok = mbar_wait(&bar->a_full[as.i], as.phase, stop);
+        for (int bt = r.lo; bt < r.hi && ok; ++bt, ++t) {
+          const uint32_t b = t & 1;
+          ok = mbar_wait(&bar->b_full[bs.i], bs.phase, stop) && mbar_wait(&bar->s_free[b], ((t >> 1) & 1) ^ 1, stop);
+          if (!ok) break;
+          fence_after();
+          const uint32_t asrc = a0 + as.i * a_bytes, bsrc = b0 + bs.i * b_bytes;
+          bool accumulate = false;
+#pragma unroll
+          for (int q = 0; q < plane_products(NP); ++q)
+            for (int k = 0; k < D8; k += 2) {
+              mma_ss(tmem + b * SBUF, smem_desc(asrc + (plane_of_a(NP, q) * D8 + k) * 2048, 2048, 128),
+                     smem_desc(bsrc + (plane_of_b(NP, q) * D8 + k) * TN * 16, TN * 16, 128), idesc1, accumulate);
+              accumulate = true;
+            }
+          mma_commit(&bar->s_full[b]);
+          if (bt + 1 == r.hi) mma_commit(&bar->a_empty[as.i]);
+          if (MODE == FWD) {
+            mma_commit(&bar->b_empty[bs.i]);
+          } else {
+            if (pending) ok = second_product();
+            pending = true;
+            p_first = bt == r.lo;
+            p_last = bt + 1 == r.hi;
+            p_stage = bs.i;
+            p_t = t;
+            p_acc = acc.i;
+            p_acc_phase = acc.phase;
+          }
+          bs.next(g.stages);
+        }
+        as.next(g.a_slots);
+        acc.next(g.acc_slots);
+      }
+      if (MODE != FWD && ok && pending) ok = second_product();
+      if (!ok) {
+        // what was issued ends before the tensor memory is freed
+        int never = 0;
+        mma_commit(&bar->drained);
+        mbar_wait(&bar->drained, 0, &never);
+      }
+    }
+    __syncwarp();
+  } else if (warp < 8) {
+    // ---- z -> row statistics, or P ----
+    Ring bs;
+    uint32_t t = 0;
+    bool ok = true;
+    const uint32_t buffer = tmem + lanes + group * SBUF;
+    for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+      const Range r = unit_range(g, u);
+      const int row = r.tile * TILE + (warp & 3) * 32 + lane;
+      int y = 0;
+      float row_c = 0.f;  // -lse2 (DX) or the class's bias (DW)
+      if (MODE != DW) y = g.y[row];
+      if (MODE == DX) row_c = -g.lse2[row];
+      if (MODE == DW) row_c = g.b2[row];
+      float m = -INFINITY, s = 0.f;
+      float2 bias_sum = make_float2(0.f, 0.f);
+      for (int bt = r.lo; bt < r.hi; ++bt, ++t, bs.next(g.stages)) {
+        if ((int)(t & 1) != group) continue;
+        // the meta data comes with the tile that z is made of
+        ok = __all_sync(0xffffffffu, mbar_wait(&bar->b_full[bs.i], bs.phase, stop) &&
+                                         mbar_wait(&bar->s_full[group], (t >> 1) & 1, stop));
+        if (!ok) break;
+        fence_after();
+        const float* meta = sMeta + bs.i * META;
+        const long long col0 = (long long)bt * TN;
+        uint32_t v[2][32];
+        tmem_load32(buffer, v[0]);
+        float2 tile_s[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int c = 0; c < TN / 32; ++c) {
+          uint32_t(&z)[32] = v[c & 1];
+          tmem_load_wait(z);
+          if (c + 1 < TN / 32) tmem_load32(buffer + 32 * (c + 1), v[(c + 1) & 1]);
+          if (MODE == FWD && c + 1 == TN / 32) {
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar->s_free[group]);
+          }
+          float2 x[16];
+          if (MODE == DW) {
+            const float2 l2e = make_float2(LOG2E, LOG2E), cst = make_float2(row_c, row_c);
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              const float4 l = *reinterpret_cast<const float4*>(meta + 32 * c + 2 * i);
+              x[i] = fma2(make_float2(__uint_as_float(z[2 * i]), __uint_as_float(z[2 * i + 1])), l2e, cst);
+              x[i + 1] = fma2(make_float2(__uint_as_float(z[2 * i + 2]), __uint_as_float(z[2 * i + 3])), l2e, cst);
+              x[i] = add2(x[i], make_float2(-l.x, -l.y));
+              x[i + 1] = add2(x[i + 1], make_float2(-l.z, -l.w));
+            }
+          } else {
+            const float2 l2e = make_float2(LOG2E, LOG2E);
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              const float4 b = *reinterpret_cast<const float4*>(meta + 32 * c + 2 * i);
+              x[i] = fma2(make_float2(__uint_as_float(z[2 * i]), __uint_as_float(z[2 * i + 1])), l2e,
+                          make_float2(b.x, b.y));
+              x[i + 1] = fma2(make_float2(__uint_as_float(z[2 * i + 2]), __uint_as_float(z[2 * i + 3])), l2e,
+                              make_float2(b.z, b.w));
+            }
+          }
+          if (MODE == FWD) {
+            const int rel = (int)(y - (col0 + 32 * c));
+            if (__any_sync(0xffffffffu, rel >= 0 && rel < 32 && y >= 0)) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                if (rel == 2 * i) g.t_label[row] = x[i].x;
+                if (rel == 2 * i + 1) g.t_label[row] = x[i].y;
+              }
+            }
+            float cm = fmaxf(x[0].x, x[0].y);
+#pragma unroll
+            for (int i = 1; i < 16; ++i) cm = fmaxf(cm, fmaxf(x[i].x, x[i].y));
+            // The sums' base follows the maximum only when it is left behind by 2^8: fp32 has the range,
+            // and the rescaling is rare.
+            if (cm > m + 8.f) {
+              const float f = ex2(m - cm);
+              s *= f;
+              tile_s[0].x *= f;
+              tile_s[0].y *= f;
+              tile_s[1].x *= f;
+              tile_s[1].y *= f;
+              m = cm;
+            }
+            const float nb = m == -INFINITY ? 0.f : -m;
+            const float2 base = make_float2(nb, nb);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float2 d = add2(x[i], base);
+              tile_s[i & 1] = add2(tile_s[i & 1], make_float2(ex2(d.x), ex2(d.y)));
+            }
+          } else {
+            if (MODE == DX) {
+              const float2 l = make_float2(row_c, row_c);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) x[i] = add2(x[i], l);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = make_float2(ex2(x[i].x), ex2(x[i].y));
+            if (MODE == DX) {
+              const int rel = (int)(y - (col0 + 32 * c));
+              if (__any_sync(0xffffffffu, rel >= 0 && rel < 32 && y >= 0)) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  if (y >= 0 && rel == 2 * i) x[i].x -= 1.f;
+                  if (y >= 0 && rel == 2 * i + 1) x[i].y -= 1.f;
+                }
+              }
+            } else {
+              const int* ym = reinterpret_cast<const int*>(meta + TN) + 32 * c;
+              const int wrow = row - lane;
+              const int yl = ym[lane];
+              if (__any_sync(0xffffffffu, yl >= wrow && yl < wrow + 32)) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  if (ym[2 * i] == row) x[i].x -= 1.f;
+                  if (ym[2 * i + 1] == row) x[i].y -= 1.f;
+                }
+              }
+              if (g.row_u) {
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                  const float4 w = *reinterpret_cast<const float4*>(meta + 2 * TN + 32 * c + 2 * i);
+                  x[i] = make_float2(x[i].x * w.x, x[i].y * w.y);
+                  x[i + 1] = make_float2(x[i + 1].x * w.z, x[i + 1].y * w.w);
+                }
+              }
+#pragma unroll
+              for (int i = 0; i < 16; ++i) tile_s[i & 1] = add2(tile_s[i & 1], x[i]);
+            }
+            store_p<NP, TN>(buffer, c, x);
+          }
+        }
+        if (MODE != FWD) {
+          tmem_store_wait();
+          fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) {
+          if (MODE != FWD) mbar_arrive(&bar->p_full[group]);
+          mbar_arrive(&bar->b_empty[bs.i]);
+        }
+        const float2 ts = add2(tile_s[0], tile_s[1]);
+        if (MODE == FWD) s += ts.x + ts.y;
+        if (MODE == DW) bias_sum = add2(bias_sum, ts);
+      }
+      if (!ok) break;
+      const size_t at = ((size_t)r.split * 2 + group) * ((size_t)g.a_tiles * TILE) + row;
+      if (MODE == FWD) {
+        g.part_m[at] = m;
+        g.part_s[at] = s;
+      }
+      if (MODE == DW) g.part_bias[at] = bias_sum.x + bias_sum.y;
     }
   } else {
-    float* dst = g.part_acc + ((size_t)split * rows + row0) * D;
-    for (int i = tid; i < TILE * D; i += THREADS) dst[i] = sAcc[i / D * (D + 1) + i % D];
-    if (MODE == DW && tid < TILE) g.part_bias[split * rows + row0 + tid] = bias_sum;
+    // ---- finished accumulators ----
+    Ring acc;
+    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+      const Range r = unit_range(g, u);
+      const int row = r.tile * TILE + (warp & 3) * 32 + lane;
+      if (!__all_sync(0xffffffffu, mbar_wait(&bar->acc_full[acc.i], acc.phase, stop))) break;
+      fence_after();
+      float4* dst = reinterpret_cast<float4*>(
+          g.part_acc + ((size_t)r.split * ((size_t)g.a_tiles * TILE) + row) * D);
+      for (int c = 0; c < D; c += 16) {
+        uint32_t v[16];
+        tmem_load16(tmem + lanes + 2 * SBUF + acc.i * D + c, v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          dst[c / 4 + i] = make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]),
+                                       __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
+      }
+      fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar->acc_empty[acc.i]);
+      acc.next(g.acc_slots);
+    }
   }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == 9) tmem_free(tmem, TMEM_COLUMNS);
+  if (threadIdx.x == 0 && *stop)
+    atomicOr((unsigned long long*)g.error_word, (unsigned long long)ERR_LOOKBACK_TIMEOUT);
 }
 
 // ---------------------------------------------------------------------------
@@ -415,14 +732,28 @@ __global__ void __launch_bounds__(THREADS) join_dw_kernel(const gsb_class_loss_a
 constexpr int SMS = 148;
 constexpr int JOIN_BLOCKS = SMS * 4;
 
+// Pieces of the streamed axis: enough work units to fill the SMs.
 inline int split_count(long long a_tiles, long long b_tiles) {
-  const long long want = (SMS + a_tiles - 1) / a_tiles;
-  return (int)std::max(1ll, std::min(want, b_tiles));
+  return (int)std::max(1ll, std::min(SMS / a_tiles, b_tiles));
+}
+
+// Shared memory of a pass.  Above half of an SM's, so that a CTA that holds
+// all tensor memory columns never shares an SM with another one.
+constexpr size_t SMEM_MIN = 118 * 1024, SMEM_MAX = 227 * 1024;
+
+// Columns of a streamed tile: the most of 128, 64 and 32 with which the
+// resident tile and three stages fit.
+inline int tile_columns(int planes, int D8) {
+  for (int tn = 128; tn > 32; tn /= 2)
+    if ((size_t)planes * D8 * (2048 + 3 * tn * 16) + 3 * 3 * tn * 4 + sizeof(Barriers) + 128 <= SMEM_MAX) return tn;
+  return 32;
 }
 
 struct Dims {
-  long long N, x_tiles, w_tiles;
-  int D, D8, planes, v_splits, n_splits;
+  long long N, x_tiles, w_tiles;  // tiles of 128 rows, as packed
+  int D, D8, planes, tn;
+  int x_cols, w_cols;             // tiles of tn rows, as streamed
+  int v_splits, n_splits;
 };
 inline Dims dims_of(const gsb_class_loss_args* a) {
   Dims d;
@@ -432,8 +763,11 @@ inline Dims dims_of(const gsb_class_loss_args* a) {
   d.D = pad_c(a->C);
   d.D8 = d.D / 8;
   d.planes = planes_of(a->dtype);
-  d.v_splits = d.x_tiles > 0 ? split_count(d.x_tiles, d.w_tiles) : 1;
-  d.n_splits = split_count(d.w_tiles, std::max(d.x_tiles, 1ll));
+  d.tn = tile_columns(d.planes, d.D8);
+  d.x_cols = (int)((d.N + d.tn - 1) / d.tn);
+  d.w_cols = (int)((a->V + d.tn - 1) / d.tn);
+  d.v_splits = d.x_tiles > 0 ? split_count(d.x_tiles, d.w_cols) : 1;
+  d.n_splits = split_count(d.w_tiles, std::max(d.x_cols, 1));
   return d;
 }
 
@@ -455,8 +789,8 @@ struct FwdWs {
 inline size_t carve_fwd(void* base, const Dims& d, FwdWs* w) {
   Carver c{(char*)base};
   const size_t rows = (size_t)d.x_tiles * TILE;
-  w->part_m = c.take<float>(rows * d.v_splits);
-  w->part_s = c.take<float>(rows * d.v_splits);
+  w->part_m = c.take<float>(rows * d.v_splits * 2);
+  w->part_s = c.take<float>(rows * d.v_splits * 2);
   w->t_label = c.take<float>(rows);
   w->block_loss = c.take<double>(JOIN_BLOCKS);
   w->block_count = c.take<double>(JOIN_BLOCKS);
@@ -470,7 +804,7 @@ inline size_t carve_bwd(void* base, const Dims& d, BwdWs* w) {
   Carver c{(char*)base};
   w->part_x = c.take<float>((size_t)d.x_tiles * TILE * d.v_splits * d.D);
   w->part_w = c.take<float>((size_t)d.w_tiles * TILE * d.n_splits * d.D);
-  w->part_bias = c.take<float>((size_t)d.w_tiles * TILE * d.n_splits);
+  w->part_bias = c.take<float>((size_t)d.w_tiles * TILE * d.n_splits * 2);
   w->row_u = c.take<float>((size_t)d.x_tiles * TILE);
   return c.off;
 }
@@ -491,8 +825,9 @@ int check_args(const gsb_class_loss_args* a, const char* what) {
     set_error("%s: sizes out of range (B %lld, S %lld, C %d, V %lld)", what, a->B, a->S, a->C, a->V);
     return GSB_ERR_INVALID;
   }
-  if ((uintptr_t)a->packed_x % 16 || (uintptr_t)a->packed_w % 16) {
-    set_error("%s: packed buffers must be 16-byte aligned", what);
+  if ((uintptr_t)a->packed_x % 16 || (uintptr_t)a->packed_w % 16 || (uintptr_t)a->class_bias2 % 16 ||
+      (uintptr_t)a->row_lse2 % 16 || (uintptr_t)a->row_y % 16) {
+    set_error("%s: the buffers kept for backward must be 16-byte aligned", what);
     return GSB_ERR_INVALID;
   }
   if (!a->packed_x || !a->packed_w || !a->class_bias2 || !a->row_lse2 || !a->row_y || !a->inv_count ||
@@ -503,12 +838,35 @@ int check_args(const gsb_class_loss_args* a, const char* what) {
   return GSB_OK;
 }
 
-template <int MODE>
-int launch_stream(const StreamArgs& g, cudaStream_t s) {
-  const size_t smem = (size_t)(16 * TILE + TILE * (TILE + 1) + (MODE == FWD ? 0 : TILE * (g.D8 * 8 + 1))) * 4;
-  cudaFuncSetAttribute(stream_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  stream_kernel<MODE><<<dim3(g.a_tiles, g.splits), THREADS, smem, s>>>(g);
+template <int MODE, int NP, int TN>
+int launch_tiled(StreamArgs g, cudaStream_t s) {
+  const size_t a_bytes = (size_t)NP * g.D8 * 2048;
+  const size_t stage = (size_t)NP * g.D8 * TN * 16 + meta_floats<MODE>(TN) * 4;
+  const size_t fixed = sizeof(Barriers) + 128;
+  constexpr int SBUF = TN * (NP == 3 ? 3 : 2) / 2;
+  g.a_slots = 2 * a_bytes + 3 * stage + fixed <= SMEM_MAX ? 2 : 1;
+  g.stages = (int)std::min<size_t>(MAX_STAGES, (SMEM_MAX - fixed - g.a_slots * a_bytes) / stage);
+  g.acc_slots = 2 * SBUF + 2 * g.D8 * 8 <= TMEM_COLUMNS ? 2 : 1;
+  const size_t smem = std::max(SMEM_MIN, g.a_slots * a_bytes + g.stages * stage + fixed);
+  cudaFuncSetAttribute(stream_kernel<MODE, NP, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  const int units = g.a_tiles * g.splits;
+  stream_kernel<MODE, NP, TN><<<std::min(units, SMS), stream_threads<MODE>(), smem, s>>>(g);
   return check_launch("class loss pass");
+}
+
+template <int MODE>
+int launch_stream(const StreamArgs& g, int planes, int tn, cudaStream_t s) {
+  switch (planes * 1000 + tn) {
+    case 1128: return launch_tiled<MODE, 1, 128>(g, s);
+    case 1064: return launch_tiled<MODE, 1, 64>(g, s);
+    case 2128: return launch_tiled<MODE, 2, 128>(g, s);
+    case 2064: return launch_tiled<MODE, 2, 64>(g, s);
+    case 2032: return launch_tiled<MODE, 2, 32>(g, s);
+    case 3128: return launch_tiled<MODE, 3, 128>(g, s);
+    case 3064: return launch_tiled<MODE, 3, 64>(g, s);
+    case 3032: return launch_tiled<MODE, 3, 32>(g, s);
+    default: set_error("class loss: no pass for %d planes and tiles of %d", planes, tn); return GSB_ERR_INVALID;
+  }
 }
 
 inline int blocks_for(long long n) { return (int)std::max(1ll, std::min((n + THREADS - 1) / THREADS, (long long)SMS * 16)); }
@@ -553,9 +911,9 @@ GSB_EXPORT int gsb_class_loss_fwd(const gsb_class_loss_args* a, void* stream) {
   g.b2 = a->class_bias2;
   g.y = a->row_y;
   g.a_tiles = (int)d.x_tiles;
-  g.b_tiles = (int)d.w_tiles;
+  g.b_tiles = d.w_cols;
   g.splits = d.v_splits;
-  g.planes = d.planes;
+  g.error_word = a->error_word;
   g.D8 = d.D8;
   g.part_m = w.part_m;
   g.part_s = w.part_s;
@@ -564,11 +922,11 @@ GSB_EXPORT int gsb_class_loss_fwd(const gsb_class_loss_args* a, void* stream) {
   pack_classes_kernel<<<blocks_for(w_total), THREADS, 0, s>>>(*a, d.D8, w_total, (uint4*)a->packed_w, a->class_bias2);
   if (d.N > 0) {
     pack_rows_kernel<<<blocks_for(x_total), THREADS, 0, s>>>(*a, d.D8, x_total, (uint4*)a->packed_x, a->row_y);
-    const int r = launch_stream<FWD>(g, s);
+    const int r = launch_stream<FWD>(g, d.planes, d.tn, s);
     if (r != GSB_OK) return r;
   }
   const int blocks = (int)std::max(1ll, std::min<long long>(JOIN_BLOCKS, (d.x_tiles * TILE + THREADS - 1) / THREADS));
-  join_rows_kernel<<<blocks, THREADS, 0, s>>>(g, d.v_splits, d.N, a->row_lse2, a->row_y,
+  join_rows_kernel<<<blocks, THREADS, 0, s>>>(g, 2 * d.v_splits, d.N, a->row_lse2, a->row_y,
                                               a->reduction == GSB_REDUCE_NONE ? a->loss : nullptr, w.block_loss,
                                               w.block_count);
   finish_loss_kernel<<<1, THREADS, 0, s>>>(w.block_loss, w.block_count, blocks, a->reduction, a->loss, a->inv_count);
@@ -600,16 +958,16 @@ GSB_EXPORT int gsb_class_loss_bwd(const gsb_class_loss_args* a, void* stream) {
   g.b2 = a->class_bias2;
   g.lse2 = a->row_lse2;
   g.y = a->row_y;
-  g.planes = d.planes;
+  g.error_word = a->error_word;
   g.D8 = d.D8;
   if (a->grad_features) {
     g.a = (const uint4*)a->packed_x;
     g.b = (const uint4*)a->packed_w;
     g.a_tiles = (int)d.x_tiles;
-    g.b_tiles = (int)d.w_tiles;
+    g.b_tiles = d.w_cols;
     g.splits = d.v_splits;
     g.part_acc = w.part_x;
-    const int r = launch_stream<DX>(g, s);
+    const int r = launch_stream<DX>(g, d.planes, d.tn, s);
     if (r != GSB_OK) return r;
     join_dx_kernel<<<blocks_for(d.N * a->C), THREADS, 0, s>>>(*a, w.part_x, d.v_splits, d.D, d.x_tiles * TILE);
   }
@@ -617,7 +975,7 @@ GSB_EXPORT int gsb_class_loss_bwd(const gsb_class_loss_args* a, void* stream) {
     g.a = (const uint4*)a->packed_w;
     g.b = (const uint4*)a->packed_x;
     g.a_tiles = (int)d.w_tiles;
-    g.b_tiles = (int)d.x_tiles;
+    g.b_tiles = d.x_cols;
     g.splits = d.n_splits;
     g.part_acc = w.part_w;
     g.part_bias = w.part_bias;
@@ -625,10 +983,10 @@ GSB_EXPORT int gsb_class_loss_bwd(const gsb_class_loss_args* a, void* stream) {
       row_upstream_kernel<<<blocks_for(d.x_tiles * TILE), THREADS, 0, s>>>(a->upstream, a->row_y, d.x_tiles * TILE, w.row_u);
       g.row_u = w.row_u;
     }
-    const int r = launch_stream<DW>(g, s);
+    const int r = launch_stream<DW>(g, d.planes, d.tn, s);
     if (r != GSB_OK) return r;
     join_dw_kernel<<<blocks_for(a->V * (a->C + 1ll)), THREADS, 0, s>>>(*a, w.part_w, w.part_bias, d.n_splits,
-                                                                      d.n_splits, d.D, d.w_tiles * TILE);
+                                                                      2 * d.n_splits, d.D, d.w_tiles * TILE);
   }
   return check_launch("gsb_class_loss_bwd");
 }

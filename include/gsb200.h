@@ -504,9 +504,9 @@ typedef struct {
   const float* bias;      /* (V) or NULL */
   const void* labels;     /* (B * S) int64, or int32 if labels64 is 0 */
   float* loss;            /* 1, or B * S with GSB_REDUCE_NONE */
-  /* kept from forward for backward: */
-  void* packed_x;         /* gsb_class_loss_packed_bytes(B * S, C, dtype), 16-byte aligned */
-  void* packed_w;         /* gsb_class_loss_packed_bytes(V, C, dtype), 16-byte aligned */
+  /* kept from forward for backward, each 16-byte aligned: */
+  void* packed_x;         /* gsb_class_loss_packed_bytes(B * S, C, dtype) */
+  void* packed_w;         /* gsb_class_loss_packed_bytes(V, C, dtype) */
   float* class_bias2;     /* V rounded up to 128 */
   float* row_lse2;        /* B * S rounded up to 128 */
   int* row_y;             /* B * S rounded up to 128 */

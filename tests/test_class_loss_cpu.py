@@ -87,7 +87,7 @@ def _args(**kw):
                                 dict(C=257, dtype=1), dict(dtype=3), dict(reduction=3), dict(packed_x=None),
                                 dict(packed_w=None), dict(row_y=None), dict(inv_count=None), dict(workspace=None),
                                 dict(error_word=None), dict(workspace_bytes=0), dict(packed_x=264),
-                                dict(packed_w=264)])
+                                dict(packed_w=264), dict(class_bias2=260), dict(row_lse2=264), dict(row_y=252)])
 def test_c_abi_refuses(kw):
     L = _lib.load()
     for fn in (L.gsb_class_loss_fwd, L.gsb_class_loss_bwd):
