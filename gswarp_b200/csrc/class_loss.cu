@@ -162,10 +162,11 @@ struct StreamArgs {
   const float* row_u;      // per-row upstream (DW, reduction none) or NULL
   int a_tiles, b_tiles, splits, D8;
   int a_slots, stages, acc_slots;
+  int flush;               // tiles per accumulator
   float* part_m;           // FWD: [split][group][row]
   float* part_s;
   float* t_label;          // FWD: [row]
-  float* part_acc;         // DX, DW: [split][row][D8 * 8]
+  float* part_acc;         // DX, DW: [split][tile][column / 4][row][4 columns]
   float* part_bias;        // DW: [split][group][row]
   long long* error_word;
 };
@@ -176,6 +177,22 @@ struct Barriers {
   uint32_t tmem;
   int stop;
 };
+
+// Tensor memory: two buffers of z, over which P is written (two planes fit
+// its 32-bit columns, the third has its own), then the accumulators.
+__host__ __device__ constexpr int z_columns(int np, int tn) { return tn * (np == 3 ? 3 : 2) / 2; }
+
+// The matrix instructions truncate when they add to an accumulator, half an
+// ulp of the running sum on average, always towards zero, so a long chain is
+// off by its length times 2^-25 (measured: 6.5e-5 of dW after 10,000
+// additions).  Accumulators are therefore taken out after a bounded number of
+// additions and added up with rounding.  fp32 features: 16 additions of the
+// leading planes' product; the other five products, 2^-8 of it and less, have
+// an accumulator of their own, so that they do not lengthen the chain (5e-7).
+// fp16 (four products): 256 additions, 8e-6; bf16: 512, 1.5e-5; both far below
+// the half step of the gradients' type.
+__host__ __device__ constexpr int accumulators(int np) { return np == 3 ? 2 : 1; }
+__host__ __device__ constexpr int chain_products(int np) { return np == 3 ? 16 : np == 2 ? 64 : 512; }
 
 template <int MODE>
 __host__ __device__ constexpr int meta_floats(int tn) { return MODE == DW ? 3 * tn : tn; }
@@ -257,7 +274,8 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
   volatile int* const stop = &bar->stop;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int units = g.a_tiles * g.splits;
-  constexpr int SBUF = TN * (NP == 3 ? 3 : 2) / 2;  // columns of one z (and P) buffer
+  constexpr int SBUF = z_columns(NP, TN);
+  constexpr int ACCS = accumulators(NP);
   const int group = warp >> 2;                      // consumer groups 0 and 1
 
   if (threadIdx.x == 0) {
@@ -345,17 +363,18 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
         if (!mbar_wait(&bar->p_full[b], (p_t >> 1) & 1, stop)) return false;
         if (p_first && !mbar_wait(&bar->acc_empty[p_acc], p_acc_phase ^ 1, stop)) return false;
         fence_after();
-        const uint32_t dst = tmem + 2 * SBUF + p_acc * D;
+        const uint32_t dst = tmem + 2 * SBUF + p_acc * ACCS * D;
         const uint32_t src = b0 + p_stage * b_bytes;
-        bool accumulate = !p_first;
 #pragma unroll
         for (int q = 0; q < plane_products(NP); ++q)
 #pragma unroll
           for (int k = 0; k < TN / 16; ++k) {
             const int pa = plane_of_a(NP, q);
+            const bool main = q + 1 == plane_products(NP);
             const uint32_t a = tmem + b * SBUF + (pa < 2 ? 32 * (k / 2) + 16 * pa : TN + 16 * (k / 2)) + 8 * (k & 1);
-            mma_ts(dst, a, smem_desc(src + plane_of_b(NP, q) * D8 * TN * 16 + k * 256, 128, TN * 16), idesc2, accumulate);
-            accumulate = true;
+            mma_ts(ACCS == 2 && !main ? dst + D : dst, a,
+                   smem_desc(src + plane_of_b(NP, q) * D8 * TN * 16 + k * 256, 128, TN * 16), idesc2,
+                   !p_first || k > 0 || (ACCS == 2 && main ? false : q > 0));
           }
         mma_commit(&bar->b_empty[p_stage]);
         mma_commit(&bar->s_free[b]);
@@ -387,17 +406,18 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
           } else {
             if (pending) ok = second_product();
             pending = true;
-            p_first = bt == r.lo;
-            p_last = bt + 1 == r.hi;
+            const int in_acc = (bt - r.lo) % g.flush;
+            p_first = in_acc == 0;
+            p_last = in_acc + 1 == g.flush || bt + 1 == r.hi;
             p_stage = bs.i;
             p_t = t;
             p_acc = acc.i;
             p_acc_phase = acc.phase;
+            if (p_last) acc.next(g.acc_slots);
           }
           bs.next(g.stages);
         }
         as.next(g.a_slots);
-        acc.next(g.acc_slots);
       }
       if (MODE != FWD && ok && pending) ok = second_product();
       if (!ok) {
@@ -561,28 +581,56 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
       }
       if (MODE == DW) g.part_bias[at] = bias_sum.x + bias_sum.y;
     }
-  } else {
-    // ---- finished accumulators ----
+  } else if (MODE != FWD) {
+    // ---- finished accumulators: added up in fp32 in the unit's partial rows ----
     Ring acc;
-    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+    bool ok = true;
+    for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
       const Range r = unit_range(g, u);
-      const int row = r.tile * TILE + (warp & 3) * 32 + lane;
-      if (!__all_sync(0xffffffffu, mbar_wait(&bar->acc_full[acc.i], acc.phase, stop))) break;
-      fence_after();
-      float4* dst = reinterpret_cast<float4*>(
-          g.part_acc + ((size_t)r.split * ((size_t)g.a_tiles * TILE) + row) * D);
-      for (int c = 0; c < D; c += 16) {
-        uint32_t v[16];
-        tmem_load16(tmem + lanes + 2 * SBUF + acc.i * D + c, v);
+      const size_t tile = (size_t)r.split * g.a_tiles + r.tile;
+      float4* const dst = reinterpret_cast<float4*>(g.part_acc) + tile * (D / 4) * TILE + (warp & 3) * 32 + lane;
+      for (int bt = r.lo; bt < r.hi; bt += g.flush) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&bar->acc_full[acc.i], acc.phase, stop));
+        if (!ok) break;
+        fence_after();
+        const uint32_t src = tmem + lanes + 2 * SBUF + acc.i * ACCS * D;
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          float4 v[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          dst[c / 4 + i] = make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]),
-                                       __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
+          for (int c = 0; c < 2; ++c) {
+            if (c0 + 16 * c >= D) break;
+            uint32_t main[16], rest[16];
+            tmem_load16(src + c0 + 16 * c, main);
+            if (ACCS == 2) tmem_load16(src + D + c0 + 16 * c, rest);
+            float x[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              x[i] = __uint_as_float(main[i]) + (ACCS == 2 ? __uint_as_float(rest[i]) : 0.f);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[4 * c + i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+          }
+          if (c0 + 32 >= D) {
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar->acc_empty[acc.i]);
+          }
+          float4* at = dst + (size_t)(c0 / 4) * TILE;
+          if (bt > r.lo) {
+            float4 old[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (c0 + 4 * i < D) old[i] = at[(size_t)i * TILE];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (c0 + 4 * i < D)
+                v[i] = make_float4(old[i].x + v[i].x, old[i].y + v[i].y, old[i].z + v[i].z, old[i].w + v[i].w);
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (c0 + 4 * i < D) at[(size_t)i * TILE] = v[i];
+        }
+        acc.next(g.acc_slots);
       }
-      fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar->acc_empty[acc.i]);
-      acc.next(g.acc_slots);
     }
   }
   fence_before();
@@ -678,6 +726,12 @@ __global__ void __launch_bounds__(THREADS) row_upstream_kernel(const float* __re
     out[n] = row_y[n] >= 0 ? up[n] : 0.f;
 }
 
+// Where the streaming passes leave column c of row n of a split.
+__device__ __forceinline__ size_t part_index(int split, long long rows, long long n, int c, int D) {
+  const size_t tile = (size_t)split * (rows / TILE) + n / TILE;
+  return ((tile * (D / 4) + c / 4) * TILE + n % TILE) * 4 + c % 4;
+}
+
 // Sums the splits of dX in order, scales, and writes the features' layout.
 __global__ void __launch_bounds__(THREADS) join_dx_kernel(const gsb_class_loss_args a, const float* __restrict__ part,
                                                           int splits, int D, long long rows) {
@@ -696,7 +750,7 @@ __global__ void __launch_bounds__(THREADS) join_dx_kernel(const gsb_class_loss_a
       n = b * a.S + (r - c * a.S);
     }
     float v = 0.f;
-    for (int k = 0; k < splits; ++k) v += part[((size_t)k * rows + n) * D + c];
+    for (int k = 0; k < splits; ++k) v += part[part_index(k, rows, n, c, D)];
     const float u = a.reduction == GSB_REDUCE_NONE ? a.upstream[n] : a.upstream[0] * a.inv_count[0];
     const long long b = n / a.S;
     // rows without a gradient stay exactly zero whatever upstream holds
@@ -717,7 +771,7 @@ __global__ void __launch_bounds__(THREADS) join_dw_kernel(const gsb_class_loss_a
     float sum = 0.f;
     if (c < a.C) {
       if (!a.grad_weight) continue;
-      for (int k = 0; k < splits; ++k) sum += part[((size_t)k * rows + v) * D + c];
+      for (int k = 0; k < splits; ++k) sum += part[part_index(k, rows, v, c, D)];
       store_elem(a.grad_weight, v * a.C + c, a.dtype, sum * u);
     } else if (a.grad_bias) {
       for (int k = 0; k < slots; ++k) sum += part_bias[k * rows + v];
@@ -843,10 +897,11 @@ int launch_tiled(StreamArgs g, cudaStream_t s) {
   const size_t a_bytes = (size_t)NP * g.D8 * 2048;
   const size_t stage = (size_t)NP * g.D8 * TN * 16 + meta_floats<MODE>(TN) * 4;
   const size_t fixed = sizeof(Barriers) + 128;
-  constexpr int SBUF = TN * (NP == 3 ? 3 : 2) / 2;
+  constexpr int SBUF = z_columns(NP, TN), ACCS = accumulators(NP);
+  g.flush = chain_products(NP) / (TN / 16);
   g.a_slots = 2 * a_bytes + 3 * stage + fixed <= SMEM_MAX ? 2 : 1;
   g.stages = (int)std::min<size_t>(MAX_STAGES, (SMEM_MAX - fixed - g.a_slots * a_bytes) / stage);
-  g.acc_slots = 2 * SBUF + 2 * g.D8 * 8 <= TMEM_COLUMNS ? 2 : 1;
+  g.acc_slots = 2 * SBUF + 2 * ACCS * g.D8 * 8 <= TMEM_COLUMNS ? 2 : 1;
   const size_t smem = std::max(SMEM_MIN, g.a_slots * a_bytes + g.stages * stage + fixed);
   cudaFuncSetAttribute(stream_kernel<MODE, NP, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   const int units = g.a_tiles * g.splits;
