@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(THREADS) pack_classes_kernel(const gsb_class_l
 // ---------------------------------------------------------------------------
 enum { FWD = 0, DX = 1, DW = 2 };
 
-constexpr int MAX_STAGES = 6;
+constexpr int MAX_STAGES = 16, MAX_A_SLOTS = 4;
 constexpr int TMEM_COLUMNS = 512;
 
 struct StreamArgs {
@@ -161,7 +161,7 @@ struct StreamArgs {
   const int* y;            // rows
   const float* row_u;      // per-row upstream (DW, reduction none) or NULL
   int a_tiles, b_tiles, splits, D8;
-  int a_slots, stages, acc_slots;
+  int a_slots, stages, acc_slots, z_shift;  // z_shift: log2 of the number of z buffers
   int flush;               // tiles per accumulator
   float* part_m;           // FWD: [split][group][row]
   float* part_s;
@@ -172,15 +172,18 @@ struct StreamArgs {
 };
 
 struct Barriers {
-  uint64_t a_full[2], a_empty[2], b_full[MAX_STAGES], b_empty[MAX_STAGES];
-  uint64_t s_full[2], s_free[2], p_full[2], acc_full[2], acc_empty[2], drained;
+  uint64_t a_full[MAX_A_SLOTS], a_empty[MAX_A_SLOTS], b_full[MAX_STAGES], b_empty[MAX_STAGES];
+  uint64_t s_full[4], s_free[4], p_full[4], acc_full[2], acc_empty[2], drained;
   uint32_t tmem;
   int stop;
 };
 
 // Tensor memory: two buffers of z, over which P is written (two planes fit
 // its 32-bit columns, the third has its own), then the accumulators.
-__host__ __device__ constexpr int z_columns(int np, int tn) { return tn * (np == 3 ? 3 : 2) / 2; }
+template <int MODE>
+__host__ __device__ constexpr int z_columns(int np, int tn) {
+  return MODE == FWD ? tn : tn * (np == 3 ? 3 : 2) / 2;
+}
 
 // The matrix instructions truncate when they add to an accumulator, half an
 // ulp of the running sum on average, always towards zero, so a long chain is
@@ -222,6 +225,31 @@ __device__ __forceinline__ Range unit_range(const StreamArgs& g, int unit) {
   r.hi = (int)((long long)g.b_tiles * (r.split + 1) / g.splits);
   return r;
 }
+
+// Walks a CTA's units tile by tile, with the rings that go along.
+struct Cursor {
+  int unit, bt;
+  Range r;
+  Ring as, bs, acc;
+  uint32_t t = 0;
+  __device__ __forceinline__ explicit Cursor(const StreamArgs& g) : unit(blockIdx.x) {
+    if (unit < g.a_tiles * g.splits) {
+      r = unit_range(g, unit);
+      bt = r.lo;
+    }
+  }
+  __device__ __forceinline__ void next(const StreamArgs& g) {
+    ++t;
+    bs.next(g.stages);
+    if (++bt < r.hi) return;
+    as.next(g.a_slots);
+    unit += gridDim.x;
+    if (unit < g.a_tiles * g.splits) {
+      r = unit_range(g, unit);
+      bt = r.lo;
+    }
+  }
+};
 
 // Packed pairs of fp32 (sm_100a issues both halves at once).
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
@@ -274,20 +302,26 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
   volatile int* const stop = &bar->stop;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int units = g.a_tiles * g.splits;
-  constexpr int SBUF = z_columns(NP, TN);
+  constexpr int SBUF = z_columns<MODE>(NP, TN);
   constexpr int ACCS = accumulators(NP);
+  const uint32_t z_mask = (1u << g.z_shift) - 1;
+  const uint32_t ACC0 = SBUF << g.z_shift;          // first accumulator column
   const int group = warp >> 2;                      // consumer groups 0 and 1
 
   if (threadIdx.x == 0) {
     bar->stop = 0;
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < MAX_A_SLOTS; ++i) {
       mbar_init(&bar->a_full[i], 1);
       mbar_init(&bar->a_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar->acc_full[i], 1);
+      mbar_init(&bar->acc_empty[i], 4);
+    }
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&bar->s_full[i], 1);
       mbar_init(&bar->s_free[i], MODE == FWD ? 4 : 1);
       mbar_init(&bar->p_full[i], 4);
-      mbar_init(&bar->acc_full[i], 1);
-      mbar_init(&bar->acc_empty[i], 4);
     }
     for (int i = 0; i < MAX_STAGES; ++i) {
       mbar_init(&bar->b_full[i], 1);
@@ -351,75 +385,75 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
     // ---- matrix instructions ----
     if (lane == 0) {
       const uint32_t idesc1 = instr_desc(TN, false), idesc2 = instr_desc(D, true);
+      const uint32_t hi1 = desc_hi(128), hi2 = desc_hi(TN * 16);
       const uint32_t a0 = smem_u32(sA), b0 = smem_u32(sB);
-      Ring as, bs, acc;
-      uint32_t t = 0;
-      bool ok = true, pending = false, p_first = false, p_last = false;
-      int p_stage = 0, p_acc = 0;
-      uint32_t p_t = 0, p_acc_phase = 0;
+      bool ok = true;
 
-      auto second_product = [&]() {
-        const uint32_t b = p_t & 1;
-        if (!mbar_wait(&bar->p_full[b], (p_t >> 1) & 1, stop)) return false;
-        if (p_first && !mbar_wait(&bar->acc_empty[p_acc], p_acc_phase ^ 1, stop)) return false;
+      auto first_product = [&](Cursor& c) {
+        const uint32_t b = c.t & z_mask;
+        if (c.bt == c.r.lo && !mbar_wait(&bar->a_full[c.as.i], c.as.phase, stop)) return false;
+        if (!mbar_wait(&bar->b_full[c.bs.i], c.bs.phase, stop)) return false;
+        if (!mbar_wait(&bar->s_free[b], ((c.t >> g.z_shift) & 1) ^ 1, stop)) return false;
         fence_after();
-        const uint32_t dst = tmem + 2 * SBUF + p_acc * ACCS * D;
-        const uint32_t src = b0 + p_stage * b_bytes;
+        const uint32_t a_lo = desc_lo(a0 + c.as.i * a_bytes, 2048), b_lo = desc_lo(b0 + c.bs.i * b_bytes, TN * 16);
+        const uint32_t z = tmem + b * SBUF;
 #pragma unroll
-        for (int q = 0; q < plane_products(NP); ++q)
-#pragma unroll
-          for (int k = 0; k < TN / 16; ++k) {
-            const int pa = plane_of_a(NP, q);
-            const bool main = q + 1 == plane_products(NP);
-            const uint32_t a = tmem + b * SBUF + (pa < 2 ? 32 * (k / 2) + 16 * pa : TN + 16 * (k / 2)) + 8 * (k & 1);
-            mma_ts(ACCS == 2 && !main ? dst + D : dst, a,
-                   smem_desc(src + plane_of_b(NP, q) * D8 * TN * 16 + k * 256, 128, TN * 16), idesc2,
-                   !p_first || k > 0 || (ACCS == 2 && main ? false : q > 0));
-          }
-        mma_commit(&bar->b_empty[p_stage]);
-        mma_commit(&bar->s_free[b]);
-        if (p_last) mma_commit(&bar->acc_full[p_acc]);
+        for (int q = 0; q < plane_products(NP); ++q) {
+          const uint32_t aq = a_lo + plane_of_a(NP, q) * D8 * 128, bq = b_lo + plane_of_b(NP, q) * D8 * TN;
+          mma_ss(z, aq, hi1, bq, hi1, idesc1, q > 0);
+#pragma unroll 4
+          for (int k = 2; k < D8; k += 2) mma_ss(z, aq + k * 128, hi1, bq + k * TN, hi1, idesc1, true);
+        }
+        mma_commit(&bar->s_full[b]);
+        if (c.bt + 1 == c.r.hi) mma_commit(&bar->a_empty[c.as.i]);
+        if (MODE == FWD) mma_commit(&bar->b_empty[c.bs.i]);
         return true;
       };
 
-      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
-        const Range r = unit_range(g, u);
-        ok = mbar_wait(&bar->a_full[as.i], as.phase, stop);
-        for (int bt = r.lo; bt < r.hi && ok; ++bt, ++t) {
-          const uint32_t b = t & 1;
-          ok = mbar_wait(&bar->b_full[bs.i], bs.phase, stop) && mbar_wait(&bar->s_free[b], ((t >> 1) & 1) ^ 1, stop);
-          if (!ok) break;
-          fence_after();
-          const uint32_t asrc = a0 + as.i * a_bytes, bsrc = b0 + bs.i * b_bytes;
-          bool accumulate = false;
+      auto second_product = [&](Cursor& c) {
+        const uint32_t b = c.t & z_mask;
+        const int in_acc = (c.bt - c.r.lo) % g.flush;
+        const bool first = in_acc == 0, last = in_acc + 1 == g.flush || c.bt + 1 == c.r.hi;
+        if (!mbar_wait(&bar->p_full[b], (c.t >> g.z_shift) & 1, stop)) return false;
+        if (first && !mbar_wait(&bar->acc_empty[c.acc.i], c.acc.phase ^ 1, stop)) return false;
+        fence_after();
+        const uint32_t dst = tmem + ACC0 + c.acc.i * ACCS * D, p = tmem + b * SBUF;
+        const uint32_t b_lo = desc_lo(b0 + c.bs.i * b_bytes, 128);
 #pragma unroll
-          for (int q = 0; q < plane_products(NP); ++q)
-            for (int k = 0; k < D8; k += 2) {
-              mma_ss(tmem + b * SBUF, smem_desc(asrc + (plane_of_a(NP, q) * D8 + k) * 2048, 2048, 128),
-                     smem_desc(bsrc + (plane_of_b(NP, q) * D8 + k) * TN * 16, TN * 16, 128), idesc1, accumulate);
-              accumulate = true;
-            }
-          mma_commit(&bar->s_full[b]);
-          if (bt + 1 == r.hi) mma_commit(&bar->a_empty[as.i]);
-          if (MODE == FWD) {
-            mma_commit(&bar->b_empty[bs.i]);
-          } else {
-            if (pending) ok = second_product();
-            pending = true;
-            const int in_acc = (bt - r.lo) % g.flush;
-            p_first = in_acc == 0;
-            p_last = in_acc + 1 == g.flush || bt + 1 == r.hi;
-            p_stage = bs.i;
-            p_t = t;
-            p_acc = acc.i;
-            p_acc_phase = acc.phase;
-            if (p_last) acc.next(g.acc_slots);
-          }
-          bs.next(g.stages);
+        for (int q = 0; q < plane_products(NP); ++q) {
+          const int pa = plane_of_a(NP, q);
+          const bool main = q + 1 == plane_products(NP);
+          const uint32_t to = ACCS == 2 && !main ? dst + D : dst;
+          const uint32_t bq = b_lo + plane_of_b(NP, q) * D8 * TN;
+#pragma unroll
+          for (int k = 0; k < TN / 16; ++k)
+            mma_ts(to, p + (pa < 2 ? 32 * (k / 2) + 16 * pa : TN + 16 * (k / 2)) + 8 * (k & 1), bq + k * 16, hi2,
+                   idesc2, k > 0 || (q > 0 && !(ACCS == 2 && main)) || !first);
         }
-        as.next(g.a_slots);
+        mma_commit(&bar->b_empty[c.bs.i]);
+        mma_commit(&bar->s_free[b]);
+        if (last) {
+          mma_commit(&bar->acc_full[c.acc.i]);
+          c.acc.next(g.acc_slots);
+        }
+        return true;
+      };
+
+      // The second product follows the first at a distance: with four z
+      // buffers a group finds its next tile ready while P of its last one
+      // still waits for its product.
+      Cursor c1(g), c2(g);
+      const uint32_t distance = 1u << (g.z_shift - 1);
+      while (ok && c1.unit < units) {
+        ok = first_product(c1);
+        c1.next(g);
+        if (MODE != FWD && ok && c1.t > distance) {
+          ok = second_product(c2);
+          c2.next(g);
+        }
       }
-      if (MODE != FWD && ok && pending) ok = second_product();
+      if (MODE != FWD)
+        for (; ok && c2.unit < units; c2.next(g)) ok = second_product(c2);
       if (!ok) {
         // what was issued ends before the tensor memory is freed
         int never = 0;
@@ -433,38 +467,45 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
     Ring bs;
     uint32_t t = 0;
     bool ok = true;
-    const uint32_t buffer = tmem + lanes + group * SBUF;
-    for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+    const int step = gridDim.x;
+    int y_next = 0;
+    float c_next = 0.f;
+    auto fetch = [&](int u) {  // the row's constants, one unit ahead
+      if (u >= units) return;
+      const int row = unit_range(g, u).tile * TILE + (warp & 3) * 32 + lane;
+      if (MODE != DW) y_next = g.y[row];
+      if (MODE == DX) c_next = -g.lse2[row];
+      if (MODE == DW) c_next = g.b2[row];
+    };
+    fetch(blockIdx.x);
+    for (int u = blockIdx.x; u < units && ok; u += step) {
       const Range r = unit_range(g, u);
       const int row = r.tile * TILE + (warp & 3) * 32 + lane;
-      int y = 0;
-      float row_c = 0.f;  // -lse2 (DX) or the class's bias (DW)
-      if (MODE != DW) y = g.y[row];
-      if (MODE == DX) row_c = -g.lse2[row];
-      if (MODE == DW) row_c = g.b2[row];
+      const int y = y_next;
+      const float row_c = c_next;  // -lse2 (DX) or the class's bias (DW)
+      fetch(u + step);
       float m = -INFINITY, s = 0.f;
       float2 bias_sum = make_float2(0.f, 0.f);
       for (int bt = r.lo; bt < r.hi; ++bt, ++t, bs.next(g.stages)) {
         if ((int)(t & 1) != group) continue;
         // the meta data comes with the tile that z is made of
         ok = __all_sync(0xffffffffu, mbar_wait(&bar->b_full[bs.i], bs.phase, stop) &&
-                                         mbar_wait(&bar->s_full[group], (t >> 1) & 1, stop));
+                                         mbar_wait(&bar->s_full[t & z_mask], (t >> g.z_shift) & 1, stop));
         if (!ok) break;
         fence_after();
         const float* meta = sMeta + bs.i * META;
         const long long col0 = (long long)bt * TN;
-        uint32_t v[2][32];
-        tmem_load32(buffer, v[0]);
+        const uint32_t buffer = tmem + lanes + (t & z_mask) * SBUF;
+        uint32_t z[32];
+        tmem_load32(buffer, z);
         float2 tile_s[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < TN / 32; ++c) {
-          uint32_t(&z)[32] = v[c & 1];
           tmem_load_wait(z);
-          if (c + 1 < TN / 32) tmem_load32(buffer + 32 * (c + 1), v[(c + 1) & 1]);
           if (MODE == FWD && c + 1 == TN / 32) {
             fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bar->s_free[group]);
+            if (lane == 0) mbar_arrive(&bar->s_free[t & z_mask]);
           }
           float2 x[16];
           if (MODE == DW) {
@@ -488,14 +529,17 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
                               make_float2(b.z, b.w));
             }
           }
+          if (c + 1 < TN / 32) tmem_load32(buffer + 32 * (c + 1), z);
           if (MODE == FWD) {
             const int rel = (int)(y - (col0 + 32 * c));
             if (__any_sync(0xffffffffu, rel >= 0 && rel < 32 && y >= 0)) {
+              float tl = 0.f;
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
-                if (rel == 2 * i) g.t_label[row] = x[i].x;
-                if (rel == 2 * i + 1) g.t_label[row] = x[i].y;
+                if (rel == 2 * i) tl = x[i].x;
+                if (rel == 2 * i + 1) tl = x[i].y;
               }
+              if (rel >= 0 && rel < 32 && y >= 0) g.t_label[row] = tl;
             }
             float cm = fmaxf(x[0].x, x[0].y);
 #pragma unroll
@@ -566,7 +610,7 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
         }
         __syncwarp();
         if (lane == 0) {
-          if (MODE != FWD) mbar_arrive(&bar->p_full[group]);
+          if (MODE != FWD) mbar_arrive(&bar->p_full[t & z_mask]);
           mbar_arrive(&bar->b_empty[bs.i]);
         }
         const float2 ts = add2(tile_s[0], tile_s[1]);
@@ -593,7 +637,7 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
         ok = __all_sync(0xffffffffu, mbar_wait(&bar->acc_full[acc.i], acc.phase, stop));
         if (!ok) break;
         fence_after();
-        const uint32_t src = tmem + lanes + 2 * SBUF + acc.i * ACCS * D;
+        const uint32_t src = tmem + lanes + ACC0 + acc.i * ACCS * D;
         for (int c0 = 0; c0 < D; c0 += 32) {
           float4 v[8];
 #pragma unroll
@@ -795,19 +839,24 @@ inline int split_count(long long a_tiles, long long b_tiles) {
 // all tensor memory columns never shares an SM with another one.
 constexpr size_t SMEM_MIN = 118 * 1024, SMEM_MAX = 227 * 1024;
 
-// Columns of a streamed tile: the most of 128, 64 and 32 with which the
-// resident tile and three stages fit.
+// Columns of a streamed tile: the most of 128 (64 in the gradient passes,
+// whose tensor memory then has room for four z buffers), 64 and 32 with which
+// the resident tile and four stages fit.
+template <int MODE>
 inline int tile_columns(int planes, int D8) {
-  for (int tn = 128; tn > 32; tn /= 2)
-    if ((size_t)planes * D8 * (2048 + 3 * tn * 16) + 3 * 3 * tn * 4 + sizeof(Barriers) + 128 <= SMEM_MAX) return tn;
-  return 32;
+  int tn = MODE == FWD ? 128 : 64;
+  while (tn > 32 && (size_t)planes * D8 * (2048 + 4 * tn * 16) + 4 * meta_floats<MODE>(tn) * 4 + sizeof(Barriers) + 128 >
+                        SMEM_MAX)
+    tn /= 2;
+  return tn;
 }
 
 struct Dims {
   long long N, x_tiles, w_tiles;  // tiles of 128 rows, as packed
-  int D, D8, planes, tn;
-  int x_cols, w_cols;             // tiles of tn rows, as streamed
-  int v_splits, n_splits;
+  int D, D8, planes;
+  int fwd_tn, dx_tn, dw_tn;       // rows of a streamed tile
+  int fwd_cols, dx_cols, dw_cols;  // streamed tiles
+  int fwd_splits, dx_splits, dw_splits;
 };
 inline Dims dims_of(const gsb_class_loss_args* a) {
   Dims d;
@@ -817,11 +866,15 @@ inline Dims dims_of(const gsb_class_loss_args* a) {
   d.D = pad_c(a->C);
   d.D8 = d.D / 8;
   d.planes = planes_of(a->dtype);
-  d.tn = tile_columns(d.planes, d.D8);
-  d.x_cols = (int)((d.N + d.tn - 1) / d.tn);
-  d.w_cols = (int)((a->V + d.tn - 1) / d.tn);
-  d.v_splits = d.x_tiles > 0 ? split_count(d.x_tiles, d.w_cols) : 1;
-  d.n_splits = split_count(d.w_tiles, std::max(d.x_cols, 1));
+  d.fwd_tn = tile_columns<FWD>(d.planes, d.D8);
+  d.dx_tn = tile_columns<DX>(d.planes, d.D8);
+  d.dw_tn = tile_columns<DW>(d.planes, d.D8);
+  d.fwd_cols = div_up(a->V, d.fwd_tn);
+  d.dx_cols = div_up(a->V, d.dx_tn);
+  d.dw_cols = div_up(d.N, d.dw_tn);
+  d.fwd_splits = d.x_tiles > 0 ? split_count(d.x_tiles, d.fwd_cols) : 1;
+  d.dx_splits = d.x_tiles > 0 ? split_count(d.x_tiles, d.dx_cols) : 1;
+  d.dw_splits = split_count(d.w_tiles, std::max(d.dw_cols, 1));
   return d;
 }
 
@@ -843,8 +896,8 @@ struct FwdWs {
 inline size_t carve_fwd(void* base, const Dims& d, FwdWs* w) {
   Carver c{(char*)base};
   const size_t rows = (size_t)d.x_tiles * TILE;
-  w->part_m = c.take<float>(rows * d.v_splits * 2);
-  w->part_s = c.take<float>(rows * d.v_splits * 2);
+  w->part_m = c.take<float>(rows * d.fwd_splits * 2);
+  w->part_s = c.take<float>(rows * d.fwd_splits * 2);
   w->t_label = c.take<float>(rows);
   w->block_loss = c.take<double>(JOIN_BLOCKS);
   w->block_count = c.take<double>(JOIN_BLOCKS);
@@ -856,9 +909,9 @@ struct BwdWs {
 };
 inline size_t carve_bwd(void* base, const Dims& d, BwdWs* w) {
   Carver c{(char*)base};
-  w->part_x = c.take<float>((size_t)d.x_tiles * TILE * d.v_splits * d.D);
-  w->part_w = c.take<float>((size_t)d.w_tiles * TILE * d.n_splits * d.D);
-  w->part_bias = c.take<float>((size_t)d.w_tiles * TILE * d.n_splits * 2);
+  w->part_x = c.take<float>((size_t)d.x_tiles * TILE * d.dx_splits * d.D);
+  w->part_w = c.take<float>((size_t)d.w_tiles * TILE * d.dw_splits * d.D);
+  w->part_bias = c.take<float>((size_t)d.w_tiles * TILE * d.dw_splits * 2);
   w->row_u = c.take<float>((size_t)d.x_tiles * TILE);
   return c.off;
 }
@@ -897,11 +950,14 @@ int launch_tiled(StreamArgs g, cudaStream_t s) {
   const size_t a_bytes = (size_t)NP * g.D8 * 2048;
   const size_t stage = (size_t)NP * g.D8 * TN * 16 + meta_floats<MODE>(TN) * 4;
   const size_t fixed = sizeof(Barriers) + 128;
-  constexpr int SBUF = z_columns(NP, TN), ACCS = accumulators(NP);
+  constexpr int SBUF = z_columns<MODE>(NP, TN), ACCS = accumulators(NP);
   g.flush = chain_products(NP) / (TN / 16);
-  g.a_slots = 2 * a_bytes + 3 * stage + fixed <= SMEM_MAX ? 2 : 1;
+  for (g.a_slots = MAX_A_SLOTS; g.a_slots > 1; --g.a_slots)
+    if (g.a_slots * a_bytes + 6 * stage + fixed <= SMEM_MAX) break;
   g.stages = (int)std::min<size_t>(MAX_STAGES, (SMEM_MAX - fixed - g.a_slots * a_bytes) / stage);
-  g.acc_slots = 2 * SBUF + 2 * ACCS * g.D8 * 8 <= TMEM_COLUMNS ? 2 : 1;
+  const int acc = MODE == FWD ? 0 : ACCS * g.D8 * 8;
+  g.z_shift = 4 * SBUF + acc <= TMEM_COLUMNS ? 2 : 1;
+  g.acc_slots = (SBUF << g.z_shift) + 2 * acc <= TMEM_COLUMNS ? 2 : 1;
   const size_t smem = std::max(SMEM_MIN, g.a_slots * a_bytes + g.stages * stage + fixed);
   cudaFuncSetAttribute(stream_kernel<MODE, NP, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   const int units = g.a_tiles * g.splits;
@@ -912,16 +968,21 @@ int launch_tiled(StreamArgs g, cudaStream_t s) {
 template <int MODE>
 int launch_stream(const StreamArgs& g, int planes, int tn, cudaStream_t s) {
   switch (planes * 1000 + tn) {
-    case 1128: return launch_tiled<MODE, 1, 128>(g, s);
     case 1064: return launch_tiled<MODE, 1, 64>(g, s);
-    case 2128: return launch_tiled<MODE, 2, 128>(g, s);
     case 2064: return launch_tiled<MODE, 2, 64>(g, s);
     case 2032: return launch_tiled<MODE, 2, 32>(g, s);
-    case 3128: return launch_tiled<MODE, 3, 128>(g, s);
     case 3064: return launch_tiled<MODE, 3, 64>(g, s);
     case 3032: return launch_tiled<MODE, 3, 32>(g, s);
-    default: set_error("class loss: no pass for %d planes and tiles of %d", planes, tn); return GSB_ERR_INVALID;
   }
+  if constexpr (MODE == FWD) {
+    switch (planes * 1000 + tn) {
+      case 1128: return launch_tiled<MODE, 1, 128>(g, s);
+      case 2128: return launch_tiled<MODE, 2, 128>(g, s);
+      case 3128: return launch_tiled<MODE, 3, 128>(g, s);
+    }
+  }
+  set_error("class loss: no pass for %d planes and tiles of %d", planes, tn);
+  return GSB_ERR_INVALID;
 }
 
 inline int blocks_for(long long n) { return (int)std::max(1ll, std::min((n + THREADS - 1) / THREADS, (long long)SMS * 16)); }
@@ -966,8 +1027,8 @@ GSB_EXPORT int gsb_class_loss_fwd(const gsb_class_loss_args* a, void* stream) {
   g.b2 = a->class_bias2;
   g.y = a->row_y;
   g.a_tiles = (int)d.x_tiles;
-  g.b_tiles = d.w_cols;
-  g.splits = d.v_splits;
+  g.b_tiles = d.fwd_cols;
+  g.splits = d.fwd_splits;
   g.error_word = a->error_word;
   g.D8 = d.D8;
   g.part_m = w.part_m;
@@ -977,11 +1038,11 @@ GSB_EXPORT int gsb_class_loss_fwd(const gsb_class_loss_args* a, void* stream) {
   pack_classes_kernel<<<blocks_for(w_total), THREADS, 0, s>>>(*a, d.D8, w_total, (uint4*)a->packed_w, a->class_bias2);
   if (d.N > 0) {
     pack_rows_kernel<<<blocks_for(x_total), THREADS, 0, s>>>(*a, d.D8, x_total, (uint4*)a->packed_x, a->row_y);
-    const int r = launch_stream<FWD>(g, d.planes, d.tn, s);
+    const int r = launch_stream<FWD>(g, d.planes, d.fwd_tn, s);
     if (r != GSB_OK) return r;
   }
   const int blocks = (int)std::max(1ll, std::min<long long>(JOIN_BLOCKS, (d.x_tiles * TILE + THREADS - 1) / THREADS));
-  join_rows_kernel<<<blocks, THREADS, 0, s>>>(g, 2 * d.v_splits, d.N, a->row_lse2, a->row_y,
+  join_rows_kernel<<<blocks, THREADS, 0, s>>>(g, 2 * d.fwd_splits, d.N, a->row_lse2, a->row_y,
                                               a->reduction == GSB_REDUCE_NONE ? a->loss : nullptr, w.block_loss,
                                               w.block_count);
   finish_loss_kernel<<<1, THREADS, 0, s>>>(w.block_loss, w.block_count, blocks, a->reduction, a->loss, a->inv_count);
@@ -1019,29 +1080,29 @@ GSB_EXPORT int gsb_class_loss_bwd(const gsb_class_loss_args* a, void* stream) {
     g.a = (const uint4*)a->packed_x;
     g.b = (const uint4*)a->packed_w;
     g.a_tiles = (int)d.x_tiles;
-    g.b_tiles = d.w_cols;
-    g.splits = d.v_splits;
+    g.b_tiles = d.dx_cols;
+    g.splits = d.dx_splits;
     g.part_acc = w.part_x;
-    const int r = launch_stream<DX>(g, d.planes, d.tn, s);
+    const int r = launch_stream<DX>(g, d.planes, d.dx_tn, s);
     if (r != GSB_OK) return r;
-    join_dx_kernel<<<blocks_for(d.N * a->C), THREADS, 0, s>>>(*a, w.part_x, d.v_splits, d.D, d.x_tiles * TILE);
+    join_dx_kernel<<<blocks_for(d.N * a->C), THREADS, 0, s>>>(*a, w.part_x, d.dx_splits, d.D, d.x_tiles * TILE);
   }
   if (a->grad_weight || a->grad_bias) {
     g.a = (const uint4*)a->packed_w;
     g.b = (const uint4*)a->packed_x;
     g.a_tiles = (int)d.w_tiles;
-    g.b_tiles = d.x_cols;
-    g.splits = d.n_splits;
+    g.b_tiles = d.dw_cols;
+    g.splits = d.dw_splits;
     g.part_acc = w.part_w;
     g.part_bias = w.part_bias;
     if (a->reduction == GSB_REDUCE_NONE) {
       row_upstream_kernel<<<blocks_for(d.x_tiles * TILE), THREADS, 0, s>>>(a->upstream, a->row_y, d.x_tiles * TILE, w.row_u);
       g.row_u = w.row_u;
     }
-    const int r = launch_stream<DW>(g, d.planes, d.tn, s);
+    const int r = launch_stream<DW>(g, d.planes, d.dw_tn, s);
     if (r != GSB_OK) return r;
-    join_dw_kernel<<<blocks_for(a->V * (a->C + 1ll)), THREADS, 0, s>>>(*a, w.part_w, w.part_bias, d.n_splits,
-                                                                      2 * d.n_splits, d.D, d.w_tiles * TILE);
+    join_dw_kernel<<<blocks_for(a->V * (a->C + 1ll)), THREADS, 0, s>>>(*a, w.part_w, w.part_bias, d.dw_splits,
+                                                                      2 * d.dw_splits, d.D, d.w_tiles * TILE);
   }
   return check_launch("gsb_class_loss_bwd");
 }

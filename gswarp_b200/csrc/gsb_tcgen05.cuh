@@ -24,14 +24,17 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
 __device__ __forceinline__ void mbar_expect(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
+// The thread sleeps up to this long in one try, instead of taking issue slots
+// from the warps that compute.
+constexpr uint32_t SUSPEND_NS = 1000 * 1000;
 __device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
       "{\n.reg .pred p;\n"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
       "selp.u32 %0, 1, 0, p;\n}\n"
       : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(SUSPEND_NS)
       : "memory");
   return ok != 0;
 }
@@ -48,11 +51,12 @@ __device__ __forceinline__ unsigned long long global_ns() {
 }
 
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* stop) {
-  if (mbar_try(bar, parity)) return true;
+  for (int i = 0; i < 16; ++i)
+    if (mbar_try(bar, parity)) return true;
   const unsigned long long start = global_ns();
   for (unsigned i = 1;; ++i) {
     if (mbar_try(bar, parity)) return true;
-    if ((i & 255) == 0) {
+    if ((i & 15) == 0) {
       if (*stop) return false;
       if (global_ns() - start > WAIT_NS) break;
     }
@@ -127,29 +131,31 @@ __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::
 
 // ---- matrix instructions ----
 // Shared-memory operand of 8 x 16-byte core matrices, each 128 contiguous
-// bytes, no swizzle.  K-major: `lead` is the distance between core matrices
-// along K, `stride` between groups of 8 rows.  MN-major: `lead` is the
-// distance between groups of 8 along K, `stride` along M or N.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead, uint32_t stride) {
-  return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)((lead >> 4) & 0x3FFF) << 16 |
-         (uint64_t)((stride >> 4) & 0x3FFF) << 32 | (uint64_t)1 << 46;
-}
+// bytes, no swizzle, as the two halves of its descriptor.  K-major: `lead` is
+// the distance between core matrices along K, `stride` between groups of 8
+// rows.  MN-major: `lead` is the distance between groups of 8 along K,
+// `stride` along M or N.  Adding bytes / 16 to the low half moves the operand.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lead) { return addr >> 4 | (lead >> 4) << 16; }
+__device__ __forceinline__ uint32_t desc_hi(uint32_t stride) { return stride >> 4 | 1u << 14; }
 // bf16 operands, fp32 accumulator, M = 128.
 __device__ __forceinline__ uint32_t instr_desc(int n, bool b_mn_major) {
   return 1u << 4 | 1u << 7 | 1u << 10 | (b_mn_major ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (128u >> 4) << 24;
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
+                                       uint32_t idesc, bool accumulate) {
   asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      "{\n.reg .pred p;\n.reg .b64 a, b;\nsetp.ne.u32 p, %6, 0;\n"
+      "mov.b64 a, {%1, %2};\nmov.b64 b, {%3, %4};\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n}\n" ::"r"(d),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"((uint32_t)accumulate)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                       bool accumulate) {
   asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      "{\n.reg .pred p;\n.reg .b64 b;\nsetp.ne.u32 p, %5, 0;\nmov.b64 b, {%2, %3};\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"((uint32_t)accumulate)
       : "memory");
 }
 // Arrives on `bar` once every matrix instruction issued so far is done.
