@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(THREADS) pack_classes_kernel(const gsb_class_l
 // ---------------------------------------------------------------------------
 // The streaming pass: one persistent CTA per SM.  A work unit is a resident
 // tile of 128 rows and a range of the streamed operand's tiles of TN rows
-// (columns of z).  Warp 8 loads, warp 9 issues the matrix instructions, two
+// (columns of z).  One warp loads, one issues the matrix instructions, two
 // groups of four warps take the tiles of z in turn, and in the gradient
 // passes four more warps store finished accumulators while the next unit
 // runs.  A thread owns one row of z (a lane of tensor memory):
@@ -152,6 +152,8 @@ enum { FWD = 0, DX = 1, DW = 2 };
 
 constexpr int MAX_STAGES = 16, MAX_A_SLOTS = 4;
 constexpr int TMEM_COLUMNS = 512;
+constexpr int GROUPS = 4;                      // consumer groups of four warps, one z buffer each
+constexpr int LOADER = GROUPS * 4, ISSUER = LOADER + 1;  // warps
 
 struct StreamArgs {
   const uint4* a;          // resident operand, packed
@@ -161,24 +163,26 @@ struct StreamArgs {
   const int* y;            // rows
   const float* row_u;      // per-row upstream (DW, reduction none) or NULL
   int a_tiles, b_tiles, splits, D8;
-  int a_slots, stages, acc_slots, z_shift;  // z_shift: log2 of the number of z buffers
+  int a_slots, stages, acc_slots;
+  int slots;               // partial results a unit leaves: its groups that had a tile
+  int distance;            // tiles between a tile's two products
   int flush;               // tiles per accumulator
-  float* part_m;           // FWD: [split][group][row]
+  float* part_m;           // FWD: [split][slot][row]
   float* part_s;
   float* t_label;          // FWD: [row]
   float* part_acc;         // DX, DW: [split][tile][column / 4][row][4 columns]
-  float* part_bias;        // DW: [split][group][row]
+  float* part_bias;        // DW: [split][slot][row]
   long long* error_word;
 };
 
 struct Barriers {
   uint64_t a_full[MAX_A_SLOTS], a_empty[MAX_A_SLOTS], b_full[MAX_STAGES], b_empty[MAX_STAGES];
-  uint64_t s_full[4], s_free[4], p_full[4], acc_full[2], acc_empty[2], drained;
+  uint64_t s_full[GROUPS], s_free[GROUPS], p_full[GROUPS], acc_full[2], acc_empty[2], drained;
   uint32_t tmem;
   int stop;
 };
 
-// Tensor memory: two buffers of z, over which P is written (two planes fit
+// Tensor memory: a buffer of z for each group, over which P is written (two planes fit
 // its 32-bit columns, the third has its own), then the accumulators.
 template <int MODE>
 __host__ __device__ constexpr int z_columns(int np, int tn) {
@@ -200,7 +204,7 @@ __host__ __device__ constexpr int chain_products(int np) { return np == 3 ? 16 :
 template <int MODE>
 __host__ __device__ constexpr int meta_floats(int tn) { return MODE == DW ? 3 * tn : tn; }
 template <int MODE>
-__host__ __device__ constexpr int stream_threads() { return MODE == FWD ? 320 : 448; }
+__host__ __device__ constexpr int stream_threads() { return (MODE == FWD ? GROUPS * 4 + 2 : GROUPS * 4 + 6) * 32; }
 
 // A position in a ring of buffers and the parity of its current round.
 struct Ring {
@@ -266,17 +270,22 @@ __host__ __device__ constexpr int plane_of_b(int np, int q) {
   return (np == 3 ? 0x010120 : np == 2 ? 0x0101 : 0) >> (4 * q) & 15;
 }
 
-// Splits 32 values into bf16 planes and stores them over z's chunk.
+// Splits 16 values into bf16 planes and stores them over z's columns they
+// come from: the K = 16 step at column c is 8 words of plane 0 and 8 of plane
+// 1 there, and 8 of plane 2 behind the buffer's z.
+__device__ __forceinline__ constexpr int p_column(int tn, int c, int plane) {
+  return plane < 2 ? c + 8 * plane : tn + c / 2;
+}
 template <int NP, int TN>
-__device__ __forceinline__ void store_p(uint32_t buffer, int chunk, const float2 (&p)[16]) {
-  float2 rest[16];
+__device__ __forceinline__ void store_p(uint32_t buffer, int c, const float2 (&p)[8]) {
+  float2 rest[8];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) rest[i] = p[i];
+  for (int i = 0; i < 8; ++i) rest[i] = p[i];
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
-    uint32_t h[16];
+    uint32_t h[8];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < 8; ++i) {
       const __nv_bfloat162 v = __floats2bfloat162_rn(rest[i].x, rest[i].y);
       h[i] = *reinterpret_cast<const uint32_t*>(&v);
       if (k + 1 < NP) {
@@ -284,7 +293,7 @@ __device__ __forceinline__ void store_p(uint32_t buffer, int chunk, const float2
         rest[i] = add2(rest[i], make_float2(-f.x, -f.y));
       }
     }
-    tc::tmem_store16(buffer + (k < 2 ? 32 * chunk + 16 * k : TN + 16 * chunk), h);
+    tc::tmem_store(buffer + p_column(TN, c, k), h);
   }
 }
 
@@ -304,9 +313,7 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
   const int units = g.a_tiles * g.splits;
   constexpr int SBUF = z_columns<MODE>(NP, TN);
   constexpr int ACCS = accumulators(NP);
-  const uint32_t z_mask = (1u << g.z_shift) - 1;
-  const uint32_t ACC0 = SBUF << g.z_shift;          // first accumulator column
-  const int group = warp >> 2;                      // consumer groups 0 and 1
+  constexpr uint32_t ACC0 = GROUPS * SBUF;          // first accumulator column
 
   if (threadIdx.x == 0) {
     bar->stop = 0;
@@ -318,7 +325,7 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
       mbar_init(&bar->acc_full[i], 1);
       mbar_init(&bar->acc_empty[i], 4);
     }
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < GROUPS; ++i) {
       mbar_init(&bar->s_full[i], 1);
       mbar_init(&bar->s_free[i], MODE == FWD ? 4 : 1);
       mbar_init(&bar->p_full[i], 4);
@@ -330,14 +337,14 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
     mbar_init(&bar->drained, 1);
     mbar_init_fence();
   }
-  if (warp == 9) tmem_alloc(&bar->tmem, TMEM_COLUMNS);
+  if (warp == ISSUER) tmem_alloc(&bar->tmem, TMEM_COLUMNS);
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = bar->tmem;
   const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's quarter of the 128 lanes
 
-  if (warp == 8) {
+  if (warp == LOADER) {
     // ---- loads ----
     Ring as, bs;
     bool ok = true;
@@ -381,7 +388,7 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
       for (int i = 0; i < g.a_slots; ++i)
         mbar_wait(&bar->a_full[i], i < as.i ? as.phase : as.phase ^ 1, &never);
     }
-  } else if (warp == 9) {
+  } else if (warp == ISSUER) {
     // ---- matrix instructions ----
     if (lane == 0) {
       const uint32_t idesc1 = instr_desc(TN, false), idesc2 = instr_desc(D, true);
@@ -390,10 +397,10 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
       bool ok = true;
 
       auto first_product = [&](Cursor& c) {
-        const uint32_t b = c.t & z_mask;
+        const uint32_t b = c.t % GROUPS;
         if (c.bt == c.r.lo && !mbar_wait(&bar->a_full[c.as.i], c.as.phase, stop)) return false;
         if (!mbar_wait(&bar->b_full[c.bs.i], c.bs.phase, stop)) return false;
-        if (!mbar_wait(&bar->s_free[b], ((c.t >> g.z_shift) & 1) ^ 1, stop)) return false;
+        if (!mbar_wait(&bar->s_free[b], ((c.t / GROUPS) & 1) ^ 1, stop)) return false;
         fence_after();
         const uint32_t a_lo = desc_lo(a0 + c.as.i * a_bytes, 2048), b_lo = desc_lo(b0 + c.bs.i * b_bytes, TN * 16);
         const uint32_t z = tmem + b * SBUF;
@@ -411,10 +418,10 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
       };
 
       auto second_product = [&](Cursor& c) {
-        const uint32_t b = c.t & z_mask;
+        const uint32_t b = c.t % GROUPS;
         const int in_acc = (c.bt - c.r.lo) % g.flush;
         const bool first = in_acc == 0, last = in_acc + 1 == g.flush || c.bt + 1 == c.r.hi;
-        if (!mbar_wait(&bar->p_full[b], (c.t >> g.z_shift) & 1, stop)) return false;
+        if (!mbar_wait(&bar->p_full[b], (c.t / GROUPS) & 1, stop)) return false;
         if (first && !mbar_wait(&bar->acc_empty[c.acc.i], c.acc.phase ^ 1, stop)) return false;
         fence_after();
         const uint32_t dst = tmem + ACC0 + c.acc.i * ACCS * D, p = tmem + b * SBUF;
@@ -427,7 +434,7 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
           const uint32_t bq = b_lo + plane_of_b(NP, q) * D8 * TN;
 #pragma unroll
           for (int k = 0; k < TN / 16; ++k)
-            mma_ts(to, p + (pa < 2 ? 32 * (k / 2) + 16 * pa : TN + 16 * (k / 2)) + 8 * (k & 1), bq + k * 16, hi2,
+            mma_ts(to, p + p_column(TN, 16 * k, pa), bq + k * 16, hi2,
                    idesc2, k > 0 || (q > 0 && !(ACCS == 2 && main)) || !first);
         }
         mma_commit(&bar->b_empty[c.bs.i]);
@@ -439,11 +446,11 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
         return true;
       };
 
-      // The second product follows the first at a distance: with four z
-      // buffers a group finds its next tile ready while P of its last one
-      // still waits for its product.
+      // The second product of a tile follows the first ones of the next
+      // groups' tiles, so that P of one group is awaited while the others
+      // have work.
       Cursor c1(g), c2(g);
-      const uint32_t distance = 1u << (g.z_shift - 1);
+      const uint32_t distance = g.distance;
       while (ok && c1.unit < units) {
         ok = first_product(c1);
         c1.next(g);
@@ -462,12 +469,15 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
       }
     }
     __syncwarp();
-  } else if (warp < 8) {
+  } else if (warp < LOADER) {
     // ---- z -> row statistics, or P ----
+    constexpr int CH = MODE == FWD ? 32 : 16;  // columns in registers at a time
+    const int group = warp / 4;
+    const uint32_t buffer = tmem + lanes + group * SBUF;
+    const int step = gridDim.x;
     Ring bs;
     uint32_t t = 0;
     bool ok = true;
-    const int step = gridDim.x;
     int y_next = 0;
     float c_next = 0.f;
     auto fetch = [&](int u) {  // the row's constants, one unit ahead
@@ -484,124 +494,118 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
       const int y = y_next;
       const float row_c = c_next;  // -lse2 (DX) or the class's bias (DW)
       fetch(u + step);
+      const int slot = (int)((group - t) % GROUPS);  // this group's first tile in the unit
       float m = -INFINITY, s = 0.f;
       float2 bias_sum = make_float2(0.f, 0.f);
       for (int bt = r.lo; bt < r.hi; ++bt, ++t, bs.next(g.stages)) {
-        if ((int)(t & 1) != group) continue;
+        if ((int)(t % GROUPS) != group) continue;
         // the meta data comes with the tile that z is made of
         ok = __all_sync(0xffffffffu, mbar_wait(&bar->b_full[bs.i], bs.phase, stop) &&
-                                         mbar_wait(&bar->s_full[t & z_mask], (t >> g.z_shift) & 1, stop));
+                                         mbar_wait(&bar->s_full[group], (t / GROUPS) & 1, stop));
         if (!ok) break;
         fence_after();
         const float* meta = sMeta + bs.i * META;
-        const long long col0 = (long long)bt * TN;
-        const uint32_t buffer = tmem + lanes + (t & z_mask) * SBUF;
-        uint32_t z[32];
-        tmem_load32(buffer, z);
+        const int col0 = bt * TN;
+        uint32_t z[CH];
+        tmem_load(buffer, z);
         float2 tile_s[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll 1
-        for (int c = 0; c < TN / 32; ++c) {
+        for (int c = 0; c < TN; c += CH) {
           tmem_load_wait(z);
-          if (MODE == FWD && c + 1 == TN / 32) {
+          if (MODE == FWD && c + CH == TN) {
             fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bar->s_free[t & z_mask]);
+            if (lane == 0) mbar_arrive(&bar->s_free[group]);
           }
-          float2 x[16];
-          if (MODE == DW) {
-            const float2 l2e = make_float2(LOG2E, LOG2E), cst = make_float2(row_c, row_c);
+          // t of the columns: z log2(e) + bias, less the row's or the column's log-sum in the gradients
+          float2 x[CH / 2];
+          const float2 l2e = make_float2(LOG2E, LOG2E), cst = make_float2(row_c, row_c);
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              const float4 l = *reinterpret_cast<const float4*>(meta + 32 * c + 2 * i);
-              x[i] = fma2(make_float2(__uint_as_float(z[2 * i]), __uint_as_float(z[2 * i + 1])), l2e, cst);
-              x[i + 1] = fma2(make_float2(__uint_as_float(z[2 * i + 2]), __uint_as_float(z[2 * i + 3])), l2e, cst);
-              x[i] = add2(x[i], make_float2(-l.x, -l.y));
-              x[i + 1] = add2(x[i + 1], make_float2(-l.z, -l.w));
-            }
-          } else {
-            const float2 l2e = make_float2(LOG2E, LOG2E);
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              const float4 b = *reinterpret_cast<const float4*>(meta + 32 * c + 2 * i);
-              x[i] = fma2(make_float2(__uint_as_float(z[2 * i]), __uint_as_float(z[2 * i + 1])), l2e,
-                          make_float2(b.x, b.y));
-              x[i + 1] = fma2(make_float2(__uint_as_float(z[2 * i + 2]), __uint_as_float(z[2 * i + 3])), l2e,
-                              make_float2(b.z, b.w));
+          for (int i = 0; i < CH / 2; i += 2) {
+            const float4 w = *reinterpret_cast<const float4*>(meta + c + 2 * i);
+            const float2 z0 = make_float2(__uint_as_float(z[2 * i]), __uint_as_float(z[2 * i + 1]));
+            const float2 z1 = make_float2(__uint_as_float(z[2 * i + 2]), __uint_as_float(z[2 * i + 3]));
+            if (MODE == DW) {
+              x[i] = add2(fma2(z0, l2e, cst), make_float2(-w.x, -w.y));
+              x[i + 1] = add2(fma2(z1, l2e, cst), make_float2(-w.z, -w.w));
+            } else {
+              x[i] = fma2(z0, l2e, make_float2(w.x, w.y));
+              x[i + 1] = fma2(z1, l2e, make_float2(w.z, w.w));
+              if (MODE == DX) {
+                x[i] = add2(x[i], cst);
+                x[i + 1] = add2(x[i + 1], cst);
+              }
             }
           }
-          if (c + 1 < TN / 32) tmem_load32(buffer + 32 * (c + 1), z);
+          if (c + CH < TN) tmem_load(buffer + c + CH, z);
           if (MODE == FWD) {
-            const int rel = (int)(y - (col0 + 32 * c));
-            if (__any_sync(0xffffffffu, rel >= 0 && rel < 32 && y >= 0)) {
+            const int rel = y - (col0 + c);
+            if (__any_sync(0xffffffffu, y >= 0 && rel >= 0 && rel < CH)) {
               float tl = 0.f;
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
+              for (int i = 0; i < CH / 2; ++i) {
                 if (rel == 2 * i) tl = x[i].x;
                 if (rel == 2 * i + 1) tl = x[i].y;
               }
-              if (rel >= 0 && rel < 32 && y >= 0) g.t_label[row] = tl;
+              if (y >= 0 && rel >= 0 && rel < CH) g.t_label[row] = tl;
             }
-            float cm = fmaxf(x[0].x, x[0].y);
+            float cm[2] = {fmaxf(x[0].x, x[0].y), fmaxf(x[1].x, x[1].y)};
 #pragma unroll
-            for (int i = 1; i < 16; ++i) cm = fmaxf(cm, fmaxf(x[i].x, x[i].y));
+            for (int i = 2; i < CH / 2; ++i) cm[i & 1] = fmaxf(cm[i & 1], fmaxf(x[i].x, x[i].y));
+            const float top = fmaxf(cm[0], cm[1]);
             // The sums' base follows the maximum only when it is left behind by 2^8: fp32 has the range,
             // and the rescaling is rare.
-            if (cm > m + 8.f) {
-              const float f = ex2(m - cm);
+            if (top > m + 8.f) {
+              const float f = ex2(m - top);
               s *= f;
               tile_s[0].x *= f;
               tile_s[0].y *= f;
               tile_s[1].x *= f;
               tile_s[1].y *= f;
-              m = cm;
+              m = top;
             }
             const float nb = m == -INFINITY ? 0.f : -m;
             const float2 base = make_float2(nb, nb);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
+            for (int i = 0; i < CH / 2; ++i) {
               const float2 d = add2(x[i], base);
               tile_s[i & 1] = add2(tile_s[i & 1], make_float2(ex2(d.x), ex2(d.y)));
             }
           } else {
+#pragma unroll
+            for (int i = 0; i < CH / 2; ++i) x[i] = make_float2(ex2(x[i].x), ex2(x[i].y));
             if (MODE == DX) {
-              const float2 l = make_float2(row_c, row_c);
+              const int rel = y - (col0 + c);
+              if (__any_sync(0xffffffffu, y >= 0 && rel >= 0 && rel < CH)) {
 #pragma unroll
-              for (int i = 0; i < 16; ++i) x[i] = add2(x[i], l);
-            }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = make_float2(ex2(x[i].x), ex2(x[i].y));
-            if (MODE == DX) {
-              const int rel = (int)(y - (col0 + 32 * c));
-              if (__any_sync(0xffffffffu, rel >= 0 && rel < 32 && y >= 0)) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
+                for (int i = 0; i < CH / 2; ++i) {
                   if (y >= 0 && rel == 2 * i) x[i].x -= 1.f;
                   if (y >= 0 && rel == 2 * i + 1) x[i].y -= 1.f;
                 }
               }
             } else {
-              const int* ym = reinterpret_cast<const int*>(meta + TN) + 32 * c;
+              const int* ym = reinterpret_cast<const int*>(meta + TN) + c;
               const int wrow = row - lane;
-              const int yl = ym[lane];
+              const int yl = ym[lane % CH];
               if (__any_sync(0xffffffffu, yl >= wrow && yl < wrow + 32)) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
+                for (int i = 0; i < CH / 2; ++i) {
                   if (ym[2 * i] == row) x[i].x -= 1.f;
                   if (ym[2 * i + 1] == row) x[i].y -= 1.f;
                 }
               }
               if (g.row_u) {
 #pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                  const float4 w = *reinterpret_cast<const float4*>(meta + 2 * TN + 32 * c + 2 * i);
+                for (int i = 0; i < CH / 2; i += 2) {
+                  const float4 w = *reinterpret_cast<const float4*>(meta + 2 * TN + c + 2 * i);
                   x[i] = make_float2(x[i].x * w.x, x[i].y * w.y);
                   x[i + 1] = make_float2(x[i + 1].x * w.z, x[i + 1].y * w.w);
                 }
               }
 #pragma unroll
-              for (int i = 0; i < 16; ++i) tile_s[i & 1] = add2(tile_s[i & 1], x[i]);
+              for (int i = 0; i < CH / 2; ++i) tile_s[i & 1] = add2(tile_s[i & 1], x[i]);
             }
-            store_p<NP, TN>(buffer, c, x);
+            if constexpr (MODE != FWD) store_p<NP, TN>(buffer, c, x);
           }
         }
         if (MODE != FWD) {
@@ -610,7 +614,7 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
         }
         __syncwarp();
         if (lane == 0) {
-          if (MODE != FWD) mbar_arrive(&bar->p_full[t & z_mask]);
+          if (MODE != FWD) mbar_arrive(&bar->p_full[group]);
           mbar_arrive(&bar->b_empty[bs.i]);
         }
         const float2 ts = add2(tile_s[0], tile_s[1]);
@@ -618,12 +622,14 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
         if (MODE == DW) bias_sum = add2(bias_sum, ts);
       }
       if (!ok) break;
-      const size_t at = ((size_t)r.split * 2 + group) * ((size_t)g.a_tiles * TILE) + row;
-      if (MODE == FWD) {
-        g.part_m[at] = m;
-        g.part_s[at] = s;
+      if (slot < g.slots) {
+        const size_t at = ((size_t)r.split * g.slots + slot) * ((size_t)g.a_tiles * TILE) + row;
+        if (MODE == FWD) {
+          g.part_m[at] = m;
+          g.part_s[at] = s;
+        }
+        if (MODE == DW) g.part_bias[at] = bias_sum.x + bias_sum.y;
       }
-      if (MODE == DW) g.part_bias[at] = bias_sum.x + bias_sum.y;
     }
   } else if (MODE != FWD) {
     // ---- finished accumulators: added up in fp32 in the unit's partial rows ----
@@ -638,40 +644,31 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
         if (!ok) break;
         fence_after();
         const uint32_t src = tmem + lanes + ACC0 + acc.i * ACCS * D;
-        for (int c0 = 0; c0 < D; c0 += 32) {
-          float4 v[8];
+        for (int c = 0; c < D; c += 16) {
+          float4* at = dst + (size_t)(c / 4) * TILE;
+          float4 v[4];
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            if (c0 + 16 * c >= D) break;
-            uint32_t main[16], rest[16];
-            tmem_load16(src + c0 + 16 * c, main);
-            if (ACCS == 2) tmem_load16(src + D + c0 + 16 * c, rest);
-            float x[16];
+          for (int i = 0; i < 4; ++i) v[i] = bt > r.lo ? at[i * TILE] : make_float4(0.f, 0.f, 0.f, 0.f);
+          uint32_t main[16];
+          tmem_load(src + c, main);
+          tmem_load_wait(main);
+          if (ACCS == 2) {
+            uint32_t rest[16];
+            tmem_load(src + D + c, rest);
+            tmem_load_wait(rest);
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              x[i] = __uint_as_float(main[i]) + (ACCS == 2 ? __uint_as_float(rest[i]) : 0.f);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[4 * c + i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+            for (int i = 0; i < 16; ++i) main[i] = __float_as_uint(__uint_as_float(main[i]) + __uint_as_float(rest[i]));
           }
-          if (c0 + 32 >= D) {
+          if (c + 16 >= D) {
             fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar->acc_empty[acc.i]);
           }
-          float4* at = dst + (size_t)(c0 / 4) * TILE;
-          if (bt > r.lo) {
-            float4 old[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (c0 + 4 * i < D) old[i] = at[(size_t)i * TILE];
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (c0 + 4 * i < D)
-                v[i] = make_float4(old[i].x + v[i].x, old[i].y + v[i].y, old[i].z + v[i].z, old[i].w + v[i].w);
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (c0 + 4 * i < D) at[(size_t)i * TILE] = v[i];
+          for (int i = 0; i < 4; ++i)
+            at[i * TILE] = make_float4(v[i].x + __uint_as_float(main[4 * i]), v[i].y + __uint_as_float(main[4 * i + 1]),
+                                       v[i].z + __uint_as_float(main[4 * i + 2]),
+                                       v[i].w + __uint_as_float(main[4 * i + 3]));
         }
         acc.next(g.acc_slots);
       }
@@ -680,7 +677,7 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
   fence_before();
   __syncthreads();
   fence_after();
-  if (warp == 9) tmem_free(tmem, TMEM_COLUMNS);
+  if (warp == ISSUER) tmem_free(tmem, TMEM_COLUMNS);
   if (threadIdx.x == 0 && *stop)
     atomicOr((unsigned long long*)g.error_word, (unsigned long long)ERR_LOOKBACK_TIMEOUT);
 }
@@ -841,10 +838,14 @@ constexpr size_t SMEM_MIN = 118 * 1024, SMEM_MAX = 227 * 1024;
 
 // Columns of a streamed tile: the most of 128 (64 in the gradient passes,
 // whose tensor memory then has room for four z buffers), 64 and 32 with which
-// the resident tile and four stages fit.
+// the resident tile and four stages fit.  Three planes of P take half as
+// much tensor memory again.
 template <int MODE>
 inline int tile_columns(int planes, int D8) {
   int tn = MODE == FWD ? 128 : 64;
+  while (tn > 32 && GROUPS * z_columns<MODE>(planes, tn) + (MODE == FWD ? 0 : accumulators(planes) * D8 * 8) >
+                        TMEM_COLUMNS)
+    tn /= 2;
   while (tn > 32 && (size_t)planes * D8 * (2048 + 4 * tn * 16) + 4 * meta_floats<MODE>(tn) * 4 + sizeof(Barriers) + 128 >
                         SMEM_MAX)
     tn /= 2;
@@ -857,6 +858,7 @@ struct Dims {
   int fwd_tn, dx_tn, dw_tn;       // rows of a streamed tile
   int fwd_cols, dx_cols, dw_cols;  // streamed tiles
   int fwd_splits, dx_splits, dw_splits;
+  int fwd_slots, dw_slots;        // partial results per split
 };
 inline Dims dims_of(const gsb_class_loss_args* a) {
   Dims d;
@@ -875,6 +877,8 @@ inline Dims dims_of(const gsb_class_loss_args* a) {
   d.fwd_splits = d.x_tiles > 0 ? split_count(d.x_tiles, d.fwd_cols) : 1;
   d.dx_splits = d.x_tiles > 0 ? split_count(d.x_tiles, d.dx_cols) : 1;
   d.dw_splits = split_count(d.w_tiles, std::max(d.dw_cols, 1));
+  d.fwd_slots = std::min(GROUPS, div_up(d.fwd_cols, d.fwd_splits));
+  d.dw_slots = std::min(GROUPS, std::max(1, div_up(d.dw_cols, d.dw_splits)));
   return d;
 }
 
@@ -896,8 +900,8 @@ struct FwdWs {
 inline size_t carve_fwd(void* base, const Dims& d, FwdWs* w) {
   Carver c{(char*)base};
   const size_t rows = (size_t)d.x_tiles * TILE;
-  w->part_m = c.take<float>(rows * d.fwd_splits * 2);
-  w->part_s = c.take<float>(rows * d.fwd_splits * 2);
+  w->part_m = c.take<float>(rows * d.fwd_splits * d.fwd_slots);
+  w->part_s = c.take<float>(rows * d.fwd_splits * d.fwd_slots);
   w->t_label = c.take<float>(rows);
   w->block_loss = c.take<double>(JOIN_BLOCKS);
   w->block_count = c.take<double>(JOIN_BLOCKS);
@@ -911,7 +915,7 @@ inline size_t carve_bwd(void* base, const Dims& d, BwdWs* w) {
   Carver c{(char*)base};
   w->part_x = c.take<float>((size_t)d.x_tiles * TILE * d.dx_splits * d.D);
   w->part_w = c.take<float>((size_t)d.w_tiles * TILE * d.dw_splits * d.D);
-  w->part_bias = c.take<float>((size_t)d.w_tiles * TILE * d.dw_splits * 2);
+  w->part_bias = c.take<float>((size_t)d.w_tiles * TILE * d.dw_splits * d.dw_slots);
   w->row_u = c.take<float>((size_t)d.x_tiles * TILE);
   return c.off;
 }
@@ -956,8 +960,9 @@ int launch_tiled(StreamArgs g, cudaStream_t s) {
     if (g.a_slots * a_bytes + 6 * stage + fixed <= SMEM_MAX) break;
   g.stages = (int)std::min<size_t>(MAX_STAGES, (SMEM_MAX - fixed - g.a_slots * a_bytes) / stage);
   const int acc = MODE == FWD ? 0 : ACCS * g.D8 * 8;
-  g.z_shift = 4 * SBUF + acc <= TMEM_COLUMNS ? 2 : 1;
-  g.acc_slots = (SBUF << g.z_shift) + 2 * acc <= TMEM_COLUMNS ? 2 : 1;
+  static_assert(GROUPS * SBUF <= TMEM_COLUMNS, "z buffers");
+  g.acc_slots = GROUPS * SBUF + 2 * acc <= TMEM_COLUMNS ? 2 : 1;
+  g.distance = std::min(GROUPS - 1, g.stages - 1);
   const size_t smem = std::max(SMEM_MIN, g.a_slots * a_bytes + g.stages * stage + fixed);
   cudaFuncSetAttribute(stream_kernel<MODE, NP, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   const int units = g.a_tiles * g.splits;
@@ -1029,6 +1034,7 @@ GSB_EXPORT int gsb_class_loss_fwd(const gsb_class_loss_args* a, void* stream) {
   g.a_tiles = (int)d.x_tiles;
   g.b_tiles = d.fwd_cols;
   g.splits = d.fwd_splits;
+  g.slots = d.fwd_slots;
   g.error_word = a->error_word;
   g.D8 = d.D8;
   g.part_m = w.part_m;
@@ -1042,7 +1048,7 @@ GSB_EXPORT int gsb_class_loss_fwd(const gsb_class_loss_args* a, void* stream) {
     if (r != GSB_OK) return r;
   }
   const int blocks = (int)std::max(1ll, std::min<long long>(JOIN_BLOCKS, (d.x_tiles * TILE + THREADS - 1) / THREADS));
-  join_rows_kernel<<<blocks, THREADS, 0, s>>>(g, 2 * d.fwd_splits, d.N, a->row_lse2, a->row_y,
+  join_rows_kernel<<<blocks, THREADS, 0, s>>>(g, d.fwd_splits * d.fwd_slots, d.N, a->row_lse2, a->row_y,
                                               a->reduction == GSB_REDUCE_NONE ? a->loss : nullptr, w.block_loss,
                                               w.block_count);
   finish_loss_kernel<<<1, THREADS, 0, s>>>(w.block_loss, w.block_count, blocks, a->reduction, a->loss, a->inv_count);
@@ -1093,6 +1099,7 @@ GSB_EXPORT int gsb_class_loss_bwd(const gsb_class_loss_args* a, void* stream) {
     g.a_tiles = (int)d.w_tiles;
     g.b_tiles = d.dw_cols;
     g.splits = d.dw_splits;
+    g.slots = d.dw_slots;
     g.part_acc = w.part_w;
     g.part_bias = w.part_bias;
     if (a->reduction == GSB_REDUCE_NONE) {
@@ -1102,7 +1109,7 @@ GSB_EXPORT int gsb_class_loss_bwd(const gsb_class_loss_args* a, void* stream) {
     const int r = launch_stream<DW>(g, d.planes, d.dw_tn, s);
     if (r != GSB_OK) return r;
     join_dw_kernel<<<blocks_for(a->V * (a->C + 1ll)), THREADS, 0, s>>>(*a, w.part_w, w.part_bias, d.dw_splits,
-                                                                      2 * d.dw_splits, d.D, d.w_tiles * TILE);
+                                                                      d.dw_splits * d.dw_slots, d.D, d.w_tiles * TILE);
   }
   return check_launch("gsb_class_loss_bwd");
 }
