@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(THREADS) pack_classes_kernel(const gsb_class_l
 // ---------------------------------------------------------------------------
 // The streaming pass: one persistent CTA per SM.  A work unit is a resident
 // tile of 128 rows and a range of the streamed operand's tiles of TN rows
-// (columns of z).  One warp loads, one issues the matrix instructions, two
+// (columns of z).  One warp loads, two issue the matrix instructions, four
 // groups of four warps take the tiles of z in turn, and in the gradient
 // passes four more warps store finished accumulators while the next unit
 // runs.  A thread owns one row of z (a lane of tensor memory):
@@ -153,7 +153,7 @@ enum { FWD = 0, DX = 1, DW = 2 };
 constexpr int MAX_STAGES = 16, MAX_A_SLOTS = 4;
 constexpr int TMEM_COLUMNS = 512;
 constexpr int GROUPS = 4;                      // consumer groups of four warps, one z buffer each
-constexpr int LOADER = GROUPS * 4, ISSUER = LOADER + 1;  // warps
+constexpr int LOADER = GROUPS * 4, ISSUER = LOADER + 1, ISSUER2 = LOADER + 2;  // warps
 
 struct StreamArgs {
   const uint4* a;          // resident operand, packed
@@ -165,7 +165,6 @@ struct StreamArgs {
   int a_tiles, b_tiles, splits, D8;
   int a_slots, stages, acc_slots;
   int slots;               // partial results a unit leaves: its groups that had a tile
-  int distance;            // tiles between a tile's two products
   int flush;               // tiles per accumulator
   float* part_m;           // FWD: [split][slot][row]
   float* part_s;
@@ -177,7 +176,7 @@ struct StreamArgs {
 
 struct Barriers {
   uint64_t a_full[MAX_A_SLOTS], a_empty[MAX_A_SLOTS], b_full[MAX_STAGES], b_empty[MAX_STAGES];
-  uint64_t s_full[GROUPS], s_free[GROUPS], p_full[GROUPS], acc_full[2], acc_empty[2], drained;
+  uint64_t s_full[GROUPS], s_free[GROUPS], p_full[GROUPS], acc_full[2], acc_empty[2], drained[2];
   uint32_t tmem;
   int stop;
 };
@@ -204,7 +203,7 @@ __host__ __device__ constexpr int chain_products(int np) { return np == 3 ? 16 :
 template <int MODE>
 __host__ __device__ constexpr int meta_floats(int tn) { return MODE == DW ? 3 * tn : tn; }
 template <int MODE>
-__host__ __device__ constexpr int stream_threads() { return (MODE == FWD ? GROUPS * 4 + 2 : GROUPS * 4 + 6) * 32; }
+__host__ __device__ constexpr int stream_threads() { return (MODE == FWD ? GROUPS * 4 + 2 : GROUPS * 4 + 7) * 32; }
 
 // A position in a ring of buffers and the parity of its current round.
 struct Ring {
@@ -309,7 +308,7 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
   float* const sMeta = reinterpret_cast<float*>(sB + (size_t)g.stages * b_bytes);
   Barriers* const bar = reinterpret_cast<Barriers*>(sMeta + (size_t)g.stages * META);
   volatile int* const stop = &bar->stop;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int units = g.a_tiles * g.splits;
   constexpr int SBUF = z_columns<MODE>(NP, TN);
   constexpr int ACCS = accumulators(NP);
@@ -334,7 +333,7 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
       mbar_init(&bar->b_full[i], 1);
       mbar_init(&bar->b_empty[i], 1 + 4);  // the last product, and the group's warps (bias, sums, labels)
     }
-    mbar_init(&bar->drained, 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&bar->drained[i], 1);
     mbar_init_fence();
   }
   if (warp == ISSUER) tmem_alloc(&bar->tmem, TMEM_COLUMNS);
@@ -350,7 +349,7 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
     bool ok = true;
     for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
       const Range r = unit_range(g, u);
-      ok = __all_sync(0xffffffffu, mbar_wait(&bar->a_empty[as.i], as.phase ^ 1, stop));
+      ok = warp_wait(&bar->a_empty[as.i], as.phase ^ 1, stop);
       if (!ok) break;
       if (lane == 0) mbar_expect(&bar->a_full[as.i], a_bytes);
       __syncwarp();
@@ -361,7 +360,7 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
       }
       as.next(g.a_slots);
       for (int bt = r.lo; bt < r.hi; ++bt) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&bar->b_empty[bs.i], bs.phase ^ 1, stop));
+        ok = warp_wait(&bar->b_empty[bs.i], bs.phase ^ 1, stop);
         if (!ok) break;
         uint64_t* full = &bar->b_full[bs.i];
         const bool with_u = MODE == DW && g.row_u;
@@ -389,86 +388,77 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
         mbar_wait(&bar->a_full[i], i < as.i ? as.phase : as.phase ^ 1, &never);
     }
   } else if (warp == ISSUER) {
-    // ---- matrix instructions ----
-    if (lane == 0) {
-      const uint32_t idesc1 = instr_desc(TN, false), idesc2 = instr_desc(D, true);
-      const uint32_t hi1 = desc_hi(128), hi2 = desc_hi(TN * 16);
-      const uint32_t a0 = smem_u32(sA), b0 = smem_u32(sB);
-      bool ok = true;
-
-      auto first_product = [&](Cursor& c) {
-        const uint32_t b = c.t % GROUPS;
-        if (c.bt == c.r.lo && !mbar_wait(&bar->a_full[c.as.i], c.as.phase, stop)) return false;
-        if (!mbar_wait(&bar->b_full[c.bs.i], c.bs.phase, stop)) return false;
-        if (!mbar_wait(&bar->s_free[b], ((c.t / GROUPS) & 1) ^ 1, stop)) return false;
-        fence_after();
-        const uint32_t a_lo = desc_lo(a0 + c.as.i * a_bytes, 2048), b_lo = desc_lo(b0 + c.bs.i * b_bytes, TN * 16);
-        const uint32_t z = tmem + b * SBUF;
+    // ---- first products: z ----
+    const uint32_t leader = elect_leader();
+    const uint32_t idesc = instr_desc(TN, false), hi = desc_hi(128);
+    const uint32_t a0 = smem_u32(sA), b0 = smem_u32(sB);
+    bool ok = true;
+    for (Cursor c(g); c.unit < units; c.next(g)) {
+      const uint32_t b = c.t % GROUPS;
+      ok = (c.bt > c.r.lo || warp_wait(&bar->a_full[c.as.i], c.as.phase, stop)) &&
+           warp_wait(&bar->b_full[c.bs.i], c.bs.phase, stop) &&
+           warp_wait(&bar->s_free[b], ((c.t / GROUPS) & 1) ^ 1, stop);
+      if (!ok) break;
+      fence_after();
+      const uint32_t a_lo = desc_lo(a0 + c.as.i * a_bytes, 2048), b_lo = desc_lo(b0 + c.bs.i * b_bytes, TN * 16);
+      const uint32_t z = tmem + b * SBUF;
 #pragma unroll
-        for (int q = 0; q < plane_products(NP); ++q) {
-          const uint32_t aq = a_lo + plane_of_a(NP, q) * D8 * 128, bq = b_lo + plane_of_b(NP, q) * D8 * TN;
-          mma_ss(z, aq, hi1, bq, hi1, idesc1, q > 0);
+      for (int q = 0; q < plane_products(NP); ++q) {
+        const uint32_t aq = a_lo + plane_of_a(NP, q) * D8 * 128, bq = b_lo + plane_of_b(NP, q) * D8 * TN;
+        mma_ss(leader, z, aq, hi, bq, hi, idesc, q > 0);
 #pragma unroll 4
-          for (int k = 2; k < D8; k += 2) mma_ss(z, aq + k * 128, hi1, bq + k * TN, hi1, idesc1, true);
-        }
-        mma_commit(&bar->s_full[b]);
-        if (c.bt + 1 == c.r.hi) mma_commit(&bar->a_empty[c.as.i]);
-        if (MODE == FWD) mma_commit(&bar->b_empty[c.bs.i]);
-        return true;
-      };
-
-      auto second_product = [&](Cursor& c) {
-        const uint32_t b = c.t % GROUPS;
-        const int in_acc = (c.bt - c.r.lo) % g.flush;
-        const bool first = in_acc == 0, last = in_acc + 1 == g.flush || c.bt + 1 == c.r.hi;
-        if (!mbar_wait(&bar->p_full[b], (c.t / GROUPS) & 1, stop)) return false;
-        if (first && !mbar_wait(&bar->acc_empty[c.acc.i], c.acc.phase ^ 1, stop)) return false;
-        fence_after();
-        const uint32_t dst = tmem + ACC0 + c.acc.i * ACCS * D, p = tmem + b * SBUF;
-        const uint32_t b_lo = desc_lo(b0 + c.bs.i * b_bytes, 128);
-#pragma unroll
-        for (int q = 0; q < plane_products(NP); ++q) {
-          const int pa = plane_of_a(NP, q);
-          const bool main = q + 1 == plane_products(NP);
-          const uint32_t to = ACCS == 2 && !main ? dst + D : dst;
-          const uint32_t bq = b_lo + plane_of_b(NP, q) * D8 * TN;
-#pragma unroll
-          for (int k = 0; k < TN / 16; ++k)
-            mma_ts(to, p + p_column(TN, 16 * k, pa), bq + k * 16, hi2,
-                   idesc2, k > 0 || (q > 0 && !(ACCS == 2 && main)) || !first);
-        }
-        mma_commit(&bar->b_empty[c.bs.i]);
-        mma_commit(&bar->s_free[b]);
-        if (last) {
-          mma_commit(&bar->acc_full[c.acc.i]);
-          c.acc.next(g.acc_slots);
-        }
-        return true;
-      };
-
-      // The second product of a tile follows the first ones of the next
-      // groups' tiles, so that P of one group is awaited while the others
-      // have work.
-      Cursor c1(g), c2(g);
-      const uint32_t distance = g.distance;
-      while (ok && c1.unit < units) {
-        ok = first_product(c1);
-        c1.next(g);
-        if (MODE != FWD && ok && c1.t > distance) {
-          ok = second_product(c2);
-          c2.next(g);
-        }
+        for (int k = 2; k < D8; k += 2) mma_ss(leader, z, aq + k * 128, hi, bq + k * TN, hi, idesc, true);
       }
-      if (MODE != FWD)
-        for (; ok && c2.unit < units; c2.next(g)) ok = second_product(c2);
-      if (!ok) {
-        // what was issued ends before the tensor memory is freed
-        int never = 0;
-        mma_commit(&bar->drained);
-        mbar_wait(&bar->drained, 0, &never);
+      mma_commit(leader, &bar->s_full[b]);
+      if (c.bt + 1 == c.r.hi) mma_commit(leader, &bar->a_empty[c.as.i]);
+      if (MODE == FWD) mma_commit(leader, &bar->b_empty[c.bs.i]);
+    }
+    if (!ok) {
+      // what was issued ends before the tensor memory is freed
+      int never = 0;
+      mma_commit(leader, &bar->drained[0]);
+      mbar_wait(&bar->drained[0], 0, &never);
+    }
+  } else if (MODE != FWD && warp == ISSUER2) {
+    // ---- second products: the accumulators.  A warp of its own, so that waiting for one group's P does not
+    // hold up the next group's z ----
+    const uint32_t leader = elect_leader();
+    const uint32_t idesc = instr_desc(D, true), hi = desc_hi(TN * 16);
+    const uint32_t b0 = smem_u32(sB);
+    bool ok = true;
+    for (Cursor c(g); c.unit < units; c.next(g)) {
+      const uint32_t b = c.t % GROUPS;
+      const int in_acc = (c.bt - c.r.lo) % g.flush;
+      const bool first = in_acc == 0, last = in_acc + 1 == g.flush || c.bt + 1 == c.r.hi;
+      ok = (!first || warp_wait(&bar->acc_empty[c.acc.i], c.acc.phase ^ 1, stop)) &&
+           warp_wait(&bar->p_full[b], (c.t / GROUPS) & 1, stop);
+      if (!ok) break;
+      fence_after();
+      const uint32_t dst = tmem + ACC0 + c.acc.i * ACCS * D, p = tmem + b * SBUF;
+      const uint32_t b_lo = desc_lo(b0 + c.bs.i * b_bytes, 128);
+#pragma unroll
+      for (int q = 0; q < plane_products(NP); ++q) {
+        const int pa = plane_of_a(NP, q);
+        const bool main = q + 1 == plane_products(NP);
+        const uint32_t to = ACCS == 2 && !main ? dst + D : dst;
+        const uint32_t bq = b_lo + plane_of_b(NP, q) * D8 * TN;
+#pragma unroll
+        for (int k = 0; k < TN / 16; ++k)
+          mma_ts(leader, to, p + p_column(TN, 16 * k, pa), bq + k * 16, hi, idesc,
+                 k > 0 || (q > 0 && !(ACCS == 2 && main)) || !first);
+      }
+      mma_commit(leader, &bar->b_empty[c.bs.i]);
+      mma_commit(leader, &bar->s_free[b]);
+      if (last) {
+        mma_commit(leader, &bar->acc_full[c.acc.i]);
+        c.acc.next(g.acc_slots);
       }
     }
-    __syncwarp();
+    if (!ok) {
+      int never = 0;
+      mma_commit(leader, &bar->drained[1]);
+      mbar_wait(&bar->drained[1], 0, &never);
+    }
   } else if (warp < LOADER) {
     // ---- z -> row statistics, or P ----
     constexpr int CH = MODE == FWD ? 32 : 16;  // columns in registers at a time
@@ -500,8 +490,7 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
       for (int bt = r.lo; bt < r.hi; ++bt, ++t, bs.next(g.stages)) {
         if ((int)(t % GROUPS) != group) continue;
         // the meta data comes with the tile that z is made of
-        ok = __all_sync(0xffffffffu, mbar_wait(&bar->b_full[bs.i], bs.phase, stop) &&
-                                         mbar_wait(&bar->s_full[group], (t / GROUPS) & 1, stop));
+        ok = warp_wait(&bar->b_full[bs.i], bs.phase, stop) && warp_wait(&bar->s_full[group], (t / GROUPS) & 1, stop);
         if (!ok) break;
         fence_after();
         const float* meta = sMeta + bs.i * META;
@@ -640,7 +629,7 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
       const size_t tile = (size_t)r.split * g.a_tiles + r.tile;
       float4* const dst = reinterpret_cast<float4*>(g.part_acc) + tile * (D / 4) * TILE + (warp & 3) * 32 + lane;
       for (int bt = r.lo; bt < r.hi; bt += g.flush) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&bar->acc_full[acc.i], acc.phase, stop));
+        ok = warp_wait(&bar->acc_full[acc.i], acc.phase, stop);
         if (!ok) break;
         fence_after();
         const uint32_t src = tmem + lanes + ACC0 + acc.i * ACCS * D;
@@ -962,7 +951,6 @@ int launch_tiled(StreamArgs g, cudaStream_t s) {
   const int acc = MODE == FWD ? 0 : ACCS * g.D8 * 8;
   static_assert(GROUPS * SBUF <= TMEM_COLUMNS, "z buffers");
   g.acc_slots = GROUPS * SBUF + 2 * acc <= TMEM_COLUMNS ? 2 : 1;
-  g.distance = std::min(GROUPS - 1, g.stages - 1);
   const size_t smem = std::max(SMEM_MIN, g.a_slots * a_bytes + g.stages * stage + fixed);
   cudaFuncSetAttribute(stream_kernel<MODE, NP, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   const int units = g.a_tiles * g.splits;

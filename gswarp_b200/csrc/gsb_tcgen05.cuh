@@ -65,6 +65,11 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   return false;
 }
 
+// The same for a whole warp, which stays together.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* stop) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, stop));
+}
+
 // ---- bulk copies (16-byte aligned addresses and sizes) ----
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
@@ -122,27 +127,37 @@ __device__ __forceinline__ uint32_t desc_hi(uint32_t stride) { return stride >> 
 __device__ __forceinline__ uint32_t instr_desc(int n, bool b_mn_major) {
   return 1u << 4 | 1u << 7 | 1u << 10 | (b_mn_major ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (128u >> 4) << 24;
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
+// The issuing warp runs these with all lanes, so that operands stay in uniform
+// registers; `leader` picks the lane (one, the same every time) that issues.
+__device__ __forceinline__ uint32_t elect_leader() {
+  uint32_t leader;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(leader));
+  return leader;
+}
+__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo,
+                                       uint32_t b_hi, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n.reg .pred p, e;\n.reg .b64 a, b;\nsetp.ne.u32 p, %6, 0;\nsetp.ne.u32 e, %7, 0;\n"
+      "mov.b64 a, {%1, %2};\nmov.b64 b, {%3, %4};\n"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n}\n" ::"r"(d),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"((uint32_t)accumulate), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi,
                                        uint32_t idesc, bool accumulate) {
   asm volatile(
-      "{\n.reg .pred p;\n.reg .b64 a, b;\nsetp.ne.u32 p, %6, 0;\n"
-      "mov.b64 a, {%1, %2};\nmov.b64 b, {%3, %4};\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n}\n" ::"r"(d),
-      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"((uint32_t)accumulate)
+      "{\n.reg .pred p, e;\n.reg .b64 b;\nsetp.ne.u32 p, %5, 0;\nsetp.ne.u32 e, %6, 0;\nmov.b64 b, {%2, %3};\n"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"((uint32_t)accumulate), "r"(leader)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
-                                       bool accumulate) {
+// Arrives on `bar` once every matrix instruction the leader has issued is done.
+__device__ __forceinline__ void mma_commit(uint32_t leader, uint64_t* bar) {
   asm volatile(
-      "{\n.reg .pred p;\n.reg .b64 b;\nsetp.ne.u32 p, %5, 0;\nmov.b64 b, {%2, %3};\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}\n" ::"r"(d),
-      "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"((uint32_t)accumulate)
+      "{\n.reg .pred e;\nsetp.ne.u32 e, %1, 0;\n"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar)),
+      "r"(leader)
       : "memory");
-}
-// Arrives on `bar` once every matrix instruction issued so far is done.
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
 }
 
 }  // namespace tc
