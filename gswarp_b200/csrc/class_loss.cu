@@ -22,6 +22,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "gsb_common.cuh"
 #include "gsb_tcgen05.cuh"
@@ -46,11 +47,10 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-__device__ __forceinline__ float load_elem(const void* p, long long i, int dtype) {
-  if (dtype == GSB_TYPE_FP32) return ((const float*)p)[i];
-  if (dtype == GSB_TYPE_BF16) return __bfloat162float(((const __nv_bfloat16*)p)[i]);
-  return __half2float(((const __half*)p)[i]);
-}
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+
 __device__ __forceinline__ void store_elem(void* p, long long i, int dtype, float v) {
   if (dtype == GSB_TYPE_FP32) ((float*)p)[i] = v;
   else if (dtype == GSB_TYPE_BF16) ((__nv_bfloat16*)p)[i] = __float2bfloat16_rn(v);
@@ -60,11 +60,13 @@ __device__ __forceinline__ void store_elem(void* p, long long i, int dtype, floa
 // ---------------------------------------------------------------------------
 // Packing.  Tile layout: [plane][column / 8][row][8 columns] of bf16.
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ void store_planes(uint4* tile, int D8, int d8, int row, const float (&x)[8], int planes) {
+template <int PLANES>
+__device__ __forceinline__ void store_planes(uint4* tile, int D8, int d8, int row, const float (&x)[8]) {
   float rest[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) rest[i] = x[i];
-  for (int p = 0; p < planes; ++p) {
+#pragma unroll
+  for (int p = 0; p < PLANES; ++p) {
     __nv_bfloat162 h[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -78,60 +80,77 @@ __device__ __forceinline__ void store_planes(uint4* tile, int D8, int d8, int ro
   }
 }
 
-// One thread per (tile, 8 columns, row); rows without a label are zero.
-__global__ void __launch_bounds__(THREADS) pack_rows_kernel(const gsb_class_loss_args a, int D8, long long total,
-                                                            uint4* __restrict__ packed, int* __restrict__ row_y) {
-  const int planes = planes_of(a.dtype);
-  const long long N = a.B * a.S;
-  for (long long i = (long long)blockIdx.x * THREADS + threadIdx.x; i < total; i += (long long)gridDim.x * THREADS) {
-    const int row = (int)(i % TILE);
-    const int d8 = (int)(i / TILE % D8);
-    const long long tile = i / TILE / D8;
-    const long long n = tile * TILE + row;
-    int y = -1;
-    if (n < N) {
-      const long long l = a.labels64 ? ((const long long*)a.labels)[n] : (long long)((const int*)a.labels)[n];
-      if (l != a.ignore_index) {
-        if (l >= 0 && l < a.V) y = (int)l;
-        else if (d8 == 0) atomicOr((unsigned long long*)a.error_word, (unsigned long long)ERR_BAD_LABEL);
-      }
-    }
-    if (d8 == 0) row_y[n] = y;
-    float x[8];
-    const long long b = y >= 0 ? n / a.S : 0;
-    const long long at = b * a.stride_b + (n - b * a.S) * a.stride_s;
+// Eight neighbouring elements of a row, from column c on; zero past C.
+template <typename T>
+__device__ __forceinline__ void load8(const T* at, long long stride, int c, int C, bool wide, float (&x)[8]) {
+  if (wide) {  // contiguous, aligned and whole
+    if constexpr (sizeof(T) == 4) {
+      const float4 lo = *reinterpret_cast<const float4*>(at + c), hi = *reinterpret_cast<const float4*>(at + c + 4);
+      x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w, x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
+    } else {
+      const uint4 raw = *reinterpret_cast<const uint4*>(at + c);
+      const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int c = d8 * 8 + k;
-      x[k] = y >= 0 && c < a.C ? load_elem(a.features, at + c * a.stride_c, a.dtype) : 0.f;
+      for (int k = 0; k < 8; ++k) x[k] = to_float(e[k]);
     }
-    store_planes(packed + (size_t)tile * planes * D8 * TILE, D8, d8, row, x, planes);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = c + k < C ? to_float(at[(c + k) * stride]) : 0.f;
   }
 }
 
-// The classifier's rows and its bias in base 2.  A class with the bias -inf
-// takes no part and its row is not read; finite biases stay finite.
-__global__ void __launch_bounds__(THREADS) pack_classes_kernel(const gsb_class_loss_args a, int D8, long long total,
-                                                               uint4* __restrict__ packed, float* __restrict__ b2) {
-  const int planes = planes_of(a.dtype);
-  for (long long i = (long long)blockIdx.x * THREADS + threadIdx.x; i < total; i += (long long)gridDim.x * THREADS) {
-    const int row = (int)(i % TILE);
-    const int d8 = (int)(i / TILE % D8);
-    const long long tile = i / TILE / D8;
-    const long long v = tile * TILE + row;
+// A CTA packs one tile: the classifier's tiles first (with the bias in base
+// 2), then the rows' (with their labels).  Ignored rows, rows past the end and
+// classes that take no part are zero and their elements are not read; finite
+// biases stay finite.
+template <typename T>
+__global__ void __launch_bounds__(THREADS) pack_kernel(const gsb_class_loss_args a, int D8, int w_tiles,
+                                                       int* __restrict__ ticket) {
+  constexpr int PLANES = sizeof(T) == 4 ? 3 : std::is_same<T, __half>::value ? 2 : 1;
+  const int row = threadIdx.x % TILE;
+  const bool classes = (int)blockIdx.x < w_tiles;
+  const long long tile = classes ? blockIdx.x : blockIdx.x - w_tiles;
+  const long long n = tile * TILE + row;
+  bool used;
+  const T* at;
+  long long stride;
+  if (classes) {
     float bias = -INFINITY;
-    if (v < a.V) {
-      bias = a.bias ? a.bias[v] : 0.f;
+    if (n < a.V) {
+      bias = a.bias ? a.bias[n] : 0.f;
       if (isfinite(bias)) bias = fminf(fmaxf(bias, -2e38f), 2e38f) * LOG2E;
     }
-    if (d8 == 0) b2[v] = bias;
-    float x[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int c = d8 * 8 + k;
-      x[k] = bias != -INFINITY && c < a.C ? load_elem(a.weight, v * a.C + c, a.dtype) : 0.f;
+    used = bias != -INFINITY;
+    at = (const T*)a.weight + n * a.C;
+    stride = 1;
+    if (threadIdx.x < TILE) a.class_bias2[n] = bias;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0;
+  } else {
+    int y = -1;
+    if (n < a.B * a.S) {
+      const long long l = a.labels64 ? ((const long long*)a.labels)[n] : (long long)((const int*)a.labels)[n];
+      if (l != a.ignore_index) {
+        if (l >= 0 && l < a.V) y = (int)l;
+        else atomicOr((unsigned long long*)a.error_word, (unsigned long long)ERR_BAD_LABEL);
+      }
     }
-    store_planes(packed + (size_t)tile * planes * D8 * TILE, D8, d8, row, x, planes);
+    if (threadIdx.x < TILE) a.row_y[n] = y;
+    used = y >= 0;
+    const unsigned b = a.B > 1 ? (unsigned)n / (unsigned)max(a.S, 1ll) : 0u;
+    at = (const T*)a.features + b * a.stride_b + (n - b * a.S) * a.stride_s;
+    stride = a.stride_c;
+  }
+  const bool contiguous = stride == 1 && (uintptr_t)at % 16 == 0;
+  uint4* const out = (uint4*)(classes ? a.packed_w : a.packed_x) + (size_t)tile * PLANES * D8 * TILE;
+  for (int d8 = threadIdx.x / TILE; d8 < D8; d8 += THREADS / TILE) {
+    float x[8];
+    if (used) {
+      load8(at, stride, d8 * 8, a.C, contiguous && d8 * 8 + 8 <= a.C, x);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = 0.f;
+    }
+    store_planes<PLANES>(out, D8, d8, row, x);
   }
 }
 
@@ -155,6 +174,63 @@ constexpr int TMEM_COLUMNS = 512;
 constexpr int GROUPS = 4;                      // consumer groups of four warps, one z buffer each
 constexpr int LOADER = GROUPS * 4, ISSUER = LOADER + 1, ISSUER2 = LOADER + 2;  // warps
 
+// Where and how a gradient is written: element (n, c), times the loss's
+// upstream gradient (of the row, or over the count of rows).
+struct GradOut {
+  void* out;
+  const float* upstream;
+  const float* inv_count;  // null: upstream has one factor per row
+  const int* y;            // rows without a gradient are zero (null: every row has one)
+  long long rows, S;       // S > 0: n = b * S + s, written as (b, c, s); S = 0: (n, c)
+  int C, dtype;
+};
+__device__ __forceinline__ float grad_scale(const GradOut& o, long long n) {
+  if (o.y && o.y[n] < 0) return 0.f;
+  return o.inv_count ? o.upstream[0] * o.inv_count[0] : o.upstream ? o.upstream[n] : 1.f;
+}
+// Columns c .. c + COUNT - 1 of row n; u from grad_scale.
+template <int COUNT>
+__device__ __forceinline__ void write_grad(const GradOut& o, long long n, int c, const float (&v)[COUNT], float u) {
+  long long at, step = 1;
+  if (o.S > 0) {
+    const unsigned b = (unsigned)n / (unsigned)o.S;
+    at = ((long long)b * o.C + c) * o.S + (n - b * o.S);
+    step = o.S;
+  } else {
+    at = n * o.C + c;
+    const int size = o.dtype == GSB_TYPE_FP32 ? 4 : 2;
+    if (c + COUNT <= o.C && (at * size + (long long)(uintptr_t)o.out) % 16 == 0 && COUNT * size % 16 == 0) {
+      if (o.dtype == GSB_TYPE_FP32) {
+#pragma unroll
+        for (int i = 0; i < COUNT / 4; ++i)
+          reinterpret_cast<float4*>((float*)o.out + at)[i] =
+              make_float4(u == 0.f ? 0.f : v[4 * i] * u, u == 0.f ? 0.f : v[4 * i + 1] * u,
+                          u == 0.f ? 0.f : v[4 * i + 2] * u, u == 0.f ? 0.f : v[4 * i + 3] * u);
+      } else {
+        uint32_t h[COUNT / 2];
+#pragma unroll
+        for (int i = 0; i < COUNT / 2; ++i) {
+          const float p = u == 0.f ? 0.f : v[2 * i] * u, q = u == 0.f ? 0.f : v[2 * i + 1] * u;
+          if (o.dtype == GSB_TYPE_BF16) {
+            const __nv_bfloat162 w = __floats2bfloat162_rn(p, q);
+            h[i] = *reinterpret_cast<const uint32_t*>(&w);
+          } else {
+            const __half2 w = __floats2half2_rn(p, q);
+            h[i] = *reinterpret_cast<const uint32_t*>(&w);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < COUNT / 8; ++i)
+          reinterpret_cast<uint4*>((uint16_t*)o.out + at)[i] = make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < COUNT; ++i)
+    if (c + i < o.C) store_elem(o.out, at + i * step, o.dtype, u == 0.f ? 0.f : v[i] * u);
+}
+
 struct StreamArgs {
   const uint4* a;          // resident operand, packed
   const uint4* b;          // streamed operand, packed
@@ -171,6 +247,7 @@ struct StreamArgs {
   float* t_label;          // FWD: [row]
   float* part_acc;         // DX, DW: [split][tile][column / 4][row][4 columns]
   float* part_bias;        // DW: [split][slot][row]
+  GradOut grad;            // DX, DW with one split: written by the pass itself
   long long* error_word;
 };
 
@@ -621,43 +698,69 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
       }
     }
   } else if (MODE != FWD) {
-    // ---- finished accumulators: added up in fp32 in the unit's partial rows ----
+    // ---- finished accumulators: added up in fp32 in the unit's partial rows, the last one (where the unit has
+    // all of the streamed axis) straight into the gradient ----
     Ring acc;
     bool ok = true;
     for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
       const Range r = unit_range(g, u);
       const size_t tile = (size_t)r.split * g.a_tiles + r.tile;
-      float4* const dst = reinterpret_cast<float4*>(g.part_acc) + tile * (D / 4) * TILE + (warp & 3) * 32 + lane;
+      const int row = (warp & 3) * 32 + lane;
+      const long long n = (long long)r.tile * TILE + row;
+      float4* const dst = reinterpret_cast<float4*>(g.part_acc) + tile * (D / 4) * TILE + row;
+      const bool direct = g.grad.out != nullptr, inside = direct && n < g.grad.rows;
+      const float scale = inside ? grad_scale(g.grad, n) : 0.f;
       for (int bt = r.lo; bt < r.hi; bt += g.flush) {
         ok = warp_wait(&bar->acc_full[acc.i], acc.phase, stop);
         if (!ok) break;
         fence_after();
         const uint32_t src = tmem + lanes + ACC0 + acc.i * ACCS * D;
+        if (!direct && !g.part_acc) {  // only the bias is wanted
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar->acc_empty[acc.i]);
+          acc.next(g.acc_slots);
+          continue;
+        }
         for (int c = 0; c < D; c += 16) {
           float4* at = dst + (size_t)(c / 4) * TILE;
-          float4 v[4];
+          float4 old[4];
+          if (bt > r.lo) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] = bt > r.lo ? at[i * TILE] : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int i = 0; i < 4; ++i) old[i] = at[i * TILE];
+          }
           uint32_t main[16];
+          float v[16];
           tmem_load(src + c, main);
           tmem_load_wait(main);
-          if (ACCS == 2) {
-            uint32_t rest[16];
-            tmem_load(src + D + c, rest);
-            tmem_load_wait(rest);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) main[i] = __float_as_uint(__uint_as_float(main[i]) + __uint_as_float(rest[i]));
+          for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(main[i]);
+          if (ACCS == 2) {
+            tmem_load(src + D + c, main);
+            tmem_load_wait(main);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] += __uint_as_float(main[i]);
           }
           if (c + 16 >= D) {
             fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar->acc_empty[acc.i]);
           }
+          if (bt > r.lo) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            at[i * TILE] = make_float4(v[i].x + __uint_as_float(main[4 * i]), v[i].y + __uint_as_float(main[4 * i + 1]),
-                                       v[i].z + __uint_as_float(main[4 * i + 2]),
-                                       v[i].w + __uint_as_float(main[4 * i + 3]));
+            for (int i = 0; i < 4; ++i) {
+              v[4 * i] += old[i].x;
+              v[4 * i + 1] += old[i].y;
+              v[4 * i + 2] += old[i].z;
+              v[4 * i + 3] += old[i].w;
+            }
+          }
+          if (direct && bt + g.flush >= r.hi) {
+            if (inside) write_grad(g.grad, n, c, v, scale);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) at[i * TILE] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+          }
         }
         acc.next(g.acc_slots);
       }
@@ -687,63 +790,83 @@ __device__ __forceinline__ double block_sum(double v) {
   return t;
 }
 
-// Joins the slots' (maximum, sum) pairs of every row, in slot order.  A label
-// whose class takes no part (bias -inf) has the loss +inf and no gradient.
-__global__ void __launch_bounds__(THREADS) join_rows_kernel(const StreamArgs g, int slots, long long N,
-                                                            float* __restrict__ lse2, int* __restrict__ row_y,
-                                                            float* __restrict__ row_loss,
-                                                            double* __restrict__ block_loss,
-                                                            double* __restrict__ block_count) {
-  const long long rows = (long long)g.a_tiles * TILE;
+// Joins the slots' (maximum, sum) pairs of every row: LANES threads per row
+// take every LANES-th slot and are joined in a fixed order (8 where a few rows
+// have hundreds of slots: 37 rows of 50,001 classes 63 -> 5 us).  A label whose
+// class takes no part (bias -inf) has the loss +inf and no gradient.  The last
+// CTA to finish adds up the CTAs' sums in their order.
+template <int LANES>
+__global__ void __launch_bounds__(THREADS) join_rows_kernel(const gsb_class_loss_args a, const float* __restrict__ part_m,
+                                                            const float* __restrict__ part_s,
+                                                            const float* __restrict__ t_label, int slots,
+                                                            long long rows, double* __restrict__ block_loss,
+                                                            double* __restrict__ block_count, int* __restrict__ ticket) {
+  const long long N = a.B * a.S;
   double loss = 0.0, count = 0.0;
-  for (long long n = (long long)blockIdx.x * THREADS + threadIdx.x; n < rows; n += (long long)gridDim.x * THREADS) {
-    const int y = g.y[n];
-    float l2 = INFINITY, l = 0.f;
-    if (y >= 0) {
-      float m = -INFINITY, s = 0.f;
-      for (int k = 0; k < slots; ++k) m = fmaxf(m, g.part_m[k * rows + n]);
-      const float base = m == -INFINITY ? 0.f : m;
-      for (int k = 0; k < slots; ++k) s += g.part_s[k * rows + n] * ex2(g.part_m[k * rows + n] - base);
-      const float t = g.t_label[n];
-      count += 1.0;
-      if (t == -INFINITY) {
-        l = INFINITY;
-        row_y[n] = -1;
-      } else {
-        // two addends instead of lse2 - t: the maximum and t often agree in most of their digits
-        const float ls = log2f(s);
-        l = (float)(((double)(base - t) + (double)ls) * LN2);
-        l2 = base + ls;
+  const int sub = threadIdx.x % LANES;
+  for (long long n0 = (long long)blockIdx.x * (THREADS / LANES); n0 < rows;
+       n0 += (long long)gridDim.x * (THREADS / LANES)) {
+    const long long n = n0 + threadIdx.x / LANES;
+    const bool inside = n < rows;
+    const int y = inside ? a.row_y[n] : -1;
+    float m = -INFINITY, s = 0.f;
+    if (y >= 0)
+      for (int k = sub; k < slots; k += LANES) {
+        const float pm = part_m[k * rows + n], ps = part_s[k * rows + n];
+        const float top = fmaxf(m, pm), base = top == -INFINITY ? 0.f : top;
+        s = s * ex2(m - base) + ps * ex2(pm - base);
+        m = top;
       }
-      loss += l;
+#pragma unroll
+    for (int o = 1; o < LANES; o <<= 1) {
+      const float pm = __shfl_xor_sync(0xffffffffu, m, o), ps = __shfl_xor_sync(0xffffffffu, s, o);
+      const float top = fmaxf(m, pm), base = top == -INFINITY ? 0.f : top;
+      s = s * ex2(m - base) + ps * ex2(pm - base);
+      m = top;
     }
-    lse2[n] = l2;
-    if (row_loss && n < N) row_loss[n] = l;
+    if (sub == 0 && inside) {
+      float l2 = INFINITY, l = 0.f;
+      if (y >= 0) {
+        const float t = t_label[n];
+        count += 1.0;
+        if (t == -INFINITY) {
+          l = INFINITY;
+          a.row_y[n] = -1;
+        } else {
+          // (maximum - t) + log2(sum) instead of lse2 - t: the maximum and t often agree in most digits
+          const float ls = log2f(s);
+          l = (float)(((double)(m - t) + (double)ls) * LN2);
+          l2 = m + ls;
+        }
+        loss += l;
+      }
+      a.row_lse2[n] = l2;
+      if (a.reduction == GSB_REDUCE_NONE && n < N) a.loss[n] = l;
+    }
+  }
+  loss = block_sum(loss);
+  count = block_sum(count);
+  __shared__ bool s_last;
+  if (threadIdx.x == 0) {
+    block_loss[blockIdx.x] = loss;
+    block_count[blockIdx.x] = count;
+    __threadfence();
+    s_last = atomicAdd(ticket, 1) == (int)gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  loss = count = 0.0;
+  for (int i = threadIdx.x; i < (int)gridDim.x; i += THREADS) {
+    loss += __ldcg(block_loss + i);
+    count += __ldcg(block_count + i);
   }
   loss = block_sum(loss);
   count = block_sum(count);
   if (threadIdx.x == 0) {
-    block_loss[blockIdx.x] = loss;
-    block_count[blockIdx.x] = count;
-  }
-}
-
-// The blocks' sums in one fixed order; *inv_count is what a mean divides by.
-__global__ void __launch_bounds__(THREADS) finish_loss_kernel(const double* __restrict__ block_loss,
-                                                              const double* __restrict__ block_count, int blocks,
-                                                              int reduction, float* __restrict__ loss,
-                                                              float* __restrict__ inv_count) {
-  double l = 0.0, c = 0.0;
-  for (int i = threadIdx.x; i < blocks; i += THREADS) {
-    l += block_loss[i];
-    c += block_count[i];
-  }
-  l = block_sum(l);
-  c = block_sum(c);
-  if (threadIdx.x == 0) {
-    const double inv = reduction == GSB_REDUCE_MEAN ? 1.0 / fmax(c, 1.0) : 1.0;
-    *inv_count = (float)inv;
-    if (reduction != GSB_REDUCE_NONE) *loss = (float)(l * inv);
+    const double inv = a.reduction == GSB_REDUCE_MEAN ? 1.0 / fmax(count, 1.0) : 1.0;
+    *a.inv_count = (float)inv;  // what a mean divides by
+    if (a.reduction != GSB_REDUCE_NONE) *a.loss = (float)(loss * inv);
   }
 }
 
@@ -752,62 +875,48 @@ __global__ void __launch_bounds__(THREADS) finish_loss_kernel(const double* __re
 __global__ void __launch_bounds__(THREADS) row_upstream_kernel(const float* __restrict__ up,
                                                                const int* __restrict__ row_y, long long rows,
                                                                float* __restrict__ out) {
-  for (long long n = (long long)blockIdx.x * THREADS + threadIdx.x; n < rows; n += (long long)gridDim.x * THREADS)
-    out[n] = row_y[n] >= 0 ? up[n] : 0.f;
+  const long long n = (long long)blockIdx.x * THREADS + threadIdx.x;
+  if (n < rows) out[n] = row_y[n] >= 0 ? up[n] : 0.f;
 }
 
-// Where the streaming passes leave column c of row n of a split.
-__device__ __forceinline__ size_t part_index(int split, long long rows, long long n, int c, int D) {
-  const size_t tile = (size_t)split * (rows / TILE) + n / TILE;
-  return ((tile * (D / 4) + c / 4) * TILE + n % TILE) * 4 + c % 4;
-}
-
-// Sums the splits of dX in order, scales, and writes the features' layout.
-__global__ void __launch_bounds__(THREADS) join_dx_kernel(const gsb_class_loss_args a, const float* __restrict__ part,
-                                                          int splits, int D, long long rows) {
-  const long long N = a.B * a.S;
-  const long long total = N * a.C;
-  for (long long i = (long long)blockIdx.x * THREADS + threadIdx.x; i < total; i += (long long)gridDim.x * THREADS) {
-    // consecutive threads along the layout's contiguous direction
-    long long n;
-    int c;
-    if (a.stride_c == 1) {
-      n = i / a.C;
-      c = (int)(i - n * a.C);
-    } else {
-      const long long b = i / (a.C * a.S), r = i - b * a.C * a.S;
-      c = (int)(r / a.S);
-      n = b * a.S + (r - c * a.S);
-    }
-    float v = 0.f;
-    for (int k = 0; k < splits; ++k) v += part[part_index(k, rows, n, c, D)];
-    const float u = a.reduction == GSB_REDUCE_NONE ? a.upstream[n] : a.upstream[0] * a.inv_count[0];
-    const long long b = n / a.S;
-    // rows without a gradient stay exactly zero whatever upstream holds
-    const bool used = a.row_y[n] >= 0;
-    store_elem(a.grad_features, b * a.C * a.S + (a.stride_c == 1 ? (n - b * a.S) * a.C + c : c * a.S + (n - b * a.S)),
-               a.dtype, used ? v * u : 0.f);
+// Sums the splits' partial rows: a CTA takes 32 quads of four columns, eight
+// threads each, which take every eighth split and are added in order.
+__global__ void __launch_bounds__(THREADS) join_acc_kernel(const GradOut o, const float4* __restrict__ part, int splits,
+                                                           int D, long long quads) {
+  __shared__ float4 s_part[8][32];
+  const int lane = threadIdx.x % 32, sub = threadIdx.x / 32;
+  const long long q = (long long)blockIdx.x * 32 + lane;  // [tile][column / 4][row]; a multiple of 128 in all
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = sub; k < splits; k += 8) {
+    const float4 v = part[(size_t)k * quads + q];
+    sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
   }
+  s_part[sub][lane] = sum;
+  __syncthreads();
+  if (sub != 0) return;
+  for (int k = 1; k < 8; ++k) {
+    const float4 v = s_part[k][lane];
+    sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
+  }
+  const long long strip = q / TILE;
+  const long long n = strip / (D / 4) * TILE + q % TILE;
+  if (n >= o.rows) return;
+  const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+  write_grad(o, n, (int)(strip % (D / 4)) * 4, v, grad_scale(o, n));
 }
 
-__global__ void __launch_bounds__(THREADS) join_dw_kernel(const gsb_class_loss_args a, const float* __restrict__ part,
-                                                          const float* __restrict__ part_bias, int splits, int slots,
-                                                          int D, long long rows) {
-  const float u = a.reduction == GSB_REDUCE_NONE ? 1.f : a.upstream[0] * a.inv_count[0];
-  const long long total = a.V * (a.C + 1ll);
-  for (long long i = (long long)blockIdx.x * THREADS + threadIdx.x; i < total; i += (long long)gridDim.x * THREADS) {
-    const long long v = i / (a.C + 1);
-    const int c = (int)(i - v * (a.C + 1));
-    float sum = 0.f;
-    if (c < a.C) {
-      if (!a.grad_weight) continue;
-      for (int k = 0; k < splits; ++k) sum += part[part_index(k, rows, v, c, D)];
-      store_elem(a.grad_weight, v * a.C + c, a.dtype, sum * u);
-    } else if (a.grad_bias) {
-      for (int k = 0; k < slots; ++k) sum += part_bias[k * rows + v];
-      a.grad_bias[v] = sum * u;
-    }
-  }
+__global__ void __launch_bounds__(THREADS) join_bias_kernel(const GradOut o, const float* __restrict__ part, int slots,
+                                                            long long rows) {
+  __shared__ float s_part[8][32];
+  const int lane = threadIdx.x % 32, sub = threadIdx.x / 32;
+  const long long v = (long long)blockIdx.x * 32 + lane;  // rows is a multiple of 128
+  float sum = 0.f;
+  for (int k = sub; k < slots; k += 8) sum += part[k * rows + v];
+  s_part[sub][lane] = sum;
+  __syncthreads();
+  if (sub != 0 || v >= o.rows) return;
+  for (int k = 1; k < 8; ++k) sum += s_part[k][lane];
+  ((float*)o.out)[v] = sum * grad_scale(o, v);
 }
 
 // ---------------------------------------------------------------------------
@@ -885,6 +994,7 @@ struct Carver {
 struct FwdWs {
   float *part_m, *part_s, *t_label;
   double *block_loss, *block_count;
+  int* ticket;
 };
 inline size_t carve_fwd(void* base, const Dims& d, FwdWs* w) {
   Carver c{(char*)base};
@@ -894,18 +1004,25 @@ inline size_t carve_fwd(void* base, const Dims& d, FwdWs* w) {
   w->t_label = c.take<float>(rows);
   w->block_loss = c.take<double>(JOIN_BLOCKS);
   w->block_count = c.take<double>(JOIN_BLOCKS);
+  w->ticket = c.take<int>(1);
   return c.off;
 }
 
 struct BwdWs {
   float *part_x, *part_w, *part_bias, *row_u;
 };
+// Partial rows are needed by units that have a part of the streamed axis, or
+// more of it than one accumulator takes.
+inline bool needs_partials(int splits, int cols, int tn, int planes) {
+  return splits > 1 || cols > chain_products(planes) / (tn / 16);
+}
 inline size_t carve_bwd(void* base, const Dims& d, BwdWs* w) {
   Carver c{(char*)base};
-  w->part_x = c.take<float>((size_t)d.x_tiles * TILE * d.dx_splits * d.D);
-  w->part_w = c.take<float>((size_t)d.w_tiles * TILE * d.dw_splits * d.D);
-  w->part_bias = c.take<float>((size_t)d.w_tiles * TILE * d.dw_splits * d.dw_slots);
-  w->row_u = c.take<float>((size_t)d.x_tiles * TILE);
+  const size_t x = (size_t)d.x_tiles * TILE, v = (size_t)d.w_tiles * TILE;
+  w->part_x = c.take<float>(needs_partials(d.dx_splits, d.dx_cols, d.dx_tn, d.planes) ? x * d.dx_splits * d.D : 0);
+  w->part_w = c.take<float>(needs_partials(d.dw_splits, d.dw_cols, d.dw_tn, d.planes) ? v * d.dw_splits * d.D : 0);
+  w->part_bias = c.take<float>(v * d.dw_splits * d.dw_slots);
+  w->row_u = c.take<float>(x);
   return c.off;
 }
 
@@ -978,8 +1095,6 @@ int launch_stream(const StreamArgs& g, int planes, int tn, cudaStream_t s) {
   return GSB_ERR_INVALID;
 }
 
-inline int blocks_for(long long n) { return (int)std::max(1ll, std::min((n + THREADS - 1) / THREADS, (long long)SMS * 16)); }
-
 }  // namespace
 }  // namespace gsb
 
@@ -1028,18 +1143,26 @@ GSB_EXPORT int gsb_class_loss_fwd(const gsb_class_loss_args* a, void* stream) {
   g.part_m = w.part_m;
   g.part_s = w.part_s;
   g.t_label = w.t_label;
-  const long long x_total = d.x_tiles * d.D8 * TILE, w_total = d.w_tiles * d.D8 * TILE;
-  pack_classes_kernel<<<blocks_for(w_total), THREADS, 0, s>>>(*a, d.D8, w_total, (uint4*)a->packed_w, a->class_bias2);
+  const int tiles = (int)(d.w_tiles + d.x_tiles);
+  switch (a->dtype) {
+    case GSB_TYPE_BF16: pack_kernel<__nv_bfloat16><<<tiles, THREADS, 0, s>>>(*a, d.D8, (int)d.w_tiles, w.ticket); break;
+    case GSB_TYPE_FP16: pack_kernel<__half><<<tiles, THREADS, 0, s>>>(*a, d.D8, (int)d.w_tiles, w.ticket); break;
+    default: pack_kernel<float><<<tiles, THREADS, 0, s>>>(*a, d.D8, (int)d.w_tiles, w.ticket); break;
+  }
   if (d.N > 0) {
-    pack_rows_kernel<<<blocks_for(x_total), THREADS, 0, s>>>(*a, d.D8, x_total, (uint4*)a->packed_x, a->row_y);
     const int r = launch_stream<FWD>(g, d.planes, d.fwd_tn, s);
     if (r != GSB_OK) return r;
   }
-  const int blocks = (int)std::max(1ll, std::min<long long>(JOIN_BLOCKS, (d.x_tiles * TILE + THREADS - 1) / THREADS));
-  join_rows_kernel<<<blocks, THREADS, 0, s>>>(g, d.fwd_splits * d.fwd_slots, d.N, a->row_lse2, a->row_y,
-                                              a->reduction == GSB_REDUCE_NONE ? a->loss : nullptr, w.block_loss,
-                                              w.block_count);
-  finish_loss_kernel<<<1, THREADS, 0, s>>>(w.block_loss, w.block_count, blocks, a->reduction, a->loss, a->inv_count);
+  const int slots = d.fwd_splits * d.fwd_slots;
+  const long long rows = d.x_tiles * TILE;
+  const int per_cta = slots > 8 ? THREADS / 8 : THREADS;
+  const int blocks = (int)std::max(1ll, std::min<long long>(JOIN_BLOCKS, (rows + per_cta - 1) / per_cta));
+  if (slots > 8)
+    join_rows_kernel<8><<<blocks, THREADS, 0, s>>>(*a, w.part_m, w.part_s, w.t_label, slots, rows, w.block_loss,
+                                                   w.block_count, w.ticket);
+  else
+    join_rows_kernel<1><<<blocks, THREADS, 0, s>>>(*a, w.part_m, w.part_s, w.t_label, slots, rows, w.block_loss,
+                                                   w.block_count, w.ticket);
   return check_launch("gsb_class_loss_fwd");
 }
 
@@ -1070,34 +1193,62 @@ GSB_EXPORT int gsb_class_loss_bwd(const gsb_class_loss_args* a, void* stream) {
   g.y = a->row_y;
   g.error_word = a->error_word;
   g.D8 = d.D8;
+  const bool per_row = a->reduction == GSB_REDUCE_NONE;
   if (a->grad_features) {
+    GradOut o{};
+    o.out = a->grad_features;
+    o.upstream = a->upstream;
+    o.inv_count = per_row ? nullptr : a->inv_count;
+    o.y = a->row_y;
+    o.rows = d.N;
+    o.S = a->stride_c == 1 ? 0 : a->S;
+    o.C = a->C;
+    o.dtype = a->dtype;
     g.a = (const uint4*)a->packed_x;
     g.b = (const uint4*)a->packed_w;
     g.a_tiles = (int)d.x_tiles;
     g.b_tiles = d.dx_cols;
     g.splits = d.dx_splits;
     g.part_acc = w.part_x;
+    if (d.dx_splits == 1) g.grad = o;
     const int r = launch_stream<DX>(g, d.planes, d.dx_tn, s);
     if (r != GSB_OK) return r;
-    join_dx_kernel<<<blocks_for(d.N * a->C), THREADS, 0, s>>>(*a, w.part_x, d.dx_splits, d.D, d.x_tiles * TILE);
+    const long long quads = d.x_tiles * TILE * (d.D / 4);
+    if (d.dx_splits > 1)
+      join_acc_kernel<<<(unsigned)(quads / 32), THREADS, 0, s>>>(o, (const float4*)w.part_x, d.dx_splits, d.D, quads);
   }
   if (a->grad_weight || a->grad_bias) {
+    GradOut o{};
+    o.out = a->grad_weight;
+    o.upstream = per_row ? nullptr : a->upstream;  // a row's factor is already in P
+    o.inv_count = per_row ? nullptr : a->inv_count;
+    o.rows = a->V;
+    o.C = a->C;
+    o.dtype = a->dtype;
     g.a = (const uint4*)a->packed_w;
     g.b = (const uint4*)a->packed_x;
     g.a_tiles = (int)d.w_tiles;
     g.b_tiles = d.dw_cols;
     g.splits = d.dw_splits;
     g.slots = d.dw_slots;
-    g.part_acc = w.part_w;
+    g.part_acc = a->grad_weight ? w.part_w : nullptr;
     g.part_bias = w.part_bias;
-    if (a->reduction == GSB_REDUCE_NONE) {
-      row_upstream_kernel<<<blocks_for(d.x_tiles * TILE), THREADS, 0, s>>>(a->upstream, a->row_y, d.x_tiles * TILE, w.row_u);
+    g.grad = GradOut{};
+    if (d.dw_splits == 1) g.grad = o;
+    if (per_row) {
+      row_upstream_kernel<<<div_up(d.x_tiles * TILE, THREADS), THREADS, 0, s>>>(a->upstream, a->row_y, d.x_tiles * TILE,
+                                                                               w.row_u);
       g.row_u = w.row_u;
     }
     const int r = launch_stream<DW>(g, d.planes, d.dw_tn, s);
     if (r != GSB_OK) return r;
-    join_dw_kernel<<<blocks_for(a->V * (a->C + 1ll)), THREADS, 0, s>>>(*a, w.part_w, w.part_bias, d.dw_splits,
-                                                                      d.dw_splits * d.dw_slots, d.D, d.w_tiles * TILE);
+    const long long rows = d.w_tiles * TILE, quads = rows * (d.D / 4);
+    if (a->grad_weight && d.dw_splits > 1)
+      join_acc_kernel<<<(unsigned)(quads / 32), THREADS, 0, s>>>(o, (const float4*)w.part_w, d.dw_splits, d.D, quads);
+    if (a->grad_bias) {
+      o.out = a->grad_bias;
+      join_bias_kernel<<<(unsigned)(rows / 32), THREADS, 0, s>>>(o, w.part_bias, d.dw_splits * d.dw_slots, rows);
+    }
   }
   return check_launch("gsb_class_loss_bwd");
 }
