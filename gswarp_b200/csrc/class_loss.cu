@@ -58,7 +58,9 @@ __device__ __forceinline__ void store_elem(void* p, long long i, int dtype, floa
 }
 
 // ---------------------------------------------------------------------------
-// Packing.  Tile layout: [plane][column / 8][row][8 columns] of bf16.
+// Packing.  Layout: [row / 8][plane][column / 8][row % 8][8 columns] of bf16,
+// so that any eight or more rows are one contiguous copy, and 8 x 8 core
+// matrices are 128 contiguous bytes with uniform strides in both directions.
 // ---------------------------------------------------------------------------
 template <int PLANES>
 __device__ __forceinline__ void store_planes(uint4* tile, int D8, int d8, int row, const float (&x)[8]) {
@@ -76,7 +78,7 @@ __device__ __forceinline__ void store_planes(uint4* tile, int D8, int d8, int ro
       rest[2 * i] = isinf(f.x) ? 0.f : rest[2 * i] - f.x;
       rest[2 * i + 1] = isinf(f.y) ? 0.f : rest[2 * i + 1] - f.y;
     }
-    tile[((size_t)p * D8 + d8) * TILE + row] = *reinterpret_cast<uint4*>(h);
+    tile[((size_t)(row / 8 * PLANES + p) * D8 + d8) * 8 + row % 8] = *reinterpret_cast<uint4*>(h);
   }
 }
 
@@ -428,13 +430,12 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
       const Range r = unit_range(g, u);
       ok = warp_wait(&bar->a_empty[as.i], as.phase ^ 1, stop);
       if (!ok) break;
-      if (lane == 0) mbar_expect(&bar->a_full[as.i], a_bytes);
-      __syncwarp();
-      {
-        const uint8_t* src = reinterpret_cast<const uint8_t*>(g.a) + (size_t)r.tile * a_bytes;
-        for (int k = lane; k < NP * D8; k += 32)
-          bulk_load(sA + (size_t)as.i * a_bytes + k * 2048, src + (size_t)k * 2048, 2048, &bar->a_full[as.i]);
+      if (lane == 0) {
+        mbar_expect(&bar->a_full[as.i], a_bytes);
+        bulk_load(sA + (size_t)as.i * a_bytes, reinterpret_cast<const uint8_t*>(g.a) + (size_t)r.tile * a_bytes, a_bytes,
+                  &bar->a_full[as.i]);
       }
+      __syncwarp();
       as.next(g.a_slots);
       for (int bt = r.lo; bt < r.hi; ++bt) {
         ok = warp_wait(&bar->b_empty[bs.i], bs.phase ^ 1, stop);
@@ -442,17 +443,17 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
         uint64_t* full = &bar->b_full[bs.i];
         const bool with_u = MODE == DW && g.row_u;
         const uint32_t metas = MODE == DW ? (with_u ? 3 : 2) : 1;
-        if (lane == 0) mbar_expect(full, b_bytes + metas * TN * 4);
+        if (lane == 0) {
+          const long long col0 = (long long)bt * TN;
+          float* meta = sMeta + bs.i * META;
+          mbar_expect(full, b_bytes + metas * TN * 4);
+          bulk_load(sB + (size_t)bs.i * b_bytes, reinterpret_cast<const uint8_t*>(g.b) + (size_t)bt * b_bytes, b_bytes,
+                    full);
+          bulk_load(meta, (MODE == DW ? g.lse2 : g.b2) + col0, TN * 4, full);
+          if (MODE == DW) bulk_load(meta + TN, g.y + col0, TN * 4, full);
+          if (with_u) bulk_load(meta + 2 * TN, g.row_u + col0, TN * 4, full);
+        }
         __syncwarp();
-        const long long col0 = (long long)bt * TN;
-        const uint8_t* src = reinterpret_cast<const uint8_t*>(g.b) + (size_t)(col0 / TILE) * NP * D8 * 2048 +
-                             (size_t)(col0 % TILE) * 16;
-        for (int k = lane; k < NP * D8; k += 32)
-          bulk_load(sB + (size_t)bs.i * b_bytes + (size_t)k * TN * 16, src + (size_t)k * 2048, TN * 16, full);
-        float* meta = sMeta + bs.i * META;
-        if (lane == 0) bulk_load(meta, (MODE == DW ? g.lse2 : g.b2) + col0, TN * 4, full);
-        if (MODE == DW && lane == 1) bulk_load(meta + TN, g.y + col0, TN * 4, full);
-        if (with_u && lane == 2) bulk_load(meta + 2 * TN, g.row_u + col0, TN * 4, full);
         bs.next(g.stages);
       }
     }
@@ -467,7 +468,7 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
   } else if (warp == ISSUER) {
     // ---- first products: z ----
     const uint32_t leader = elect_leader();
-    const uint32_t idesc = instr_desc(TN, false), hi = desc_hi(128);
+    const uint32_t idesc = instr_desc(TN, false), hi = desc_hi(NP * D8 * 128);
     const uint32_t a0 = smem_u32(sA), b0 = smem_u32(sB);
     bool ok = true;
     for (Cursor c(g); c.unit < units; c.next(g)) {
@@ -477,14 +478,14 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
            warp_wait(&bar->s_free[b], ((c.t / GROUPS) & 1) ^ 1, stop);
       if (!ok) break;
       fence_after();
-      const uint32_t a_lo = desc_lo(a0 + c.as.i * a_bytes, 2048), b_lo = desc_lo(b0 + c.bs.i * b_bytes, TN * 16);
+      const uint32_t a_lo = desc_lo(a0 + c.as.i * a_bytes, 128), b_lo = desc_lo(b0 + c.bs.i * b_bytes, 128);
       const uint32_t z = tmem + b * SBUF;
 #pragma unroll
       for (int q = 0; q < plane_products(NP); ++q) {
-        const uint32_t aq = a_lo + plane_of_a(NP, q) * D8 * 128, bq = b_lo + plane_of_b(NP, q) * D8 * TN;
+        const uint32_t aq = a_lo + plane_of_a(NP, q) * D8 * 8, bq = b_lo + plane_of_b(NP, q) * D8 * 8;
         mma_ss(leader, z, aq, hi, bq, hi, idesc, q > 0);
 #pragma unroll 4
-        for (int k = 2; k < D8; k += 2) mma_ss(leader, z, aq + k * 128, hi, bq + k * TN, hi, idesc, true);
+        for (int k = 2; k < D8; k += 2) mma_ss(leader, z, aq + k * 8, hi, bq + k * 8, hi, idesc, true);
       }
       mma_commit(leader, &bar->s_full[b]);
       if (c.bt + 1 == c.r.hi) mma_commit(leader, &bar->a_empty[c.as.i]);
@@ -500,7 +501,7 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
     // ---- second products: the accumulators.  A warp of its own, so that waiting for one group's P does not
     // hold up the next group's z ----
     const uint32_t leader = elect_leader();
-    const uint32_t idesc = instr_desc(D, true), hi = desc_hi(TN * 16);
+    const uint32_t idesc = instr_desc(D, true), hi = desc_hi(128), step = NP * D8 * 16;
     const uint32_t b0 = smem_u32(sB);
     bool ok = true;
     for (Cursor c(g); c.unit < units; c.next(g)) {
@@ -512,16 +513,16 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
       if (!ok) break;
       fence_after();
       const uint32_t dst = tmem + ACC0 + c.acc.i * ACCS * D, p = tmem + b * SBUF;
-      const uint32_t b_lo = desc_lo(b0 + c.bs.i * b_bytes, 128);
+      const uint32_t b_lo = desc_lo(b0 + c.bs.i * b_bytes, NP * D8 * 128);
 #pragma unroll
       for (int q = 0; q < plane_products(NP); ++q) {
         const int pa = plane_of_a(NP, q);
         const bool main = q + 1 == plane_products(NP);
         const uint32_t to = ACCS == 2 && !main ? dst + D : dst;
-        const uint32_t bq = b_lo + plane_of_b(NP, q) * D8 * TN;
+        const uint32_t bq = b_lo + plane_of_b(NP, q) * D8 * 8;
 #pragma unroll
         for (int k = 0; k < TN / 16; ++k)
-          mma_ts(leader, to, p + p_column(TN, 16 * k, pa), bq + k * 16, hi, idesc,
+          mma_ts(leader, to, p + p_column(TN, 16 * k, pa), bq + k * step, hi, idesc,
                  k > 0 || (q > 0 && !(ACCS == 2 && main)) || !first);
       }
       mma_commit(leader, &bar->b_empty[c.bs.i]);
