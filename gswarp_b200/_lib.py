@@ -181,8 +181,7 @@ class ClassLossArgs(ctypes.Structure):
         ("B", c_ll), ("S", c_ll), ("V", c_ll), ("C", c_int), ("dtype", c_int),
         ("reduction", c_int), ("labels64", c_int),
         ("stride_b", c_ll), ("stride_c", c_ll), ("stride_s", c_ll), ("ignore_index", c_ll),
-        ("features", vp), ("weight", vp), ("bias", vp), ("labels", vp), ("loss", vp),
-        ("packed_x", vp), ("packed_w", vp), ("class_bias2", vp), ("row_lse2", vp), ("row_y", vp), ("inv_count", vp),
+        ("features", vp), ("weight", vp), ("bias", vp), ("labels", vp), ("loss", vp), ("kept", vp),
         ("upstream", vp), ("grad_features", vp), ("grad_weight", vp), ("grad_bias", vp),
         ("error_word", vp), ("workspace", vp), ("workspace_bytes", ctypes.c_size_t),
     ]
@@ -202,7 +201,7 @@ EXPORTED = (
     "gsb_knn", "gsb_selftest_threshold_log", "gsb_ssim_fwd_noalloc", "gsb_photo_loss_fwd",
     "gsb_photo_loss_bwd", "gsb_adam_step", "gsb_densify_stats", "gsb_sh_colors_views",
     "gsb_sh_backward_views", "gsb_block_dim", "gsb_peak_fp32", "gsb_peak_ex2", "gsb_peak_work",
-    "gsb_class_loss_packed_bytes", "gsb_class_loss_workspace_bytes", "gsb_class_loss_fwd", "gsb_class_loss_bwd",
+    "gsb_class_loss_sizes", "gsb_class_loss_fwd", "gsb_class_loss_bwd",
     "gsb_codebook_fwd", "gsb_codebook_bwd_workspace_bytes", "gsb_codebook_bwd",
 )
 
@@ -240,8 +239,7 @@ def _declare(L) -> None:
     fn("gsb_sh_backward_views", c_int, [P(SHViewsArgs), vp])
     fn("gsb_knn_workspace_bytes", ctypes.c_size_t, [c_int])
     fn("gsb_knn", c_int, [P(KNNArgs), vp])
-    fn("gsb_class_loss_packed_bytes", ctypes.c_size_t, [c_ll, c_int, c_int])
-    fn("gsb_class_loss_workspace_bytes", ctypes.c_size_t, [P(ClassLossArgs), c_int])
+    fn("gsb_class_loss_sizes", c_int, [P(ClassLossArgs), ctypes.c_size_t * 3])
     fn("gsb_class_loss_fwd", c_int, [P(ClassLossArgs), vp])
     fn("gsb_class_loss_bwd", c_int, [P(ClassLossArgs), vp])
     fn("gsb_codebook_fwd", c_int, [P(CodebookArgs), vp])
@@ -297,3 +295,13 @@ def check(status: int, what: str) -> None:
 def call(name: str, *args) -> None:
     L = load()
     check(getattr(L, name)(*args), name)
+
+
+def call_on(device: torch.device, name: str, args) -> None:
+    """``call`` on ``device``'s current stream, with ``device`` made current
+    only if it is not (the operators of a few microseconds pay for both)."""
+    if torch.cuda.current_device() == device.index:
+        call(name, args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            call(name, args, torch.cuda.current_stream(device).cuda_stream)

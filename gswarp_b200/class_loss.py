@@ -11,6 +11,8 @@ by tile and accumulates the gradients of the map, the classifier and its bias.
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib, _pipeline
@@ -63,7 +65,7 @@ def _validate(features, weight, labels, bias, ignore_index, reduction, train) ->
 def _rows(features):
     """(B, S, C, strides of b, c and s): rows n = b * S + s of a map or a matrix.  A map whose pixels have
     no single stride is made contiguous first."""
-    x = features.detach()
+    x = features
     if x.ndim == 2:
         x = x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
         # stride_c = 1 marks rows of channels: the gradient is written (N, C)
@@ -77,93 +79,75 @@ def _rows(features):
 
 
 def _forward(features, weight, labels, bias, ignore_index, reduction):
-    """``(loss, args, kept)``: the argument block with its sizes, and the tensors backward reads."""
+    """``(loss, args, kept, bytes of the backward workspace)``: the argument block with its sizes, and the
+    buffer that backward reads."""
     x, B, S, C, (sb, sc, ss) = _rows(features)
     dev = x.device
-    L = _lib.load()
-    N, V = B * S, weight.shape[0]
-
-    def empty(n, dtype):
-        return torch.empty(max(n, 1), dtype=dtype, device=dev)
-
-    def whole_tiles(n):
-        return -(-n // TILE) * TILE
-
-    a = _lib.ClassLossArgs()
-    a.B, a.S, a.V, a.C = B, S, V, C
-    a.dtype, a.reduction = _lib.DTYPES[x.dtype], _REDUCTIONS[reduction]
-    a.labels64 = int(labels.dtype == torch.int64)
-    a.stride_b, a.stride_c, a.stride_s = sb, sc, ss
-    a.ignore_index = ignore_index
-    w = weight.detach().contiguous()
-    b = bias.detach().contiguous() if bias is not None else None
+    N = B * S
+    w = weight.contiguous()
+    b = bias.contiguous() if bias is not None else None
     y = labels.contiguous()
-    a.features, a.weight, a.bias, a.labels = _lib.ptr(x), _lib.ptr(w), _lib.ptr(b), _lib.ptr(y)
-    kept = (empty(int(L.gsb_class_loss_packed_bytes(N, C, a.dtype)), torch.uint8),
-            empty(int(L.gsb_class_loss_packed_bytes(V, C, a.dtype)), torch.uint8),
-            empty(whole_tiles(V), torch.float32), empty(whole_tiles(N), torch.float32),
-            empty(whole_tiles(N), torch.int32), empty(1, torch.float32))
-    _point_at(a, kept)
-    loss = empty(N if reduction == "none" else 1, torch.float32)
-    a.loss = _lib.ptr(loss)
-    with torch.cuda.device(dev), _pipeline._stage_timer("class_loss_fwd", {"rows": N}):
-        ws = _workspace(a, 0, dev)
-        _lib.call("gsb_class_loss_fwd", a, _lib.stream_handle(dev))
-    del ws
-    return loss[:N].view(labels.shape) if reduction == "none" else loss.view(()), a, kept
+    a = _lib.ClassLossArgs(B, S, w.shape[0], C, _lib.DTYPES[x.dtype], _REDUCTIONS[reduction],
+                           labels.dtype == torch.int64, sb, sc, ss, ignore_index,
+                           x.data_ptr(), w.data_ptr(), None if b is None else b.data_ptr(), y.data_ptr())
+    sizes = _SIZES()
+    _lib.call("gsb_class_loss_sizes", a, sizes)
+    # torch's allocations are 512-byte aligned
+    kept = torch.empty(sizes[0], dtype=torch.uint8, device=dev)
+    ws = torch.empty(sizes[1], dtype=torch.uint8, device=dev)
+    # one element at least: an empty tensor has no address
+    loss = torch.empty(max(N, 1) if reduction == "none" else 1, dtype=torch.float32, device=dev)
+    a.loss, a.kept, a.workspace, a.workspace_bytes = loss.data_ptr(), kept.data_ptr(), ws.data_ptr(), sizes[1]
+    a.error_word = _pipeline.sticky_error_word(dev).data_ptr()
+    with _pipeline._stage_timer("class_loss_fwd", {"rows": N}):
+        _lib.call_on(dev, "gsb_class_loss_fwd", a)
+    loss = loss[:N].view(labels.shape) if reduction == "none" else loss.view(())
+    return loss, a, kept, sizes[2]
 
 
-def _point_at(a, kept) -> None:
-    packed_x, packed_w, bias2, lse2, row_y, inv_count = kept
-    a.packed_x, a.packed_w = _lib.ptr(packed_x), _lib.ptr(packed_w)
-    a.class_bias2, a.row_lse2, a.row_y = _lib.ptr(bias2), _lib.ptr(lse2), _lib.ptr(row_y)
-    a.inv_count = _lib.ptr(inv_count)
-    a.error_word = _lib.ptr(_pipeline.sticky_error_word(packed_x.device))
+_SIZES = ctypes.c_size_t * 3
 
 
-def _workspace(a, backward, device):
-    n = int(_lib.load().gsb_class_loss_workspace_bytes(a, backward))
-    ws = _pipeline._workspace(n, device)
-    a.workspace, a.workspace_bytes = _lib.ptr(ws), n
-    return ws
-
-
-def _backward(args, kept, upstream, features_shape, dtype, want_features, want_weight, want_bias):
-    dev = upstream.device
+def _backward(args, kept, ws_bytes, upstream, features_shape, dtype, want_features, want_weight, want_bias):
+    dev = kept.device
     a = _lib.ClassLossArgs.from_buffer_copy(args)
     a.features = a.weight = a.bias = a.labels = a.loss = None  # not kept, not read
-    _point_at(a, kept)
-    up = upstream.detach().to(torch.float32).reshape(-1).contiguous()
-    a.upstream = _lib.ptr(up)
+    up = upstream if upstream.dtype == torch.float32 else upstream.float()
+    up = up.contiguous()
     gx = torch.empty(features_shape, dtype=dtype, device=dev) if want_features else None
     gw = torch.empty((a.V, a.C), dtype=dtype, device=dev) if want_weight else None
     gb = torch.empty(a.V, dtype=torch.float32, device=dev) if want_bias else None
-    a.grad_features, a.grad_weight, a.grad_bias = _lib.ptr(gx), _lib.ptr(gw), _lib.ptr(gb)
-    with torch.cuda.device(dev), _pipeline._stage_timer("class_loss_bwd", {"rows": a.B * a.S}):
-        ws = _workspace(a, 1, dev)
-        _lib.call("gsb_class_loss_bwd", a, _lib.stream_handle(dev))
-    del ws
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    a.kept, a.workspace, a.workspace_bytes = kept.data_ptr(), ws.data_ptr(), ws_bytes
+    a.upstream = up.data_ptr()
+    if want_features:
+        a.grad_features = gx.data_ptr()
+    if want_weight:
+        a.grad_weight = gw.data_ptr()
+    if want_bias:
+        a.grad_bias = gb.data_ptr()
+    with _pipeline._stage_timer("class_loss_bwd", {"rows": a.B * a.S}):
+        _lib.call_on(dev, "gsb_class_loss_bwd", a)
     return gx, gw, gb
 
 
 class _ClassCrossEntropy(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, features, weight, labels, bias, ignore_index, reduction, train):
-        loss, args, kept = _forward(features, weight, labels, bias, ignore_index, reduction)
-        ctx.train = train
-        if train:
-            ctx.args, ctx.shape, ctx.dtype = args, features.shape, features.dtype
-            ctx.save_for_backward(*kept)
+    def forward(ctx, features, weight, labels, bias, ignore_index, reduction):
+        loss, ctx.args, kept, ctx.ws_bytes = _forward(features, weight, labels, bias, ignore_index, reduction)
+        ctx.shape, ctx.dtype = features.shape, features.dtype
+        ctx.save_for_backward(kept)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         want = ctx.needs_input_grad
-        if not ctx.train or not (want[0] or want[1] or want[3]):
-            return (None,) * 7
-        gx, gw, gb = _backward(ctx.args, ctx.saved_tensors, grad, ctx.shape, ctx.dtype, want[0], want[1], want[3])
-        return gx, gw, None, gb, None, None, None
+        if not (want[0] or want[1] or want[3]):
+            return (None,) * 6
+        kept, = ctx.saved_tensors
+        gx, gw, gb = _backward(ctx.args, kept, ctx.ws_bytes, grad, ctx.shape, ctx.dtype, want[0], want[1], want[3])
+        return gx, gw, None, gb, None, None
 
 
 def class_cross_entropy(features, weight, labels, bias=None, ignore_index=-100, reduction="mean", train=True):
@@ -185,4 +169,7 @@ def class_cross_entropy(features, weight, labels, bias=None, ignore_index=-100, 
     packed copy of the features and the classifier instead of the tensors themselves.
     """
     _validate(features, weight, labels, bias, ignore_index, reduction, train)
-    return _ClassCrossEntropy.apply(features, weight, labels, bias, ignore_index, reduction, train)
+    if not train:
+        with torch.no_grad():
+            return _forward(features, weight, labels, bias, ignore_index, reduction)[0]
+    return _ClassCrossEntropy.apply(features, weight, labels, bias, ignore_index, reduction)

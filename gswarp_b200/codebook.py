@@ -44,26 +44,22 @@ def _validate(table, codes, scale) -> None:
 
 
 def _args(table, codes, scale, gain) -> _lib.CodebookArgs:
-    a = _lib.CodebookArgs()
-    a.P, a.K, a.D = codes.numel(), table.shape[0], math.prod(table.shape[1:])
-    a.dtype = _lib.DTYPES[table.dtype]
-    a.codes64 = int(codes.dtype == torch.int64)
-    a.scale = scale
-    a.table, a.codes, a.gain = _lib.ptr(table), _lib.ptr(codes), _lib.ptr(gain)
-    a.error_word = _lib.ptr(_pipeline.sticky_error_word(table.device))
-    return a
+    return _lib.CodebookArgs(codes.numel(), table.shape[0], math.prod(table.shape[1:]), _lib.DTYPES[table.dtype],
+                             codes.dtype == torch.int64, scale, table.data_ptr(), codes.data_ptr(),
+                             None if gain is None else gain.data_ptr())
 
 
 def lookup_forward(table: torch.Tensor, codes: torch.Tensor, scale: float = 1.0,
                    gain: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """``scale * gain * table[codes]`` of contiguous tensors, into ``out`` if given."""
+    dev = table.device
     if out is None:
-        out = torch.empty(codes.shape + table.shape[1:], dtype=table.dtype, device=table.device)
+        out = torch.empty(codes.shape + table.shape[1:], dtype=table.dtype, device=dev)
     a = _args(table, codes, scale, gain)
-    a.out = _lib.ptr(out)
-    with torch.cuda.device(table.device), _pipeline._stage_timer("codebook_fwd", {"rows": codes.numel(),
-                                                                                  "kernels": 1}):
-        _lib.call("gsb_codebook_fwd", a, _lib.stream_handle(table.device))
+    a.out = out.data_ptr()
+    a.error_word = _pipeline.sticky_error_word(dev).data_ptr()
+    with _pipeline._stage_timer("codebook_fwd", {"rows": a.P, "kernels": 1}):
+        _lib.call_on(dev, "gsb_codebook_fwd", a)
     return out
 
 
@@ -71,30 +67,31 @@ def lookup_backward(table: torch.Tensor, codes: torch.Tensor, scale: float, gain
                     grad_out: torch.Tensor, want_table: bool = True, want_gain: bool = False,
                     out: torch.Tensor | None = None):
     """``(grad_table, grad_gain)`` of contiguous tensors; ``grad_table`` into ``out`` if given."""
-    L = _lib.load()
+    dev = table.device
     a = _args(table, codes, scale, gain)
+    a.grad_out = grad_out.data_ptr()
+    a.error_word = _pipeline.sticky_error_word(dev).data_ptr()
     grad_table = grad_gain = None
-    a.grad_out = _lib.ptr(grad_out)
     if want_table:
         grad_table = torch.empty_like(table) if out is None else out
-        a.grad_table = _lib.ptr(grad_table)
-        ws_bytes = int(L.gsb_codebook_bwd_workspace_bytes(a.P, a.K, a.D))
-        ws = _pipeline._workspace(ws_bytes, table.device)
-        a.workspace, a.workspace_bytes = _lib.ptr(ws), ws_bytes
+        a.grad_table = grad_table.data_ptr()
+        n = _lib.load().gsb_codebook_bwd_workspace_bytes(a.P, a.K, a.D)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), n
     if want_gain:
         grad_gain = torch.empty_like(gain)
-        a.grad_gain = _lib.ptr(grad_gain)
-    with torch.cuda.device(table.device), _pipeline._stage_timer("codebook_bwd", {"rows": codes.numel()}):
-        _lib.call("gsb_codebook_bwd", a, _lib.stream_handle(table.device))
+        a.grad_gain = grad_gain.data_ptr()
+    with _pipeline._stage_timer("codebook_bwd", {"rows": a.P}):
+        _lib.call_on(dev, "gsb_codebook_bwd", a)
     return grad_table, grad_gain
 
 
 class _CodebookLookup(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, codes, scale, gain):
-        t = table.detach().contiguous()
+        t = table.contiguous()
         c = codes.contiguous()
-        g = gain.detach().contiguous() if gain is not None else None
+        g = gain.contiguous() if gain is not None else None
         ctx.scale = scale
         ctx.save_for_backward(t, c, g)
         return lookup_forward(t, c, scale, g)
@@ -121,4 +118,8 @@ def codebook_lookup(table, codes, scale=1.0):
     """
     _validate(table, codes, scale)
     gain = scale if isinstance(scale, torch.Tensor) else None
-    return _CodebookLookup.apply(table, codes, 1.0 if gain is not None else float(scale), gain)
+    scale = 1.0 if gain is not None else float(scale)
+    if not torch.is_grad_enabled():
+        return lookup_forward(table.contiguous(), codes.contiguous(), scale,
+                              None if gain is None else gain.contiguous())
+    return _CodebookLookup.apply(table, codes, scale, gain)

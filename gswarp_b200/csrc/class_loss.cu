@@ -38,7 +38,6 @@ constexpr double LN2 = 0.6931471805599453;
 __host__ __device__ inline int planes_of(int dtype) { return dtype == GSB_TYPE_FP32 ? 3 : dtype == GSB_TYPE_FP16 ? 2 : 1; }
 inline int pad_c(int C) { return (C + 15) & ~15; }
 inline long long tiles_of(long long n) { return (n + TILE - 1) / TILE; }
-inline size_t tile_bytes(int dtype, int C) { return (size_t)planes_of(dtype) * pad_c(C) * TILE * 2; }
 inline size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -56,6 +55,13 @@ __device__ __forceinline__ void store_elem(void* p, long long i, int dtype, floa
   else if (dtype == GSB_TYPE_BF16) ((__nv_bfloat16*)p)[i] = __float2bfloat16_rn(v);
   else ((__half*)p)[i] = __float2half_rn(v);
 }
+
+struct Kept {
+  uint4 *packed_x, *packed_w;
+  float *class_bias2, *row_lse2;  // base 2; classes and rows rounded up to whole tiles
+  int* row_y;                     // labels, -1 where a row has no gradient
+  float* inv_count;
+};
 
 // ---------------------------------------------------------------------------
 // Packing.  Layout: [row / 8][plane][column / 8][row % 8][8 columns] of bf16,
@@ -106,7 +112,7 @@ __device__ __forceinline__ void load8(const T* at, long long stride, int c, int 
 // classes that take no part are zero and their elements are not read; finite
 // biases stay finite.
 template <typename T>
-__global__ void __launch_bounds__(THREADS) pack_kernel(const gsb_class_loss_args a, int D8, int w_tiles,
+__global__ void __launch_bounds__(THREADS) pack_kernel(const gsb_class_loss_args a, const Kept kept, int D8, int w_tiles,
                                                        int* __restrict__ ticket) {
   constexpr int PLANES = sizeof(T) == 4 ? 3 : std::is_same<T, __half>::value ? 2 : 1;
   const int row = threadIdx.x % TILE;
@@ -125,7 +131,7 @@ __global__ void __launch_bounds__(THREADS) pack_kernel(const gsb_class_loss_args
     used = bias != -INFINITY;
     at = (const T*)a.weight + n * a.C;
     stride = 1;
-    if (threadIdx.x < TILE) a.class_bias2[n] = bias;
+    if (threadIdx.x < TILE) kept.class_bias2[n] = bias;
     if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0;
   } else {
     int y = -1;
@@ -136,14 +142,14 @@ __global__ void __launch_bounds__(THREADS) pack_kernel(const gsb_class_loss_args
         else atomicOr((unsigned long long*)a.error_word, (unsigned long long)ERR_BAD_LABEL);
       }
     }
-    if (threadIdx.x < TILE) a.row_y[n] = y;
+    if (threadIdx.x < TILE) kept.row_y[n] = y;
     used = y >= 0;
     const unsigned b = a.B > 1 ? (unsigned)n / (unsigned)max(a.S, 1ll) : 0u;
     at = (const T*)a.features + b * a.stride_b + (n - b * a.S) * a.stride_s;
     stride = a.stride_c;
   }
   const bool contiguous = stride == 1 && (uintptr_t)at % 16 == 0;
-  uint4* const out = (uint4*)(classes ? a.packed_w : a.packed_x) + (size_t)tile * PLANES * D8 * TILE;
+  uint4* const out = (classes ? kept.packed_w : kept.packed_x) + (size_t)tile * PLANES * D8 * TILE;
   for (int d8 = threadIdx.x / TILE; d8 < D8; d8 += THREADS / TILE) {
     float x[8];
     if (used) {
@@ -797,7 +803,7 @@ __device__ __forceinline__ double block_sum(double v) {
 // class takes no part (bias -inf) has the loss +inf and no gradient.  The last
 // CTA to finish adds up the CTAs' sums in their order.
 template <int LANES>
-__global__ void __launch_bounds__(THREADS) join_rows_kernel(const gsb_class_loss_args a, const float* __restrict__ part_m,
+__global__ void __launch_bounds__(THREADS) join_rows_kernel(const gsb_class_loss_args a, const Kept kept, const float* __restrict__ part_m,
                                                             const float* __restrict__ part_s,
                                                             const float* __restrict__ t_label, int slots,
                                                             long long rows, double* __restrict__ block_loss,
@@ -809,7 +815,7 @@ __global__ void __launch_bounds__(THREADS) join_rows_kernel(const gsb_class_loss
        n0 += (long long)gridDim.x * (THREADS / LANES)) {
     const long long n = n0 + threadIdx.x / LANES;
     const bool inside = n < rows;
-    const int y = inside ? a.row_y[n] : -1;
+    const int y = inside ? kept.row_y[n] : -1;
     float m = -INFINITY, s = 0.f;
     if (y >= 0)
       for (int k = sub; k < slots; k += LANES) {
@@ -832,7 +838,7 @@ __global__ void __launch_bounds__(THREADS) join_rows_kernel(const gsb_class_loss
         count += 1.0;
         if (t == -INFINITY) {
           l = INFINITY;
-          a.row_y[n] = -1;
+          kept.row_y[n] = -1;
         } else {
           // (maximum - t) + log2(sum) instead of lse2 - t: the maximum and t often agree in most digits
           const float ls = log2f(s);
@@ -841,7 +847,7 @@ __global__ void __launch_bounds__(THREADS) join_rows_kernel(const gsb_class_loss
         }
         loss += l;
       }
-      a.row_lse2[n] = l2;
+      kept.row_lse2[n] = l2;
       if (a.reduction == GSB_REDUCE_NONE && n < N) a.loss[n] = l;
     }
   }
@@ -866,7 +872,7 @@ __global__ void __launch_bounds__(THREADS) join_rows_kernel(const gsb_class_loss
   count = block_sum(count);
   if (threadIdx.x == 0) {
     const double inv = a.reduction == GSB_REDUCE_MEAN ? 1.0 / fmax(count, 1.0) : 1.0;
-    *a.inv_count = (float)inv;  // what a mean divides by
+    *kept.inv_count = (float)inv;  // what a mean divides by
     if (a.reduction != GSB_REDUCE_NONE) *a.loss = (float)(loss * inv);
   }
 }
@@ -992,6 +998,17 @@ struct Carver {
   }
 };
 
+inline size_t carve_kept(void* base, const Dims& d, Kept* k) {
+  Carver c{(char*)base};
+  k->packed_x = c.take<uint4>((size_t)d.x_tiles * TILE * d.planes * d.D8);
+  k->packed_w = c.take<uint4>((size_t)d.w_tiles * TILE * d.planes * d.D8);
+  k->class_bias2 = c.take<float>((size_t)d.w_tiles * TILE);
+  k->row_lse2 = c.take<float>((size_t)d.x_tiles * TILE);
+  k->row_y = c.take<int>((size_t)d.x_tiles * TILE);
+  k->inv_count = c.take<float>(1);
+  return c.off;
+}
+
 struct FwdWs {
   float *part_m, *part_s, *t_label;
   double *block_loss, *block_count;
@@ -1027,7 +1044,7 @@ inline size_t carve_bwd(void* base, const Dims& d, BwdWs* w) {
   return c.off;
 }
 
-int check_args(const gsb_class_loss_args* a, const char* what) {
+int check_sizes(const gsb_class_loss_args* a, const char* what) {
   if (!a) {
     set_error("%s: null arguments", what);
     return GSB_ERR_INVALID;
@@ -1043,14 +1060,14 @@ int check_args(const gsb_class_loss_args* a, const char* what) {
     set_error("%s: sizes out of range (B %lld, S %lld, C %d, V %lld)", what, a->B, a->S, a->C, a->V);
     return GSB_ERR_INVALID;
   }
-  if ((uintptr_t)a->packed_x % 16 || (uintptr_t)a->packed_w % 16 || (uintptr_t)a->class_bias2 % 16 ||
-      (uintptr_t)a->row_lse2 % 16 || (uintptr_t)a->row_y % 16) {
-    set_error("%s: the buffers kept for backward must be 16-byte aligned", what);
-    return GSB_ERR_INVALID;
-  }
-  if (!a->packed_x || !a->packed_w || !a->class_bias2 || !a->row_lse2 || !a->row_y || !a->inv_count ||
-      !a->error_word || !a->workspace) {
-    set_error("%s: null pointer", what);
+  return GSB_OK;
+}
+
+int check_args(const gsb_class_loss_args* a, const char* what) {
+  const int st = check_sizes(a, what);
+  if (st != GSB_OK) return st;
+  if (!a->kept || !a->error_word || !a->workspace || (uintptr_t)a->kept % 256 || (uintptr_t)a->workspace % 256) {
+    set_error("%s: null or unaligned buffer", what);
     return GSB_ERR_INVALID;
   }
   return GSB_OK;
@@ -1099,19 +1116,18 @@ int launch_stream(const StreamArgs& g, int planes, int tn, cudaStream_t s) {
 }  // namespace
 }  // namespace gsb
 
-GSB_EXPORT size_t gsb_class_loss_packed_bytes(long long rows, int C, int dtype) {
+GSB_EXPORT int gsb_class_loss_sizes(const gsb_class_loss_args* a, size_t sizes[3]) {
   using namespace gsb;
-  if (rows < 0 || C < 1 || dtype < GSB_TYPE_FP32 || dtype > GSB_TYPE_FP16) return 0;
-  return (size_t)std::max(tiles_of(rows), 1ll) * tile_bytes(dtype, C);
-}
-
-GSB_EXPORT size_t gsb_class_loss_workspace_bytes(const gsb_class_loss_args* a, int backward) {
-  using namespace gsb;
-  if (!a || a->B < 0 || a->S < 0 || a->V < 1 || a->C < 1) return 0;
+  const int st = check_sizes(a, "gsb_class_loss_sizes");
+  if (st != GSB_OK) return st;
   const Dims d = dims_of(a);
+  Kept k;
   FwdWs f;
   BwdWs b;
-  return (backward ? carve_bwd(nullptr, d, &b) : carve_fwd(nullptr, d, &f)) + 256;
+  sizes[0] = carve_kept(nullptr, d, &k);
+  sizes[1] = carve_fwd(nullptr, d, &f);
+  sizes[2] = carve_bwd(nullptr, d, &b);
+  return GSB_OK;
 }
 
 GSB_EXPORT int gsb_class_loss_fwd(const gsb_class_loss_args* a, void* stream) {
@@ -1123,18 +1139,19 @@ GSB_EXPORT int gsb_class_loss_fwd(const gsb_class_loss_args* a, void* stream) {
     set_error("gsb_class_loss_fwd: null pointer");
     return GSB_ERR_INVALID;
   }
-  if (a->workspace_bytes < gsb_class_loss_workspace_bytes(a, 0)) {
+  FwdWs w;
+  if (a->workspace_bytes < carve_fwd(a->workspace, d, &w)) {
     set_error("gsb_class_loss_fwd: workspace too small");
     return GSB_ERR_INVALID;
   }
   cudaStream_t s = (cudaStream_t)stream;
-  FwdWs w;
-  carve_fwd((void*)(((uintptr_t)a->workspace + 255) & ~(uintptr_t)255), d, &w);
+  Kept kept;
+  carve_kept(a->kept, d, &kept);
   StreamArgs g{};
-  g.a = (const uint4*)a->packed_x;
-  g.b = (const uint4*)a->packed_w;
-  g.b2 = a->class_bias2;
-  g.y = a->row_y;
+  g.a = kept.packed_x;
+  g.b = kept.packed_w;
+  g.b2 = kept.class_bias2;
+  g.y = kept.row_y;
   g.a_tiles = (int)d.x_tiles;
   g.b_tiles = d.fwd_cols;
   g.splits = d.fwd_splits;
@@ -1146,9 +1163,9 @@ GSB_EXPORT int gsb_class_loss_fwd(const gsb_class_loss_args* a, void* stream) {
   g.t_label = w.t_label;
   const int tiles = (int)(d.w_tiles + d.x_tiles);
   switch (a->dtype) {
-    case GSB_TYPE_BF16: pack_kernel<__nv_bfloat16><<<tiles, THREADS, 0, s>>>(*a, d.D8, (int)d.w_tiles, w.ticket); break;
-    case GSB_TYPE_FP16: pack_kernel<__half><<<tiles, THREADS, 0, s>>>(*a, d.D8, (int)d.w_tiles, w.ticket); break;
-    default: pack_kernel<float><<<tiles, THREADS, 0, s>>>(*a, d.D8, (int)d.w_tiles, w.ticket); break;
+    case GSB_TYPE_BF16: pack_kernel<__nv_bfloat16><<<tiles, THREADS, 0, s>>>(*a, kept, d.D8, (int)d.w_tiles, w.ticket); break;
+    case GSB_TYPE_FP16: pack_kernel<__half><<<tiles, THREADS, 0, s>>>(*a, kept, d.D8, (int)d.w_tiles, w.ticket); break;
+    default: pack_kernel<float><<<tiles, THREADS, 0, s>>>(*a, kept, d.D8, (int)d.w_tiles, w.ticket); break;
   }
   if (d.N > 0) {
     const int r = launch_stream<FWD>(g, d.planes, d.fwd_tn, s);
@@ -1159,10 +1176,10 @@ GSB_EXPORT int gsb_class_loss_fwd(const gsb_class_loss_args* a, void* stream) {
   const int per_cta = slots > 8 ? THREADS / 8 : THREADS;
   const int blocks = (int)std::max(1ll, std::min<long long>(JOIN_BLOCKS, (rows + per_cta - 1) / per_cta));
   if (slots > 8)
-    join_rows_kernel<8><<<blocks, THREADS, 0, s>>>(*a, w.part_m, w.part_s, w.t_label, slots, rows, w.block_loss,
+    join_rows_kernel<8><<<blocks, THREADS, 0, s>>>(*a, kept, w.part_m, w.part_s, w.t_label, slots, rows, w.block_loss,
                                                    w.block_count, w.ticket);
   else
-    join_rows_kernel<1><<<blocks, THREADS, 0, s>>>(*a, w.part_m, w.part_s, w.t_label, slots, rows, w.block_loss,
+    join_rows_kernel<1><<<blocks, THREADS, 0, s>>>(*a, kept, w.part_m, w.part_s, w.t_label, slots, rows, w.block_loss,
                                                    w.block_count, w.ticket);
   return check_launch("gsb_class_loss_fwd");
 }
@@ -1176,7 +1193,8 @@ GSB_EXPORT int gsb_class_loss_bwd(const gsb_class_loss_args* a, void* stream) {
     set_error("gsb_class_loss_bwd: null pointer");
     return GSB_ERR_INVALID;
   }
-  if (a->workspace_bytes < gsb_class_loss_workspace_bytes(a, 1)) {
+  BwdWs w;
+  if (a->workspace_bytes < carve_bwd(a->workspace, d, &w)) {
     set_error("gsb_class_loss_bwd: workspace too small");
     return GSB_ERR_INVALID;
   }
@@ -1186,12 +1204,12 @@ GSB_EXPORT int gsb_class_loss_bwd(const gsb_class_loss_args* a, void* stream) {
     if (a->grad_bias) cudaMemsetAsync(a->grad_bias, 0, (size_t)a->V * 4, s);
     return check_launch("gsb_class_loss_bwd");
   }
-  BwdWs w;
-  carve_bwd((void*)(((uintptr_t)a->workspace + 255) & ~(uintptr_t)255), d, &w);
+  Kept kept;
+  carve_kept(a->kept, d, &kept);
   StreamArgs g{};
-  g.b2 = a->class_bias2;
-  g.lse2 = a->row_lse2;
-  g.y = a->row_y;
+  g.b2 = kept.class_bias2;
+  g.lse2 = kept.row_lse2;
+  g.y = kept.row_y;
   g.error_word = a->error_word;
   g.D8 = d.D8;
   const bool per_row = a->reduction == GSB_REDUCE_NONE;
@@ -1199,14 +1217,14 @@ GSB_EXPORT int gsb_class_loss_bwd(const gsb_class_loss_args* a, void* stream) {
     GradOut o{};
     o.out = a->grad_features;
     o.upstream = a->upstream;
-    o.inv_count = per_row ? nullptr : a->inv_count;
-    o.y = a->row_y;
+    o.inv_count = per_row ? nullptr : kept.inv_count;
+    o.y = kept.row_y;
     o.rows = d.N;
     o.S = a->stride_c == 1 ? 0 : a->S;
     o.C = a->C;
     o.dtype = a->dtype;
-    g.a = (const uint4*)a->packed_x;
-    g.b = (const uint4*)a->packed_w;
+    g.a = kept.packed_x;
+    g.b = kept.packed_w;
     g.a_tiles = (int)d.x_tiles;
     g.b_tiles = d.dx_cols;
     g.splits = d.dx_splits;
@@ -1222,12 +1240,12 @@ GSB_EXPORT int gsb_class_loss_bwd(const gsb_class_loss_args* a, void* stream) {
     GradOut o{};
     o.out = a->grad_weight;
     o.upstream = per_row ? nullptr : a->upstream;  // a row's factor is already in P
-    o.inv_count = per_row ? nullptr : a->inv_count;
+    o.inv_count = per_row ? nullptr : kept.inv_count;
     o.rows = a->V;
     o.C = a->C;
     o.dtype = a->dtype;
-    g.a = (const uint4*)a->packed_w;
-    g.b = (const uint4*)a->packed_x;
+    g.a = kept.packed_w;
+    g.b = kept.packed_x;
     g.a_tiles = (int)d.w_tiles;
     g.b_tiles = d.dw_cols;
     g.splits = d.dw_splits;
@@ -1237,7 +1255,7 @@ GSB_EXPORT int gsb_class_loss_bwd(const gsb_class_loss_args* a, void* stream) {
     g.grad = GradOut{};
     if (d.dw_splits == 1) g.grad = o;
     if (per_row) {
-      row_upstream_kernel<<<div_up(d.x_tiles * TILE, THREADS), THREADS, 0, s>>>(a->upstream, a->row_y, d.x_tiles * TILE,
+      row_upstream_kernel<<<div_up(d.x_tiles * TILE, THREADS), THREADS, 0, s>>>(a->upstream, kept.row_y, d.x_tiles * TILE,
                                                                                w.row_u);
       g.row_u = w.row_u;
     }

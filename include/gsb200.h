@@ -504,26 +504,20 @@ typedef struct {
   const float* bias;      /* (V) or NULL */
   const void* labels;     /* (B * S) int64, or int32 if labels64 is 0 */
   float* loss;            /* 1, or B * S with GSB_REDUCE_NONE */
-  /* kept from forward for backward, each 16-byte aligned: */
-  void* packed_x;         /* gsb_class_loss_packed_bytes(B * S, C, dtype) */
-  void* packed_w;         /* gsb_class_loss_packed_bytes(V, C, dtype) */
-  float* class_bias2;     /* V rounded up to 128 */
-  float* row_lse2;        /* B * S rounded up to 128 */
-  int* row_y;             /* B * S rounded up to 128 */
-  float* inv_count;       /* 1 */
+  void* kept;             /* what forward leaves for backward: sizes[0] bytes, 256-byte aligned */
   /* backward: */
   const float* upstream;  /* device, like loss */
   void* grad_features;    /* (B,S,C) if stride_c is 1, else (B,C,S), contiguous; or NULL */
   void* grad_weight;      /* (V,C) or NULL */
   float* grad_bias;       /* (V) or NULL */
   long long* error_word;  /* device word */
-  void* workspace;        /* gsb_class_loss_workspace_bytes() */
+  void* workspace;        /* sizes[1] bytes in forward, sizes[2] in backward, 256-byte aligned */
   size_t workspace_bytes;
 } gsb_class_loss_args;
 
-size_t gsb_class_loss_packed_bytes(long long rows, int C, int dtype);
-/* reads the sizes, dtype and reduction of the arguments only */
-size_t gsb_class_loss_workspace_bytes(const gsb_class_loss_args* a, int backward);
+/* Bytes of kept, of the forward workspace and of the backward workspace; reads
+ * the sizes and the dtype of the arguments only. */
+int gsb_class_loss_sizes(const gsb_class_loss_args* a, size_t sizes[3]);
 int gsb_class_loss_fwd(const gsb_class_loss_args* a, void* stream);
 int gsb_class_loss_bwd(const gsb_class_loss_args* a, void* stream);
 

@@ -73,8 +73,7 @@ def test_rows_address_every_element_of_a_strided_map(shape, strides, copied):
 def _args(**kw):
     a = _lib.ClassLossArgs()
     a.B, a.S, a.V, a.C, a.reduction = 1, 10, 4, 3, 2
-    for k in ("packed_x", "packed_w", "class_bias2", "row_lse2", "row_y", "inv_count", "error_word", "workspace",
-              "features", "weight", "labels", "loss", "upstream"):
+    for k in ("kept", "error_word", "workspace", "features", "weight", "labels", "loss", "upstream"):
         setattr(a, k, 256)  # refused before anything reads them
     a.workspace_bytes = 1 << 40
     for k, v in kw.items():
@@ -82,12 +81,13 @@ def _args(**kw):
     return a
 
 
-@pytest.mark.parametrize("kw", [dict(B=-1), dict(S=-1), dict(S=(1 << 31) - 128), dict(B=1 << 20, S=1 << 20),
-                                dict(B=1 << 31), dict(V=0), dict(V=(1 << 31) - 128), dict(C=0), dict(C=129),
-                                dict(C=257, dtype=1), dict(dtype=3), dict(reduction=3), dict(packed_x=None),
-                                dict(packed_w=None), dict(row_y=None), dict(inv_count=None), dict(workspace=None),
-                                dict(error_word=None), dict(workspace_bytes=0), dict(packed_x=264),
-                                dict(packed_w=264), dict(class_bias2=260), dict(row_lse2=264), dict(row_y=252)])
+SIZES = [dict(B=-1), dict(S=-1), dict(S=(1 << 31) - 128), dict(B=1 << 20, S=1 << 20), dict(B=1 << 31), dict(V=0),
+         dict(V=(1 << 31) - 128), dict(C=0), dict(C=129), dict(C=257, dtype=1), dict(dtype=3), dict(reduction=3)]
+BUFFERS = [dict(kept=None), dict(workspace=None), dict(error_word=None), dict(workspace_bytes=0), dict(kept=264),
+           dict(workspace=264)]
+
+
+@pytest.mark.parametrize("kw", SIZES + BUFFERS)
 def test_c_abi_refuses(kw):
     L = _lib.load()
     for fn in (L.gsb_class_loss_fwd, L.gsb_class_loss_bwd):
@@ -103,11 +103,19 @@ def test_c_abi_refuses_missing_inputs():
     assert L.gsb_class_loss_fwd(None, None) == _lib.GSB_ERR_INVALID
 
 
+def _sizes(**kw):
+    out = (ctypes.c_size_t * 3)()
+    status = _lib.load().gsb_class_loss_sizes(ctypes.byref(_args(**kw)), out)
+    return status, list(out)
+
+
 def test_buffer_sizes():
-    L = _lib.load()
-    packed = L.gsb_class_loss_packed_bytes
-    assert packed(128, 16, 1) == 128 * 16 * 2
-    assert packed(129, 17, 0) == 2 * 3 * 128 * 32 * 2
-    assert packed(1, 16, 2) == 2 * 128 * 16 * 2
-    ws = L.gsb_class_loss_workspace_bytes
-    assert ws(ctypes.byref(_args()), 0) > 0 and ws(ctypes.byref(_args(S=1_000_000)), 1) > ws(ctypes.byref(_args()), 1)
+    for kw in SIZES:
+        assert _sizes(**kw)[0] == _lib.GSB_ERR_INVALID
+    # the packed operands: planes of bf16, channels to a multiple of 16, rows and classes to 128
+    status, (kept, fwd, bwd) = _sizes(S=129, V=300, C=17, dtype=0)
+    packed = 3 * 32 * 2 * (256 + 384)
+    assert status == _lib.GSB_OK and packed <= kept <= packed + 4 * (384 + 2 * 256) + 6 * 256
+    assert fwd > 0 and bwd > 0
+    assert _sizes(S=1_000_000)[1][0] > _sizes()[1][0]
+    assert _sizes(S=0)[0] == _lib.GSB_OK
