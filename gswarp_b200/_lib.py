@@ -299,9 +299,15 @@ def call(name: str, *args) -> None:
 
 def call_on(device: torch.device, name: str, args) -> None:
     """``call`` on ``device``'s current stream, with ``device`` made current
-    only if it is not (the operators of a few microseconds pay for both)."""
-    if torch.cuda.current_device() == device.index:
-        call(name, args, torch.cuda.current_stream(device).cuda_stream)
+    only if it is not: an operator of a few microseconds notices both the
+    context manager and a Stream object."""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        call(name, args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            call(name, args, torch.cuda.current_stream(device).cuda_stream)
+        with torch.cuda.device(index):
+            call(name, args, _raw_stream(index))
+
+
+def _raw_stream(index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(index)

@@ -76,8 +76,9 @@ def lookup_backward(table: torch.Tensor, codes: torch.Tensor, scale: float, gain
         grad_table = torch.empty_like(table) if out is None else out
         a.grad_table = grad_table.data_ptr()
         n = _lib.load().gsb_codebook_bwd_workspace_bytes(a.P, a.K, a.D)
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), n
+        if n:
+            ws = torch.empty(n, dtype=torch.uint8, device=dev)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), n
     if want_gain:
         grad_gain = torch.empty_like(gain)
         a.grad_gain = grad_gain.data_ptr()

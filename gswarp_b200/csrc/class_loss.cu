@@ -316,11 +316,11 @@ __device__ __forceinline__ Range unit_range(const StreamArgs& g, int unit) {
 
 // Walks a CTA's units tile by tile, with the rings that go along.
 struct Cursor {
-  int unit, bt;
+  int unit, bt, step;
   Range r;
   Ring as, bs, acc;
   uint32_t t = 0;
-  __device__ __forceinline__ explicit Cursor(const StreamArgs& g) : unit(blockIdx.x) {
+  __device__ __forceinline__ Cursor(const StreamArgs& g, int cta, int ctas) : unit(cta), step(ctas) {
     if (unit < g.a_tiles * g.splits) {
       r = unit_range(g, unit);
       bt = r.lo;
@@ -331,7 +331,7 @@ struct Cursor {
     bs.next(g.stages);
     if (++bt < r.hi) return;
     as.next(g.a_slots);
-    unit += gridDim.x;
+    unit += step;
     if (unit < g.a_tiles * g.splits) {
       r = unit_range(g, unit);
       bt = r.lo;
@@ -382,9 +382,8 @@ __device__ __forceinline__ void store_p(uint32_t buffer, int c, const float2 (&p
 }
 
 template <int MODE, int NP, int TN>
-__global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const StreamArgs g) {
+__device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, const int cta, const int ctas) {
   using namespace tc;
-  extern __shared__ __align__(1024) uint8_t smem[];
   const int D8 = g.D8, D = D8 * 8;
   const uint32_t a_bytes = (uint32_t)NP * D8 * 2048, b_bytes = (uint32_t)NP * D8 * TN * 16;
   constexpr uint32_t META = (uint32_t)meta_floats<MODE>(TN);
@@ -432,7 +431,7 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
     // ---- loads ----
     Ring as, bs;
     bool ok = true;
-    for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+    for (int u = cta; u < units && ok; u += ctas) {
       const Range r = unit_range(g, u);
       ok = warp_wait(&bar->a_empty[as.i], as.phase ^ 1, stop);
       if (!ok) break;
@@ -477,7 +476,7 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
     const uint32_t idesc = instr_desc(TN, false), hi = desc_hi(NP * D8 * 128);
     const uint32_t a0 = smem_u32(sA), b0 = smem_u32(sB);
     bool ok = true;
-    for (Cursor c(g); c.unit < units; c.next(g)) {
+    for (Cursor c(g, cta, ctas); c.unit < units; c.next(g)) {
       const uint32_t b = c.t % GROUPS;
       ok = (c.bt > c.r.lo || warp_wait(&bar->a_full[c.as.i], c.as.phase, stop)) &&
            warp_wait(&bar->b_full[c.bs.i], c.bs.phase, stop) &&
@@ -510,7 +509,7 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
     const uint32_t idesc = instr_desc(D, true), hi = desc_hi(128), step = NP * D8 * 16;
     const uint32_t b0 = smem_u32(sB);
     bool ok = true;
-    for (Cursor c(g); c.unit < units; c.next(g)) {
+    for (Cursor c(g, cta, ctas); c.unit < units; c.next(g)) {
       const uint32_t b = c.t % GROUPS;
       const int in_acc = (c.bt - c.r.lo) % g.flush;
       const bool first = in_acc == 0, last = in_acc + 1 == g.flush || c.bt + 1 == c.r.hi;
@@ -548,7 +547,7 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
     constexpr int CH = MODE == FWD ? 32 : 16;  // columns in registers at a time
     const int group = warp / 4;
     const uint32_t buffer = tmem + lanes + group * SBUF;
-    const int step = gridDim.x;
+    const int step = ctas;
     Ring bs;
     uint32_t t = 0;
     bool ok = true;
@@ -561,8 +560,8 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
       if (MODE == DX) c_next = -g.lse2[row];
       if (MODE == DW) c_next = g.b2[row];
     };
-    fetch(blockIdx.x);
-    for (int u = blockIdx.x; u < units && ok; u += step) {
+    fetch(cta);
+    for (int u = cta; u < units && ok; u += step) {
       const Range r = unit_range(g, u);
       const int row = r.tile * TILE + (warp & 3) * 32 + lane;
       const int y = y_next;
@@ -709,7 +708,7 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
     // all of the streamed axis) straight into the gradient ----
     Ring acc;
     bool ok = true;
-    for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+    for (int u = cta; u < units && ok; u += ctas) {
       const Range r = unit_range(g, u);
       const size_t tile = (size_t)r.split * g.a_tiles + r.tile;
       const int row = (warp & 3) * 32 + lane;
@@ -779,6 +778,21 @@ __global__ void __launch_bounds__(stream_threads<MODE>(), 1) stream_kernel(const
   if (warp == ISSUER) tmem_free(tmem, TMEM_COLUMNS);
   if (threadIdx.x == 0 && *stop)
     atomicOr((unsigned long long*)g.error_word, (unsigned long long)ERR_LOOKBACK_TIMEOUT);
+}
+
+template <int NP, int TN>
+__global__ void __launch_bounds__(stream_threads<FWD>(), 1) forward_kernel(const StreamArgs g) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  stream_pass<FWD, NP, TN>(g, smem, blockIdx.x, gridDim.x);
+}
+
+// Both gradients in one launch: dW's CTAs follow dX's without a gap.
+template <int NP, int TN>
+__global__ void __launch_bounds__(stream_threads<DX>(), 1)
+    backward_kernel(const StreamArgs gx, const StreamArgs gw, const int x_ctas) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if ((int)blockIdx.x < x_ctas) stream_pass<DX, NP, TN>(gx, smem, blockIdx.x, x_ctas);
+  else stream_pass<DW, NP, TN>(gw, smem, blockIdx.x - x_ctas, gridDim.x - x_ctas);
 }
 
 // ---------------------------------------------------------------------------
@@ -886,17 +900,37 @@ __global__ void __launch_bounds__(THREADS) row_upstream_kernel(const float* __re
   if (n < rows) out[n] = row_y[n] >= 0 ? up[n] : 0.f;
 }
 
-// Sums the splits' partial rows: a CTA takes 32 quads of four columns, eight
-// threads each, which take every eighth split and are added in order.
-__global__ void __launch_bounds__(THREADS) join_acc_kernel(const GradOut o, const float4* __restrict__ part, int splits,
-                                                           int D, long long quads) {
+// What the passes left in pieces: dX's and dW's partial rows (entries are
+// quads of columns, [tile][column / 4][row]) and the bias's partial sums.  A
+// CTA takes 32 entries, eight threads each, which take every eighth piece and
+// are added in order.  Counts are multiples of 128.
+struct Join {
+  GradOut out;
+  const float* part;
+  long long count;
+  int splits;
+};
+struct Joins {
+  Join x, w, bias;
+};
+
+__global__ void __launch_bounds__(THREADS) join_grads_kernel(const Joins j, int D) {
   __shared__ float4 s_part[8][32];
   const int lane = threadIdx.x % 32, sub = threadIdx.x / 32;
-  const long long q = (long long)blockIdx.x * 32 + lane;  // [tile][column / 4][row]; a multiple of 128 in all
+  long long q = (long long)blockIdx.x * 32 + lane;
+  const bool is_x = q < j.x.count;
+  if (!is_x) q -= j.x.count;
+  const bool is_bias = !is_x && q >= j.w.count;
+  if (is_bias) q -= j.w.count;
+  const Join& in = is_x ? j.x : is_bias ? j.bias : j.w;
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int k = sub; k < splits; k += 8) {
-    const float4 v = part[(size_t)k * quads + q];
-    sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
+  for (int k = sub; k < in.splits; k += 8) {
+    if (is_bias) {
+      sum.x += in.part[k * in.count + q];
+    } else {
+      const float4 v = reinterpret_cast<const float4*>(in.part)[k * in.count + q];
+      sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
+    }
   }
   s_part[sub][lane] = sum;
   __syncthreads();
@@ -905,25 +939,15 @@ __global__ void __launch_bounds__(THREADS) join_acc_kernel(const GradOut o, cons
     const float4 v = s_part[k][lane];
     sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
   }
+  if (is_bias) {
+    if (q < in.out.rows) ((float*)in.out.out)[q] = sum.x * grad_scale(in.out, q);
+    return;
+  }
   const long long strip = q / TILE;
   const long long n = strip / (D / 4) * TILE + q % TILE;
-  if (n >= o.rows) return;
+  if (n >= in.out.rows) return;
   const float v[4] = {sum.x, sum.y, sum.z, sum.w};
-  write_grad(o, n, (int)(strip % (D / 4)) * 4, v, grad_scale(o, n));
-}
-
-__global__ void __launch_bounds__(THREADS) join_bias_kernel(const GradOut o, const float* __restrict__ part, int slots,
-                                                            long long rows) {
-  __shared__ float s_part[8][32];
-  const int lane = threadIdx.x % 32, sub = threadIdx.x / 32;
-  const long long v = (long long)blockIdx.x * 32 + lane;  // rows is a multiple of 128
-  float sum = 0.f;
-  for (int k = sub; k < slots; k += 8) sum += part[k * rows + v];
-  s_part[sub][lane] = sum;
-  __syncthreads();
-  if (sub != 0 || v >= o.rows) return;
-  for (int k = 1; k < 8; ++k) sum += s_part[k][lane];
-  ((float*)o.out)[v] = sum * grad_scale(o, v);
+  write_grad(in.out, n, (int)(strip % (D / 4)) * 4, v, grad_scale(in.out, n));
 }
 
 // ---------------------------------------------------------------------------
@@ -960,7 +984,7 @@ inline int tile_columns(int planes, int D8) {
 struct Dims {
   long long N, x_tiles, w_tiles;  // tiles of 128 rows, as packed
   int D, D8, planes;
-  int fwd_tn, dx_tn, dw_tn;       // rows of a streamed tile
+  int fwd_tn, grad_tn;            // rows of a streamed tile
   int fwd_cols, dx_cols, dw_cols;  // streamed tiles
   int fwd_splits, dx_splits, dw_splits;
   int fwd_slots, dw_slots;        // partial results per split
@@ -974,11 +998,10 @@ inline Dims dims_of(const gsb_class_loss_args* a) {
   d.D8 = d.D / 8;
   d.planes = planes_of(a->dtype);
   d.fwd_tn = tile_columns<FWD>(d.planes, d.D8);
-  d.dx_tn = tile_columns<DX>(d.planes, d.D8);
-  d.dw_tn = tile_columns<DW>(d.planes, d.D8);
+  d.grad_tn = tile_columns<DW>(d.planes, d.D8);
   d.fwd_cols = div_up(a->V, d.fwd_tn);
-  d.dx_cols = div_up(a->V, d.dx_tn);
-  d.dw_cols = div_up(d.N, d.dw_tn);
+  d.dx_cols = div_up(a->V, d.grad_tn);
+  d.dw_cols = div_up(d.N, d.grad_tn);
   d.fwd_splits = d.x_tiles > 0 ? split_count(d.x_tiles, d.fwd_cols) : 1;
   d.dx_splits = d.x_tiles > 0 ? split_count(d.x_tiles, d.dx_cols) : 1;
   d.dw_splits = split_count(d.w_tiles, std::max(d.dw_cols, 1));
@@ -1037,8 +1060,8 @@ inline bool needs_partials(int splits, int cols, int tn, int planes) {
 inline size_t carve_bwd(void* base, const Dims& d, BwdWs* w) {
   Carver c{(char*)base};
   const size_t x = (size_t)d.x_tiles * TILE, v = (size_t)d.w_tiles * TILE;
-  w->part_x = c.take<float>(needs_partials(d.dx_splits, d.dx_cols, d.dx_tn, d.planes) ? x * d.dx_splits * d.D : 0);
-  w->part_w = c.take<float>(needs_partials(d.dw_splits, d.dw_cols, d.dw_tn, d.planes) ? v * d.dw_splits * d.D : 0);
+  w->part_x = c.take<float>(needs_partials(d.dx_splits, d.dx_cols, d.grad_tn, d.planes) ? x * d.dx_splits * d.D : 0);
+  w->part_w = c.take<float>(needs_partials(d.dw_splits, d.dw_cols, d.grad_tn, d.planes) ? v * d.dw_splits * d.D : 0);
   w->part_bias = c.take<float>(v * d.dw_splits * d.dw_slots);
   w->row_u = c.take<float>(x);
   return c.off;
@@ -1073,44 +1096,38 @@ int check_args(const gsb_class_loss_args* a, const char* what) {
   return GSB_OK;
 }
 
+// Fills in what a pass's CTAs have room for; returns its shared memory.
 template <int MODE, int NP, int TN>
-int launch_tiled(StreamArgs g, cudaStream_t s) {
-  const size_t a_bytes = (size_t)NP * g.D8 * 2048;
-  const size_t stage = (size_t)NP * g.D8 * TN * 16 + meta_floats<MODE>(TN) * 4;
+size_t plan_pass(StreamArgs* g) {
+  const size_t a_bytes = (size_t)NP * g->D8 * 2048;
+  const size_t stage = (size_t)NP * g->D8 * TN * 16 + meta_floats<MODE>(TN) * 4;
   const size_t fixed = sizeof(Barriers) + 128;
   constexpr int SBUF = z_columns<MODE>(NP, TN), ACCS = accumulators(NP);
-  g.flush = chain_products(NP) / (TN / 16);
-  for (g.a_slots = MAX_A_SLOTS; g.a_slots > 1; --g.a_slots)
-    if (g.a_slots * a_bytes + 6 * stage + fixed <= SMEM_MAX) break;
-  g.stages = (int)std::min<size_t>(MAX_STAGES, (SMEM_MAX - fixed - g.a_slots * a_bytes) / stage);
-  const int acc = MODE == FWD ? 0 : ACCS * g.D8 * 8;
   static_assert(GROUPS * SBUF <= TMEM_COLUMNS, "z buffers");
-  g.acc_slots = GROUPS * SBUF + 2 * acc <= TMEM_COLUMNS ? 2 : 1;
-  const size_t smem = std::max(SMEM_MIN, g.a_slots * a_bytes + g.stages * stage + fixed);
-  cudaFuncSetAttribute(stream_kernel<MODE, NP, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  const int units = g.a_tiles * g.splits;
-  stream_kernel<MODE, NP, TN><<<std::min(units, SMS), stream_threads<MODE>(), smem, s>>>(g);
-  return check_launch("class loss pass");
+  g->flush = chain_products(NP) / (TN / 16);
+  for (g->a_slots = MAX_A_SLOTS; g->a_slots > 1; --g->a_slots)
+    if (g->a_slots * a_bytes + 6 * stage + fixed <= SMEM_MAX) break;
+  g->stages = (int)std::min<size_t>(MAX_STAGES, (SMEM_MAX - fixed - g->a_slots * a_bytes) / stage);
+  const int acc = MODE == FWD ? 0 : ACCS * g->D8 * 8;
+  g->acc_slots = GROUPS * SBUF + 2 * acc <= TMEM_COLUMNS ? 2 : 1;
+  return std::max(SMEM_MIN, g->a_slots * a_bytes + g->stages * stage + fixed);
 }
+inline int pass_ctas(const StreamArgs& g) { return std::min(g.a_tiles * g.splits, SMS); }
 
-template <int MODE>
-int launch_stream(const StreamArgs& g, int planes, int tn, cudaStream_t s) {
-  switch (planes * 1000 + tn) {
-    case 1064: return launch_tiled<MODE, 1, 64>(g, s);
-    case 2064: return launch_tiled<MODE, 2, 64>(g, s);
-    case 2032: return launch_tiled<MODE, 2, 32>(g, s);
-    case 3064: return launch_tiled<MODE, 3, 64>(g, s);
-    case 3032: return launch_tiled<MODE, 3, 32>(g, s);
-  }
-  if constexpr (MODE == FWD) {
-    switch (planes * 1000 + tn) {
-      case 1128: return launch_tiled<MODE, 1, 128>(g, s);
-      case 2128: return launch_tiled<MODE, 2, 128>(g, s);
-      case 3128: return launch_tiled<MODE, 3, 128>(g, s);
-    }
-  }
-  set_error("class loss: no pass for %d planes and tiles of %d", planes, tn);
-  return GSB_ERR_INVALID;
+template <int NP, int TN>
+int launch_forward(StreamArgs g, cudaStream_t s) {
+  const size_t smem = plan_pass<FWD, NP, TN>(&g);
+  cudaFuncSetAttribute(forward_kernel<NP, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  forward_kernel<NP, TN><<<pass_ctas(g), stream_threads<FWD>(), smem, s>>>(g);
+  return check_launch("class loss forward");
+}
+template <int NP, int TN>
+int launch_backward(StreamArgs gx, StreamArgs gw, cudaStream_t s) {
+  const size_t smem = std::max(plan_pass<DX, NP, TN>(&gx), plan_pass<DW, NP, TN>(&gw));
+  cudaFuncSetAttribute(backward_kernel<NP, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  const int x_ctas = pass_ctas(gx);
+  backward_kernel<NP, TN><<<x_ctas + pass_ctas(gw), stream_threads<DX>(), smem, s>>>(gx, gw, x_ctas);
+  return check_launch("class loss backward");
 }
 
 }  // namespace
@@ -1168,7 +1185,18 @@ GSB_EXPORT int gsb_class_loss_fwd(const gsb_class_loss_args* a, void* stream) {
     default: pack_kernel<float><<<tiles, THREADS, 0, s>>>(*a, kept, d.D8, (int)d.w_tiles, w.ticket); break;
   }
   if (d.N > 0) {
-    const int r = launch_stream<FWD>(g, d.planes, d.fwd_tn, s);
+    int r = GSB_ERR_INVALID;
+    switch (d.planes * 1000 + d.fwd_tn) {
+      case 1128: r = launch_forward<1, 128>(g, s); break;
+      case 1064: r = launch_forward<1, 64>(g, s); break;
+      case 2128: r = launch_forward<2, 128>(g, s); break;
+      case 2064: r = launch_forward<2, 64>(g, s); break;
+      case 2032: r = launch_forward<2, 32>(g, s); break;
+      case 3128: r = launch_forward<3, 128>(g, s); break;
+      case 3064: r = launch_forward<3, 64>(g, s); break;
+      case 3032: r = launch_forward<3, 32>(g, s); break;
+      default: set_error("gsb_class_loss_fwd: no pass for %d planes and tiles of %d", d.planes, d.fwd_tn);
+    }
     if (r != GSB_OK) return r;
   }
   const int slots = d.fwd_splits * d.fwd_slots;
@@ -1212,9 +1240,12 @@ GSB_EXPORT int gsb_class_loss_bwd(const gsb_class_loss_args* a, void* stream) {
   g.y = kept.row_y;
   g.error_word = a->error_word;
   g.D8 = d.D8;
-  const bool per_row = a->reduction == GSB_REDUCE_NONE;
+  const bool per_row = a->reduction == GSB_REDUCE_NONE, want_w = a->grad_weight || a->grad_bias;
+  if (!a->grad_features && !want_w) return GSB_OK;
+  StreamArgs gx = g, gw = g;  // no units unless wanted
+  Joins joins{};
   if (a->grad_features) {
-    GradOut o{};
+    GradOut& o = joins.x.out;
     o.out = a->grad_features;
     o.upstream = a->upstream;
     o.inv_count = per_row ? nullptr : kept.inv_count;
@@ -1223,51 +1254,67 @@ GSB_EXPORT int gsb_class_loss_bwd(const gsb_class_loss_args* a, void* stream) {
     o.S = a->stride_c == 1 ? 0 : a->S;
     o.C = a->C;
     o.dtype = a->dtype;
-    g.a = kept.packed_x;
-    g.b = kept.packed_w;
-    g.a_tiles = (int)d.x_tiles;
-    g.b_tiles = d.dx_cols;
-    g.splits = d.dx_splits;
-    g.part_acc = w.part_x;
-    if (d.dx_splits == 1) g.grad = o;
-    const int r = launch_stream<DX>(g, d.planes, d.dx_tn, s);
-    if (r != GSB_OK) return r;
-    const long long quads = d.x_tiles * TILE * (d.D / 4);
-    if (d.dx_splits > 1)
-      join_acc_kernel<<<(unsigned)(quads / 32), THREADS, 0, s>>>(o, (const float4*)w.part_x, d.dx_splits, d.D, quads);
+    gx.a = kept.packed_x;
+    gx.b = kept.packed_w;
+    gx.a_tiles = (int)d.x_tiles;
+    gx.b_tiles = d.dx_cols;
+    gx.splits = d.dx_splits;
+    gx.part_acc = w.part_x;
+    if (d.dx_splits == 1) {
+      gx.grad = o;
+    } else {
+      joins.x.part = w.part_x;
+      joins.x.splits = d.dx_splits;
+      joins.x.count = d.x_tiles * TILE * (d.D / 4);
+    }
   }
-  if (a->grad_weight || a->grad_bias) {
-    GradOut o{};
+  if (want_w) {
+    GradOut& o = joins.w.out;
     o.out = a->grad_weight;
     o.upstream = per_row ? nullptr : a->upstream;  // a row's factor is already in P
     o.inv_count = per_row ? nullptr : kept.inv_count;
     o.rows = a->V;
     o.C = a->C;
     o.dtype = a->dtype;
-    g.a = kept.packed_w;
-    g.b = kept.packed_x;
-    g.a_tiles = (int)d.w_tiles;
-    g.b_tiles = d.dw_cols;
-    g.splits = d.dw_splits;
-    g.slots = d.dw_slots;
-    g.part_acc = a->grad_weight ? w.part_w : nullptr;
-    g.part_bias = w.part_bias;
-    g.grad = GradOut{};
-    if (d.dw_splits == 1) g.grad = o;
-    if (per_row) {
-      row_upstream_kernel<<<div_up(d.x_tiles * TILE, THREADS), THREADS, 0, s>>>(a->upstream, kept.row_y, d.x_tiles * TILE,
-                                                                               w.row_u);
-      g.row_u = w.row_u;
+    joins.bias.out = o;
+    gw.a = kept.packed_w;
+    gw.b = kept.packed_x;
+    gw.a_tiles = (int)d.w_tiles;
+    gw.b_tiles = d.dw_cols;
+    gw.splits = d.dw_splits;
+    gw.slots = d.dw_slots;
+    gw.part_acc = a->grad_weight ? w.part_w : nullptr;
+    gw.part_bias = w.part_bias;
+    if (d.dw_splits == 1) {
+      gw.grad = o;
+    } else if (a->grad_weight) {
+      joins.w.part = w.part_w;
+      joins.w.splits = d.dw_splits;
+      joins.w.count = d.w_tiles * TILE * (d.D / 4);
     }
-    const int r = launch_stream<DW>(g, d.planes, d.dw_tn, s);
-    if (r != GSB_OK) return r;
-    const long long rows = d.w_tiles * TILE, quads = rows * (d.D / 4);
-    if (a->grad_weight && d.dw_splits > 1)
-      join_acc_kernel<<<(unsigned)(quads / 32), THREADS, 0, s>>>(o, (const float4*)w.part_w, d.dw_splits, d.D, quads);
     if (a->grad_bias) {
-      o.out = a->grad_bias;
-      join_bias_kernel<<<(unsigned)(rows / 32), THREADS, 0, s>>>(o, w.part_bias, d.dw_splits * d.dw_slots, rows);
+      joins.bias.out.out = a->grad_bias;
+      joins.bias.part = w.part_bias;
+      joins.bias.splits = d.dw_splits * d.dw_slots;
+      joins.bias.count = d.w_tiles * TILE;
+    }
+    if (per_row) {
+      row_upstream_kernel<<<div_up(d.x_tiles * TILE, THREADS), THREADS, 0, s>>>(a->upstream, kept.row_y,
+                                                                               d.x_tiles * TILE, w.row_u);
+      gw.row_u = w.row_u;
     }
   }
+  int r = GSB_ERR_INVALID;
+  switch (d.planes * 1000 + d.grad_tn) {
+    case 1064: r = launch_backward<1, 64>(gx, gw, s); break;
+    case 2064: r = launch_backward<2, 64>(gx, gw, s); break;
+    case 2032: r = launch_backward<2, 32>(gx, gw, s); break;
+    case 3064: r = launch_backward<3, 64>(gx, gw, s); break;
+    case 3032: r = launch_backward<3, 32>(gx, gw, s); break;
+    default: set_error("gsb_class_loss_bwd: no pass for %d planes and tiles of %d", d.planes, d.grad_tn);
+  }
+  if (r != GSB_OK) return r;
+  const long long blocks = (joins.x.count + joins.w.count + joins.bias.count) / 32;
+  if (blocks > 0) join_grads_kernel<<<(unsigned)blocks, THREADS, 0, s>>>(joins, d.D);
   return check_launch("gsb_class_loss_bwd");
 }

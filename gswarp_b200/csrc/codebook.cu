@@ -11,14 +11,16 @@
 //   dgain[p] = scale * <g[p,:], T[c_p,:]>.
 //
 // Forward moves P rows and is bound by that write.  Backward is bound by the
-// one read of g; the sums go by sorted code instead of atomics, so that they
-// have one order (the same bits on every call) and no hot row serializes:
-// the codes are sorted (radix_sort.cuh, only the key bits of K), the sorted
-// positions are cut into chunks of equal length, and one group of lanes sums
-// each chunk's runs in registers in fp32.  A run that lies inside its chunk
-// is stored at once; the at most two that cross a chunk's ends become rows of
-// a next level (key, fp32 sum), summed by the same kernel, until one chunk is
-// left.  Sums are therefore trees of short sequential sums.
+// one read of g; the sums go by code instead of atomics, so that they have one
+// order (the same bits on every call) and no hot row serializes.
+//
+// Many rows: the codes are sorted (radix_sort.cuh's passes over the key bits
+// of K), the sorted positions are cut into chunks of equal length, and one
+// group of lanes sums each chunk's runs in registers in fp32.  A run that lies
+// inside its chunk is stored at once; the at most two that cross a chunk's
+// ends leave fp32 partial rows, which a second kernel adds up, a warp for each
+// such run (a CTA for the longest).  Few rows or codes: warps scan all the
+// codes for the ones they own, in one launch.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -32,7 +34,6 @@ namespace {
 
 constexpr int THREADS = launch::CODEBOOK;
 constexpr int SEG_UNROLL = 4;       // rows in flight per group of lanes
-constexpr int FWD_CTA_ROWS = 64;    // rows per CTA of the gather; a multiple of 16 keeps CTAs 16-byte aligned
 constexpr long long MAX_ROWS = (1ll << 31) - 4096;
 
 template <typename T>
@@ -82,113 +83,233 @@ __device__ __forceinline__ long long read_code(const void* codes, int codes64, l
 }
 
 // ---------------------------------------------------------------------------
-// Forward.  A CTA owns FWD_CTA_ROWS consecutive rows; their codes and factors
-// go through shared memory, and the threads walk the CTA's flat output in
-// 16-byte pieces.  ALIGNED: rows are whole 16-byte pieces and both pointers
-// are aligned, so a piece is one load; otherwise a piece may cross rows and
-// is gathered element by element (the rows come from L1/L2), while its store
-// still is one when the output is aligned.
+// Forward.  A CTA owns ROWS consecutive rows (a multiple of 16, which keeps
+// CTAs 16-byte aligned); their codes and factors go through shared memory, and
+// the threads walk the CTA's flat output in 16-byte pieces, several in flight.
+// ALIGNED: rows are whole 16-byte pieces and both pointers are aligned, so a
+// piece is one load; otherwise a piece may cross rows and is gathered element
+// by element (the rows come from L1/L2), while its store still is one when the
+// output is aligned.
 // ---------------------------------------------------------------------------
-template <typename T, bool ALIGNED>
+template <typename T, bool ALIGNED, int ROWS>
 __global__ void __launch_bounds__(THREADS) codebook_gather_kernel(const gsb_codebook_args a, int out_aligned) {
   constexpr int VW = Vec16<T>::N;
-  __shared__ int s_code[FWD_CTA_ROWS];
-  __shared__ float s_scale[FWD_CTA_ROWS];
-  const long long base = (long long)blockIdx.x * FWD_CTA_ROWS;
-  const int rows = (int)min((long long)FWD_CTA_ROWS, a.P - base);
+  constexpr int UNROLL = ALIGNED ? 4 : 2;
+  __shared__ int s_code[ROWS];
+  __shared__ float s_scale[ROWS];
+  const long long base = (long long)blockIdx.x * ROWS;
+  const int rows = (int)min((long long)ROWS, a.P - base);
   const int tid = threadIdx.x;
-  if (tid < rows) {
-    const long long c = read_code(a.codes, a.codes64, base + tid);
+  for (int i = tid; i < rows; i += THREADS) {
+    const long long c = read_code(a.codes, a.codes64, base + i);
     const bool ok = c >= 0 && c < a.K;
     if (c < -1 || c >= a.K) atomicOr((unsigned long long*)a.error_word, (unsigned long long)ERR_BAD_CODE);
-    s_code[tid] = ok ? (int)c : -1;
-    s_scale[tid] = a.gain ? a.scale * a.gain[base + tid] : a.scale;
+    s_code[i] = ok ? (int)c : -1;
+    s_scale[i] = a.gain ? a.scale * a.gain[base + i] : a.scale;
   }
   __syncthreads();
   const T* table = (const T*)a.table;
   T* out = (T*)a.out + base * a.D;
   const unsigned D = (unsigned)a.D;
   const unsigned total = (unsigned)rows * D;
-  for (unsigned e = (unsigned)tid * VW; e < total; e += THREADS * VW) {
-    unsigned r = e / D, col = e - r * D;
-    float v[VW];
-    if constexpr (ALIGNED) {
-      const int c = s_code[r];
-      if (c >= 0) {
-        load_vec<T, VW>(table + (long long)c * D + col, v);
-        const float s = s_scale[r];
+  for (unsigned e0 = (unsigned)tid * VW; e0 < total; e0 += THREADS * VW * UNROLL) {
+    float v[UNROLL][VW], s[UNROLL];
 #pragma unroll
-        for (int i = 0; i < VW; ++i) v[i] *= s;
+    for (int u = 0; u < UNROLL; ++u) {
+      const unsigned e = e0 + u * (THREADS * VW);
+      s[u] = 1.f;
+#pragma unroll
+      for (int i = 0; i < VW; ++i) v[u][i] = 0.f;
+      if (e >= total) continue;
+      unsigned r = e / D, col = e - r * D;
+      if constexpr (ALIGNED) {
+        const int c = s_code[r];
+        s[u] = s_scale[r];
+        if (c >= 0) load_vec<T, VW>(table + (long long)c * D + col, v[u]);
       } else {
 #pragma unroll
-        for (int i = 0; i < VW; ++i) v[i] = 0.f;
+        for (int i = 0; i < VW; ++i) {
+          if (e + i < total) {
+            const int c = s_code[r];
+            if (c >= 0) v[u][i] = s_scale[r] * to_f(table[(long long)c * D + col]);
+          }
+          if (++col == D) {
+            col = 0;
+            r = min(r + 1, (unsigned)rows - 1);
+          }
+        }
       }
-      store_vec<T, VW>(out + e, v);
-    } else {
+    }
 #pragma unroll
-      for (int i = 0; i < VW; ++i) {
-        v[i] = 0.f;
-        if (e + i < total) {
-          const int c = s_code[r];
-          if (c >= 0) v[i] = s_scale[r] * to_f(table[(long long)c * D + col]);
-        }
-        if (++col == D) {
-          col = 0;
-          ++r;
-          if (r >= (unsigned)rows) r = rows - 1;
-        }
+    for (int u = 0; u < UNROLL; ++u) {
+      const unsigned e = e0 + u * (THREADS * VW);
+      if (e >= total) continue;
+      if constexpr (ALIGNED) {
+#pragma unroll
+        for (int i = 0; i < VW; ++i) v[u][i] *= s[u];
       }
-      if (out_aligned && e + VW <= total) {
-        store_vec<T, VW>(out + e, v);
+      if (ALIGNED || (out_aligned && e + VW <= total)) {
+        store_vec<T, VW>(out + e, v[u]);
       } else {
 #pragma unroll
         for (int i = 0; i < VW; ++i)
-          if (e + i < total) out[e + i] = from_f<T>(v[i]);
+          if (e + i < total) out[e + i] = from_f<T>(v[u][i]);
       }
     }
   }
 }
 
 // ---------------------------------------------------------------------------
-// Backward, step 1: sort keys.  Rows without a code get key K, behind every
-// code.
+// Backward of few rows: P * K and P below the bounds of small_case().  A code
+// belongs to `wpc` warps of a CTA, each of which scans its part of the codes
+// and adds up the rows it finds, in order; the parts are then added in order.
+// One more "code" takes the rows without one (their gains' gradient is zero).
 // ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(THREADS) code_keys_kernel(const void* codes, int codes64, int P, unsigned K,
-                                                            unsigned* __restrict__ keys,
-                                                            unsigned* __restrict__ ids) {
-  const int p = blockIdx.x * THREADS + threadIdx.x;
-  if (p >= P) return;
-  const long long c = read_code(codes, codes64, p);
-  keys[p] = c >= 0 && c < (long long)K ? (unsigned)c : K;
-  ids[p] = (unsigned)p;
+constexpr int SMALL_COLS = 128;  // columns a warp sums at a time, four per lane
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS) code_scan_kernel(const gsb_codebook_args a, int wpc) {
+  __shared__ float s_sum[THREADS / 32][SMALL_COLS];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int per_cta = THREADS / 32 / wpc, part = warp % wpc;
+  const long long code = (long long)blockIdx.x * per_cta + warp / wpc;
+  const int lo = (int)(a.P * part / wpc), hi = (int)(a.P * (part + 1) / wpc);
+  const int c0 = blockIdx.y * SMALL_COLS;
+  const T* grad = (const T*)a.grad_out;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f}, trow[4] = {0.f, 0.f, 0.f, 0.f};
+  if (code < a.K && a.grad_gain) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (c0 + lane + 32 * j < a.D) trow[j] = to_f(((const T*)a.table)[code * a.D + c0 + lane + 32 * j]);
+  }
+  for (int p0 = lo; p0 < hi && code <= a.K; p0 += 32 * 4) {
+    // four codes per lane at a time: the loads are in flight together
+    long long c[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int p = p0 + 32 * u + lane;
+      c[u] = p < hi ? read_code(a.codes, a.codes64, p) : -2;
+      if (p < hi && (c[u] < 0 || c[u] >= a.K)) c[u] = a.K;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      unsigned hit = __ballot_sync(0xffffffffu, c[u] == code);
+      if (code == a.K) {
+        if (a.grad_gain && blockIdx.y == 0 && c[u] == code) a.grad_gain[p0 + 32 * u + lane] = 0.f;
+        continue;
+      }
+      while (hit) {
+        // two rows in flight
+        const int i0 = __ffs(hit) - 1;
+        hit &= hit - 1;
+        const int i1 = hit ? __ffs(hit) - 1 : -1;
+        if (i1 >= 0) hit &= hit - 1;
+        const int r0 = p0 + 32 * u + i0, r1 = p0 + 32 * u + (i1 < 0 ? i0 : i1);
+        float v0[4], v1[4], dot0 = 0.f, dot1 = 0.f;
+        const float g0 = a.gain ? a.scale * a.gain[r0] : a.scale;
+        const float g1 = i1 < 0 ? 0.f : a.gain ? a.scale * a.gain[r1] : a.scale;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int col = c0 + lane + 32 * j;
+          v0[j] = col < a.D ? to_f(grad[(long long)r0 * a.D + col]) : 0.f;
+          v1[j] = col < a.D && i1 >= 0 ? to_f(grad[(long long)r1 * a.D + col]) : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          acc[j] += g0 * v0[j];
+          acc[j] += g1 * v1[j];
+          dot0 += v0[j] * trow[j];
+          dot1 += v1[j] * trow[j];
+        }
+        if (a.grad_gain) {
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) {
+            dot0 += __shfl_xor_sync(0xffffffffu, dot0, o);
+            dot1 += __shfl_xor_sync(0xffffffffu, dot1, o);
+          }
+          if (lane == 0) {
+            a.grad_gain[r0] = a.scale * dot0;
+            if (i1 >= 0) a.grad_gain[r1] = a.scale * dot1;
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) s_sum[warp][lane + 32 * j] = acc[j];
+  __syncthreads();
+  if (part != 0 || code >= a.K || !a.grad_table) return;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int col = c0 + lane + 32 * j;
+    if (col >= a.D) continue;
+    float sum = s_sum[warp][lane + 32 * j];
+    for (int w = 1; w < wpc; ++w) sum += s_sum[warp + w][lane + 32 * j];
+    ((T*)a.grad_table)[code * a.D + col] = from_f<T>(sum);
+  }
 }
 
 // ---------------------------------------------------------------------------
-// Backward, step 2: sums of runs of equal keys.  A group of `1 << gshift`
-// lanes covers a row (or a column block of it, blockIdx.y) in NV pieces of VW
-// elements per lane and owns `len` consecutive sorted positions.
-//   level 0: position i is the row ids[i] of grad_out, times its factor;
-//   above:   position i is row i of the fp32 partial sums below.
-// Partial rows of a chunk: 2c is the run that enters from the left, 2c + 1
-// the one that leaves to the right; a run that does both is (sum, zero) with
-// both keys set, so equal keys stay neighbours.
+// Backward of many rows, step 1: sort keys, the histograms of their digits,
+// and a zero gradient (codes that no row has keep it).  Rows without a code
+// take some key and are marked in their id, so that K codes need no more key
+// bits.
 // ---------------------------------------------------------------------------
+constexpr unsigned SKIP = 1u << 31;
+
+__global__ void __launch_bounds__(THREADS) code_keys_kernel(const void* codes, int codes64, int P, unsigned K,
+                                                            int passes, unsigned last_mask,
+                                                            unsigned* __restrict__ keys, unsigned* __restrict__ ids,
+                                                            unsigned* __restrict__ hist, uint4* __restrict__ zero,
+                                                            long long zero_vecs, uint8_t* __restrict__ zero_tail,
+                                                            int zero_bytes) {
+  __shared__ unsigned s_hist[radix::MAX_PASSES][radix::RADIX];
+  for (int i = threadIdx.x; i < passes * radix::RADIX; i += THREADS) (&s_hist[0][0])[i] = 0u;
+  __syncthreads();
+  const int stride = gridDim.x * THREADS, first = blockIdx.x * THREADS + threadIdx.x;
+  for (long long i = first; i < zero_vecs; i += stride) zero[i] = make_uint4(0u, 0u, 0u, 0u);
+  if (first < zero_bytes) zero_tail[first] = 0;
+  for (long long p = first; p < P; p += stride) {
+    const long long c = read_code(codes, codes64, p);
+    const bool ok = c >= 0 && c < (long long)K;
+    // rows without a code are spread over the keys: one long run would be summed for nothing
+    const unsigned key = ok ? (unsigned)c : (unsigned)p % K;
+    keys[p] = key;
+    ids[p] = ok ? (unsigned)p : (unsigned)p | SKIP;
+    for (int q = 0; q < passes; ++q)
+      atomicAdd(&s_hist[q][(key >> (q * radix::RADIX_BITS)) & (q == passes - 1 ? last_mask : radix::RADIX - 1)], 1u);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < passes * radix::RADIX; i += THREADS) {
+    const unsigned c = (&s_hist[0][0])[i];
+    if (c) atomicAdd(&hist[i], c);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Step 2: sums of runs of equal keys.  A group of `1 << gshift` lanes covers a
+// row (or a column block of it, blockIdx.y) in NV pieces of VW elements per
+// lane and owns `len` consecutive sorted positions.  The run that enters a
+// chunk from the left leaves its partial row at 2c, the one that leaves to the
+// right at 2c + 1 (a run that does both: its sum at 2c, both keys set).
+// ---------------------------------------------------------------------------
+constexpr unsigned NONE = 0xffffffffu;
+
 struct SegArgs {
   const unsigned* keys;
-  const unsigned* ids;     // level 0
-  const void* rows;        // grad_out (level 0) or fp32 partial rows
-  const float* gain;       // level 0, optional
+  const unsigned* ids;
+  const void* rows;        // grad_out
+  const float* gain;       // optional
   float scale;
   const void* table;       // with grad_gain
-  float* grad_gain;        // level 0, optional
+  float* grad_gain;        // optional
   void* grad_table;
-  unsigned* out_keys;      // 2 per chunk
-  float* out_rows;         // 2 per chunk, D floats each
+  unsigned* part_keys;     // 2 per chunk
+  float* part_rows;        // 2 per chunk, D floats each
   int n, len, chunks, D, gshift;
-  unsigned K;
 };
 
-template <typename T, typename R, int VW, int NV, bool LEVEL0, bool DGAIN>
+template <typename T, int VW, int NV, bool DGAIN>
 __global__ void __launch_bounds__(THREADS) segment_sum_kernel(const SegArgs a) {
   const int G = 1 << a.gshift;
   const int lane = threadIdx.x & (G - 1);
@@ -197,12 +318,11 @@ __global__ void __launch_bounds__(THREADS) segment_sum_kernel(const SegArgs a) {
   const bool live = chunk < a.chunks;
   const long long start = live ? chunk * a.len : 0;
   const long long end = live ? min(start + (long long)a.len, (long long)a.n) : 0;
-  const R* rows = (const R*)a.rows;
+  const T* rows = (const T*)a.rows;
   const T* table = (const T*)a.table;
   T* grad_table = (T*)a.grad_table;
-  const unsigned K = a.K;
-  const unsigned before = live && start > 0 ? a.keys[start - 1] : K;
-  const unsigned after = live && end < a.n ? a.keys[end] : K;
+  const unsigned before = live && start > 0 ? a.keys[start - 1] : NONE;
+  const unsigned after = live && end < a.n ? a.keys[end] : NONE;
 
   int col[NV];
 #pragma unroll
@@ -215,75 +335,66 @@ __global__ void __launch_bounds__(THREADS) segment_sum_kernel(const SegArgs a) {
   for (int j = 0; j < NV; ++j)
 #pragma unroll
     for (int i = 0; i < VW; ++i) acc[j][i] = trow[j][i] = 0.f;
-  unsigned cur = K;
+  unsigned cur = NONE;
   bool first_run = true;  // the run that began at `start`
-  unsigned left_key = K, right_key = K;
+  unsigned left_key = NONE, right_key = NONE;
 
-  auto put_partial = [&](int side, bool zero) {
-    float* dst = a.out_rows + (2 * chunk + side) * a.D;
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (col[j] >= 0) {
-        float v[VW];
-#pragma unroll
-        for (int i = 0; i < VW; ++i) v[i] = zero ? 0.f : acc[j][i];
-#pragma unroll
-        for (int i = 0; i < VW; ++i) dst[col[j] + i] = v[i];
-      }
-  };
   auto flush = [&](bool at_end) {
-    if (cur == K) return;
-    const bool from_left = first_run && before == cur;
-    const bool to_right = at_end && after == cur;
-    if (from_left) {
-      put_partial(0, false);
-      left_key = cur;
-      if (to_right) {
-        put_partial(1, true);
-        right_key = cur;
-      }
-    } else if (to_right) {
-      put_partial(1, false);
-      right_key = cur;
+    if (cur == NONE) return;
+    const bool from_left = first_run && before == cur, to_right = at_end && after == cur;
+    if (from_left) left_key = cur;
+    if (to_right) right_key = cur;
+    if (from_left || to_right) {
+      float* dst = a.part_rows + (2 * chunk + (from_left ? 0 : 1)) * a.D;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (col[j] >= 0) {
+#pragma unroll
+          for (int i = 0; i < VW; ++i) dst[col[j] + i] = acc[j][i];
+        }
     } else {
 #pragma unroll
       for (int j = 0; j < NV; ++j)
         if (col[j] >= 0) store_vec<T, VW>(grad_table + (long long)cur * a.D + col[j], acc[j]);
     }
   };
-
+  // keys and ids are read one round ahead of the rows that they name
+  unsigned next_key[SEG_UNROLL], next_id[SEG_UNROLL];
+  auto fetch = [&](long long pos) {
+#pragma unroll
+    for (int u = 0; u < SEG_UNROLL; ++u) {
+      next_key[u] = pos + u < end ? a.keys[pos + u] : NONE;
+      next_id[u] = pos + u < end ? a.ids[pos + u] : SKIP;
+    }
+  };
+  fetch(start);
   for (int off = 0; off < a.len; off += SEG_UNROLL) {
     unsigned key[SEG_UNROLL], id[SEG_UNROLL];
     float s[SEG_UNROLL], v[SEG_UNROLL][NV][VW];
 #pragma unroll
     for (int u = 0; u < SEG_UNROLL; ++u) {
-      const long long pos = start + off + u;
-      key[u] = pos < end ? a.keys[pos] : K;
-      id[u] = LEVEL0 ? (pos < end ? a.ids[pos] : 0u) : (unsigned)pos;
-    }
-#pragma unroll
-    for (int u = 0; u < SEG_UNROLL; ++u) {
-      s[u] = 1.f;
-      if (LEVEL0) s[u] = a.gain && key[u] != K ? a.scale * a.gain[id[u]] : a.scale;
+      key[u] = next_key[u];
+      id[u] = next_id[u];
+      s[u] = a.gain && !(id[u] & SKIP) ? a.scale * a.gain[id[u]] : a.scale;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
 #pragma unroll
         for (int i = 0; i < VW; ++i) v[u][j][i] = 0.f;
-        if (key[u] != K && col[j] >= 0) load_vec<R, VW>(rows + (long long)id[u] * a.D + col[j], v[u][j]);
+        if (!(id[u] & SKIP) && col[j] >= 0) load_vec<T, VW>(rows + (long long)id[u] * a.D + col[j], v[u][j]);
       }
     }
+    if (off + SEG_UNROLL < a.len) fetch(start + off + SEG_UNROLL);
 #pragma unroll
     for (int u = 0; u < SEG_UNROLL; ++u) {
-      const bool valid = start + off + u < end;
-      if (valid && key[u] != cur) {
+      if (key[u] != NONE && key[u] != cur) {
         flush(false);
         if (off + u > 0) first_run = false;
         cur = key[u];
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
 #pragma unroll
-          for (int i = 0; i < VW; ++i) acc[j][i] = trow[j][i] = 0.f;
-          if (DGAIN && cur != K && col[j] >= 0) load_vec<T, VW>(table + (long long)cur * a.D + col[j], trow[j]);
+          for (int i = 0; i < VW; ++i) acc[j][i] = 0.f;
+          if (DGAIN && col[j] >= 0) load_vec<T, VW>(table + (long long)cur * a.D + col[j], trow[j]);
         }
       }
       if (DGAIN) {
@@ -294,7 +405,7 @@ __global__ void __launch_bounds__(THREADS) segment_sum_kernel(const SegArgs a) {
           for (int i = 0; i < VW; ++i) dot += v[u][j][i] * trow[j][i];
         __syncwarp();
         for (int o = G >> 1; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-        if (valid && lane == 0) a.grad_gain[id[u]] = key[u] != K ? a.scale * dot : 0.f;
+        if (key[u] != NONE && lane == 0) a.grad_gain[id[u] & ~SKIP] = id[u] & SKIP ? 0.f : a.scale * dot;
       }
 #pragma unroll
       for (int j = 0; j < NV; ++j)
@@ -303,9 +414,79 @@ __global__ void __launch_bounds__(THREADS) segment_sum_kernel(const SegArgs a) {
     }
   }
   flush(true);
-  if (live && a.out_keys && lane == 0 && blockIdx.y == 0) {
-    a.out_keys[2 * chunk] = left_key;
-    a.out_keys[2 * chunk + 1] = right_key;
+  if (live && a.chunks > 1 && lane == 0 && blockIdx.y == 0) {
+    a.part_keys[2 * chunk] = left_key;
+    a.part_keys[2 * chunk + 1] = right_key;
+  }
+}
+
+// Step 3: the runs that cross chunks.  A warp looks at one chunk; if a run
+// starts there and leaves to the right, it adds up that run's partial rows.
+// Runs of more than LONG_RUN chunks are left to the whole CTA, whose warps
+// take every eighth partial row.
+constexpr int LONG_RUN = 32;
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS) run_join_kernel(const SegArgs a) {
+  constexpr int WARPS = THREADS / 32;
+  __shared__ int s_last[WARPS];
+  __shared__ float s_sum[WARPS][128];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int first = blockIdx.x * WARPS;
+  const int mine = first + warp;
+  int last = -1;  // the run's last chunk
+  if (mine < a.chunks) {
+    const unsigned key = a.part_keys[2 * mine + 1];
+    if (key != NONE && a.part_keys[2 * mine] != key) {
+      for (int c = mine + 1;; c += 32) {
+        const unsigned stop = __ballot_sync(0xffffffffu, c + lane >= a.chunks || a.part_keys[2 * (c + lane) + 1] != key);
+        if (stop) {
+          last = c + __ffs(stop) - 1;
+          break;
+        }
+      }
+    }
+  }
+  // rows of the run in chunk order: 2 * start + 1, 2 * (start + 1), 2 * (start + 2), ...
+  auto sum_rows = [&](int start, int end, int c, int from, int step) {
+    float sum = 0.f;
+    if (c < a.D) {
+      for (int k = start + from; k <= end; k += 4 * step) {
+        float v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const long long r = (long long)k + u * step;
+          v[u] = r <= end ? a.part_rows[(2 * r + (r == start ? 1 : 0)) * a.D + c] : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) sum += v[u];
+      }
+    }
+    return sum;
+  };
+  const bool is_long = last - mine > LONG_RUN && last >= 0;
+  if (last >= 0 && !is_long) {
+    T* dst = (T*)a.grad_table + (long long)a.part_keys[2 * mine + 1] * a.D;
+    for (int c = lane; c < a.D; c += 32) dst[c] = from_f<T>(sum_rows(mine, last, c, 0, 1));
+  }
+  if (lane == 0) s_last[warp] = is_long ? last : -1;
+  __syncthreads();
+  for (int w = 0; w < WARPS; ++w) {
+    const int end = s_last[w];
+    if (end < 0) continue;
+    T* dst = (T*)a.grad_table + (long long)a.part_keys[2 * (first + w) + 1] * a.D;
+    for (int c0 = 0; c0 < a.D; c0 += 128) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s_sum[warp][lane + 32 * j] = sum_rows(first + w, end, c0 + lane + 32 * j, warp, WARPS);
+      __syncthreads();
+      const int c = threadIdx.x;
+      if (c < 128 && c0 + c < a.D) {
+        float sum = 0.f;
+        for (int k = 0; k < WARPS; ++k) sum += s_sum[k][c];
+        dst[c0 + c] = from_f<T>(sum);
+      }
+      __syncthreads();
+    }
   }
 }
 
@@ -330,18 +511,23 @@ __global__ void __launch_bounds__(THREADS) gain_dot_kernel(const gsb_codebook_ar
 // ---------------------------------------------------------------------------
 // Host side.
 // ---------------------------------------------------------------------------
-// Chunk length of level 0: long chunks leave few partial rows to write and
-// read again, short ones keep enough groups in flight when there are few rows.
-inline int level0_len(long long P) { return P >= (1 << 20) ? 128 : 32; }
-constexpr int UPPER_LEN = 32;
+// Chunk length: long chunks leave few partial rows to write and read again,
+// short ones keep enough groups in flight when there are few rows.
+inline int chunk_len(long long P) { return P >= (1 << 20) ? 128 : P >= (1 << 17) ? 32 : 16; }
 
 inline long long chunks_of(long long n, int len) { return (n + len - 1) / len; }
 
-inline int bits_for(long long max_key) {
+// Bits of the keys 0 .. K - 1.
+inline int key_bits(long long K) {
   int b = 1;
-  while ((max_key >> b) != 0) ++b;
+  while (((K - 1) >> b) > 0) ++b;
   return b;
 }
+
+// Warps per code of the scan, and when it is taken: it reads every code K / 8 *
+// wpc times (from L2), so it stops paying once that is tens of microseconds.
+inline int scan_warps(long long P) { return P > 4096 ? 8 : P > 2048 ? 4 : P > 1024 ? 2 : 1; }
+inline bool small_case(long long P, long long K) { return P <= (1 << 15) && P * K <= (1 << 23); }
 
 struct Shape {
   int vw, nv, gshift, col_blocks;
@@ -364,15 +550,15 @@ inline Shape pick_shape(int D, int vw) {
   return best;
 }
 
-template <typename T, typename R, int VW, bool LEVEL0, bool DGAIN>
+template <typename T, int VW, bool DGAIN>
 void launch_seg(const SegArgs& a, const Shape& sh, cudaStream_t s) {
   const long long threads = (long long)a.chunks << sh.gshift;
   const dim3 grid((unsigned)((threads + THREADS - 1) / THREADS), sh.col_blocks);
   switch (sh.nv) {
-    case 1: segment_sum_kernel<T, R, VW, 1, LEVEL0, DGAIN><<<grid, THREADS, 0, s>>>(a); break;
-    case 2: segment_sum_kernel<T, R, VW, 2, LEVEL0, DGAIN><<<grid, THREADS, 0, s>>>(a); break;
-    case 3: segment_sum_kernel<T, R, VW, 3, LEVEL0, DGAIN><<<grid, THREADS, 0, s>>>(a); break;
-    default: segment_sum_kernel<T, R, VW, 4, LEVEL0, DGAIN><<<grid, THREADS, 0, s>>>(a); break;
+    case 1: segment_sum_kernel<T, VW, 1, DGAIN><<<grid, THREADS, 0, s>>>(a); break;
+    case 2: segment_sum_kernel<T, VW, 2, DGAIN><<<grid, THREADS, 0, s>>>(a); break;
+    case 3: segment_sum_kernel<T, VW, 3, DGAIN><<<grid, THREADS, 0, s>>>(a); break;
+    default: segment_sum_kernel<T, VW, 4, DGAIN><<<grid, THREADS, 0, s>>>(a); break;
   }
 }
 
@@ -380,13 +566,17 @@ struct Workspace {
   unsigned* keys[2];
   unsigned* ids[2];
   void* sort;
-  unsigned* part_keys[2];
-  float* part_rows[2];
+  unsigned* part_keys;
+  float* part_rows;
   size_t bytes;
 };
 
 inline Workspace carve(void* base, long long P, long long K, int D) {
-  Workspace w;
+  Workspace w{};
+  if (small_case(P, K) || K == 0) {
+    w.bytes = 0;
+    return w;
+  }
   char* p = (char*)(((uintptr_t)base + 255) & ~(uintptr_t)255);
   char* start = p;
   auto take = [&](size_t b) {
@@ -396,13 +586,10 @@ inline Workspace carve(void* base, long long P, long long K, int D) {
   };
   for (int i = 0; i < 2; ++i) w.keys[i] = (unsigned*)take((size_t)P * 4);
   for (int i = 0; i < 2; ++i) w.ids[i] = (unsigned*)take((size_t)P * 4);
-  w.sort = take(radix::scratch_bytes(P, radix::passes_for_bits(bits_for(K))));
-  long long n = 2 * chunks_of(P, level0_len(P));
-  for (int i = 0; i < 2; ++i) {
-    w.part_keys[i] = (unsigned*)take((size_t)n * 4);
-    w.part_rows[i] = (float*)take((size_t)n * D * 4);
-    n = 2 * chunks_of(n, UPPER_LEN);
-  }
+  w.sort = take(radix::scratch_bytes(P, radix::passes_for_bits(key_bits(K))));
+  const long long n = 2 * chunks_of(P, chunk_len(P));
+  w.part_keys = (unsigned*)take((size_t)n * 4);
+  w.part_rows = (float*)take((size_t)n * D * 4);
   w.bytes = (size_t)(p - start) + 256;
   return w;
 }
@@ -410,22 +597,42 @@ inline Workspace carve(void* base, long long P, long long K, int D) {
 template <typename T>
 int run_bwd(const gsb_codebook_args* a, cudaStream_t s) {
   constexpr int VW = Vec16<T>::N;
-  const long long P = a->P;
+  const long long P = a->P, K = a->K;
+  if (P == 0) {
+    if (a->grad_table) cudaMemsetAsync(a->grad_table, 0, (size_t)K * a->D * sizeof(T), s);
+    return check_launch("gsb_codebook_bwd");
+  }
   const bool aligned = (long long)a->D * sizeof(T) % 16 == 0 && (uintptr_t)a->grad_out % 16 == 0 &&
                        (uintptr_t)a->table % 16 == 0 && (uintptr_t)a->grad_table % 16 == 0;
   const Shape sh = pick_shape(a->D, aligned ? VW : 1);
-  const bool fused_gain = a->grad_gain && a->grad_table && sh.col_blocks == 1;
-  if (a->grad_gain && !fused_gain && P > 0)
+  const bool scan = a->grad_table && K > 0 && small_case(P, K);
+  const bool fused_gain = a->grad_gain && a->grad_table && K > 0 && (scan ? a->D <= SMALL_COLS : sh.col_blocks == 1);
+  if (a->grad_gain && !fused_gain)
     gain_dot_kernel<T><<<div_up(P * 32, THREADS), THREADS, 0, s>>>(*a);
-  if (!a->grad_table) return check_launch("gsb_codebook_bwd");
-  cudaMemsetAsync(a->grad_table, 0, (size_t)a->K * a->D * sizeof(T), s);
-  if (P == 0) return check_launch("gsb_codebook_bwd");
+  if (!a->grad_table || K == 0) return check_launch("gsb_codebook_bwd");
+  if (scan) {
+    gsb_codebook_args b = *a;
+    if (!fused_gain) b.grad_gain = nullptr;
+    const int wpc = scan_warps(P), per_cta = THREADS / 32 / wpc;
+    code_scan_kernel<T><<<dim3(div_up(K + 1, per_cta), div_up(a->D, SMALL_COLS)), THREADS, 0, s>>>(b, wpc);
+    return check_launch("gsb_codebook_bwd");
+  }
 
-  Workspace w = carve(a->workspace, P, a->K, a->D);
-  code_keys_kernel<<<div_up(P, THREADS), THREADS, 0, s>>>(a->codes, a->codes64, (int)P, (unsigned)a->K, w.keys[0],
-                                                          w.ids[0]);
-  const int where = radix::sort_pairs(w.keys, w.ids, P, nullptr, bits_for(a->K), w.sort, a->error_word, s, nullptr,
-                                      0, true);
+  const Workspace w = carve(a->workspace, P, K, a->D);
+  const int bits = key_bits(K), passes = radix::passes_for_bits(bits);
+  const radix::SortScratch scratch = radix::carve_scratch(w.sort, P, passes);
+  cudaMemsetAsync(scratch.hist, 0, scratch.zero_bytes, s);
+  const size_t grad_bytes = (size_t)K * a->D * sizeof(T);
+  // 16-byte stores where the table's gradient is aligned, bytes at its end (or a fill of its own)
+  const bool fill = (uintptr_t)a->grad_table % 16 == 0;
+  if (!fill) cudaMemsetAsync(a->grad_table, 0, grad_bytes, s);
+  const long long vecs = fill ? (long long)(grad_bytes / 16) : 0;
+  const int tail = fill ? (int)(grad_bytes % 16) : 0;
+  code_keys_kernel<<<(int)std::min<long long>(148 * 8, (P + THREADS - 1) / THREADS), THREADS, 0, s>>>(
+      a->codes, a->codes64, (int)P, (unsigned)K, passes, (1u << (bits - radix::RADIX_BITS * (passes - 1))) - 1u,
+      w.keys[0], w.ids[0], scratch.hist, (uint4*)a->grad_table, vecs, (uint8_t*)a->grad_table + vecs * 16, tail);
+  unsigned *k[2] = {w.keys[0], w.keys[1]}, *v[2] = {w.ids[0], w.ids[1]};
+  const int where = radix::sort_passes(k, v, P, nullptr, bits, scratch, a->error_word, s, nullptr, 0, true);
   SegArgs g{};
   g.keys = w.keys[where];
   g.ids = w.ids[where];
@@ -435,48 +642,41 @@ int run_bwd(const gsb_codebook_args* a, cudaStream_t s) {
   g.table = a->table;
   g.grad_gain = fused_gain ? a->grad_gain : nullptr;
   g.grad_table = a->grad_table;
+  g.part_keys = w.part_keys;
+  g.part_rows = w.part_rows;
   g.n = (int)P;
-  g.len = level0_len(P);
+  g.len = chunk_len(P);
   g.chunks = (int)chunks_of(P, g.len);
   g.D = a->D;
   g.gshift = sh.gshift;
-  g.K = (unsigned)a->K;
-  for (int level = 0;; ++level) {
-    const bool more = g.chunks > 1;
-    g.out_keys = more ? w.part_keys[level & 1] : nullptr;
-    g.out_rows = more ? w.part_rows[level & 1] : nullptr;
-    if (level == 0) {
-      if (aligned) {
-        if (fused_gain) launch_seg<T, T, VW, true, true>(g, sh, s);
-        else launch_seg<T, T, VW, true, false>(g, sh, s);
-      } else {
-        if (fused_gain) launch_seg<T, T, 1, true, true>(g, sh, s);
-        else launch_seg<T, T, 1, true, false>(g, sh, s);
-      }
-    } else {
-      const Shape up = pick_shape(a->D, 1);
-      g.gshift = up.gshift;
-      launch_seg<T, float, 1, false, false>(g, up, s);
-    }
-    if (!more) break;
-    g.keys = g.out_keys;
-    g.rows = g.out_rows;
-    g.grad_gain = nullptr;
-    g.gain = nullptr;
-    g.n = 2 * g.chunks;
-    g.len = UPPER_LEN;
-    g.chunks = (int)chunks_of(g.n, g.len);
+  if (aligned) {
+    if (fused_gain) launch_seg<T, VW, true>(g, sh, s);
+    else launch_seg<T, VW, false>(g, sh, s);
+  } else {
+    if (fused_gain) launch_seg<T, 1, true>(g, sh, s);
+    else launch_seg<T, 1, false>(g, sh, s);
   }
+  if (g.chunks > 1) run_join_kernel<T><<<div_up(g.chunks, THREADS / 32), THREADS, 0, s>>>(g);
   return check_launch("gsb_codebook_bwd");
+}
+
+template <typename T, int ROWS>
+void launch_gather(const gsb_codebook_args* a, cudaStream_t s) {
+  const bool out_aligned = (uintptr_t)a->out % 16 == 0;
+  const bool aligned = out_aligned && (long long)a->D * sizeof(T) % 16 == 0 && (uintptr_t)a->table % 16 == 0;
+  const int blocks = div_up(a->P, ROWS);
+  if (aligned) codebook_gather_kernel<T, true, ROWS><<<blocks, THREADS, 0, s>>>(*a, 1);
+  else codebook_gather_kernel<T, false, ROWS><<<blocks, THREADS, 0, s>>>(*a, out_aligned);
 }
 
 template <typename T>
 int run_fwd(const gsb_codebook_args* a, cudaStream_t s) {
-  const bool out_aligned = (uintptr_t)a->out % 16 == 0;
-  const bool aligned = out_aligned && (long long)a->D * sizeof(T) % 16 == 0 && (uintptr_t)a->table % 16 == 0;
-  const int blocks = div_up(a->P, FWD_CTA_ROWS);
-  if (aligned) codebook_gather_kernel<T, true><<<blocks, THREADS, 0, s>>>(*a, 1);
-  else codebook_gather_kernel<T, false><<<blocks, THREADS, 0, s>>>(*a, out_aligned);
+  // Longer CTAs spend less of their time on reading codes; short rows or few
+  // of them need shorter ones to fill the SMs.  About 16 KB of output each.
+  const long long bytes = (long long)a->D * sizeof(T);
+  if (a->P >= 148 * 8 * 256 && bytes <= 128) launch_gather<T, 256>(a, s);
+  else if (a->P >= 148 * 8 * 128) launch_gather<T, 128>(a, s);
+  else launch_gather<T, 32>(a, s);
   return check_launch("gsb_codebook_fwd");
 }
 
@@ -521,7 +721,7 @@ GSB_EXPORT int gsb_codebook_fwd(const gsb_codebook_args* a, void* stream) {
 }
 
 GSB_EXPORT size_t gsb_codebook_bwd_workspace_bytes(long long P, long long K, int D) {
-  if (P <= 0 || P >= gsb::MAX_ROWS || K < 0 || D < 1) return 256;
+  if (P <= 0 || P >= gsb::MAX_ROWS || K < 0 || D < 1) return 0;
   return gsb::carve(nullptr, P, K, D).bytes;
 }
 
@@ -537,8 +737,8 @@ GSB_EXPORT int gsb_codebook_bwd(const gsb_codebook_args* a, void* stream) {
     set_error("gsb_codebook_bwd: grad_gain without gain");
     return GSB_ERR_INVALID;
   }
-  if (a->grad_table && a->P > 0 &&
-      (!a->workspace || a->workspace_bytes < gsb_codebook_bwd_workspace_bytes(a->P, a->K, a->D))) {
+  const size_t need = a->grad_table ? gsb_codebook_bwd_workspace_bytes(a->P, a->K, a->D) : 0;
+  if (need > 0 && (!a->workspace || a->workspace_bytes < need)) {
     set_error("gsb_codebook_bwd: workspace too small");
     return GSB_ERR_INVALID;
   }

@@ -363,22 +363,18 @@ __host__ inline void launch_pass(int tiles, cudaStream_t stream, const unsigned*
 // ignored).  Buffers ping-pong: pass 0 reads (k[0],v[0]) and writes
 // (k[1],v[1]), pass 1 the reverse, ...  Returns the index (0/1) of the
 // buffer pair that holds the sorted values; the last pass does not write
-// keys, so the sorted keys are not kept, unless keep_keys asks for them.  With n_dev non-null the count is read on
+// keys, so the sorted keys are not kept.  With n_dev non-null the count is read on
 // the device (at most n, which sizes the grids and the scratch).
 // With `ranges` (and n_dev null) the last pass also writes, for every key
 // value below range_keys, its [start, end) in the sorted output into the
 // zero-initialised int2 array `ranges` ((0, 0) for absent keys).
-__host__ inline int sort_pairs(unsigned* k[2], unsigned* v[2], long long n, const int* n_dev, int key_bits,
-                               void* scratch, long long* err, cudaStream_t stream, int* ranges = nullptr,
-                               int range_keys = 0, bool keep_keys = false) {
+// sort_passes runs the passes alone, over scratch that is cleared and holds the
+// digit histograms already, and with keep_keys writes the sorted keys too.
+__host__ inline int sort_passes(unsigned* k[2], unsigned* v[2], long long n, const int* n_dev, int key_bits,
+                                const SortScratch& s, long long* err, cudaStream_t stream, int* ranges,
+                                int range_keys, bool keep_keys) {
   const int passes = passes_for_bits(key_bits);
-  if ((n <= 1 && !n_dev) || n <= 0 || passes == 0) return 0;
   const int last_bits = key_bits - RADIX_BITS * (passes - 1);
-  SortScratch s = carve_scratch(scratch, n, passes);
-  cudaMemsetAsync(s.hist, 0, s.zero_bytes, stream);
-  const int hist_blocks = (int)std::min<long long>(148 * 4, (n + THREADS * 8 - 1) / (THREADS * 8));
-  histogram_kernel<<<std::max(hist_blocks, 1), THREADS, 0, stream>>>(k[0], (int)n, n_dev, passes,
-                                                                      (1u << last_bits) - 1u, s.hist);
   bin_base_kernel<<<passes, THREADS, 0, stream>>>(s.hist, s.bin_base);
   const int tiles = num_tiles(n);
   int cur = 0;
@@ -407,6 +403,20 @@ __host__ inline int sort_pairs(unsigned* k[2], unsigned* v[2], long long n, cons
   if (ranges && !n_dev && range_keys > 0)
     ranges_fixup_kernel<<<(range_keys + 255) / 256, 256, 0, stream>>>(range_keys, (int)n, ranges);
   return cur;
+}
+
+__host__ inline int sort_pairs(unsigned* k[2], unsigned* v[2], long long n, const int* n_dev, int key_bits,
+                               void* scratch, long long* err, cudaStream_t stream, int* ranges = nullptr,
+                               int range_keys = 0) {
+  const int passes = passes_for_bits(key_bits);
+  if ((n <= 1 && !n_dev) || n <= 0 || passes == 0) return 0;
+  const int last_bits = key_bits - RADIX_BITS * (passes - 1);
+  SortScratch s = carve_scratch(scratch, n, passes);
+  cudaMemsetAsync(s.hist, 0, s.zero_bytes, stream);
+  const int hist_blocks = (int)std::min<long long>(148 * 4, (n + THREADS * 8 - 1) / (THREADS * 8));
+  histogram_kernel<<<std::max(hist_blocks, 1), THREADS, 0, stream>>>(k[0], (int)n, n_dev, passes,
+                                                                      (1u << last_bits) - 1u, s.hist);
+  return sort_passes(k, v, n, n_dev, key_bits, s, err, stream, ranges, range_keys, false);
 }
 
 }  // namespace

@@ -73,15 +73,16 @@ def test_c_abi_refuses_missing_buffers():
     assert L.gsb_codebook_bwd(ctypes.byref(_args(**full)), None) == _lib.GSB_ERR_INVALID  # no grad_out
     full["grad_out"] = p
     assert L.gsb_codebook_bwd(ctypes.byref(_args(grad_gain=p, **full)), None) == _lib.GSB_ERR_INVALID  # no gain
-    need = L.gsb_codebook_bwd_workspace_bytes(10, 4, 3)
-    short = _args(grad_table=p, workspace=p, workspace_bytes=need - 1, **full)
+    need = L.gsb_codebook_bwd_workspace_bytes(100_000, 400, 3)
+    assert need > 0
+    short = _args(P=100_000, K=400, grad_table=p, workspace=p, workspace_bytes=need - 1, **full)
     assert L.gsb_codebook_bwd(ctypes.byref(short), None) == _lib.GSB_ERR_INVALID
     assert L.gsb_codebook_fwd(None, None) == _lib.GSB_ERR_INVALID
 
 
 def test_workspace_grows_with_the_rows_and_their_width():
     ws = _lib.load().gsb_codebook_bwd_workspace_bytes
-    assert ws(0, 4, 3) > 0
+    assert ws(0, 4, 3) == 0 and ws(10_000, 256, 3) == 0  # few rows need none
     assert ws(1_000_000, 4096, 45) >= 16 * 1_000_000
     assert ws(2_000_000, 4096, 45) > ws(1_000_000, 4096, 45)
     assert ws(1_000_000, 4096, 96) > ws(1_000_000, 4096, 45)
