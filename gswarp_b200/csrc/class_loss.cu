@@ -250,6 +250,7 @@ struct StreamArgs {
   int a_slots, stages, acc_slots;
   int slots;               // partial results a unit leaves: its groups that had a tile
   int flush;               // tiles per accumulator
+  int wide, accs;          // second product: planes of B side by side; column groups of an accumulator
   float* part_m;           // FWD: [split][slot][row]
   float* part_s;
   float* t_label;          // FWD: [row]
@@ -279,9 +280,16 @@ __host__ __device__ constexpr int z_columns(int np, int tn) {
 // additions).  Accumulators are therefore taken out after a bounded number of
 // additions and added up with rounding.  fp32 features: 16 additions of the
 // leading planes' product; the other five products, 2^-8 of it and less, have
-// an accumulator of their own, so that they do not lengthen the chain (5e-7).
-// fp16 (four products): 256 additions, 8e-6; bf16: 512, 1.5e-5; both far below
-// the half step of the gradients' type.
+// columns of their own, so that they do not lengthen the chain (5e-7).
+// fp16 (up to four products): 256 additions, 8e-6; bf16: 512, 1.5e-5; both far
+// below the half step of the gradients' type.
+//
+// A matrix instruction takes 45 cycles or more however few columns it has, so
+// few channels waste most of it.  Where tensor memory has room, one
+// instruction therefore multiplies a plane of P with all the planes of B that
+// it meets, side by side (B's planes are neighbours in the tile): columns
+// [h h | h m | h l], then [m h | m m] from the second group on, then [l h] in
+// the third: three instructions instead of six (fp16: two instead of four).
 __host__ __device__ constexpr int accumulators(int np) { return np == 3 ? 2 : 1; }
 __host__ __device__ constexpr int chain_products(int np) { return np == 3 ? 16 : np == 2 ? 64 : 512; }
 
@@ -395,7 +403,7 @@ __device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int units = g.a_tiles * g.splits;
   constexpr int SBUF = z_columns<MODE>(NP, TN);
-  constexpr int ACCS = accumulators(NP);
+  const int accs = g.accs;
   constexpr uint32_t ACC0 = GROUPS * SBUF;          // first accumulator column
 
   if (threadIdx.x == 0) {
@@ -517,18 +525,30 @@ __device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, 
            warp_wait(&bar->p_full[b], (c.t / GROUPS) & 1, stop);
       if (!ok) break;
       fence_after();
-      const uint32_t dst = tmem + ACC0 + c.acc.i * ACCS * D, p = tmem + b * SBUF;
+      const uint32_t dst = tmem + ACC0 + c.acc.i * accs * D, p = tmem + b * SBUF;
       const uint32_t b_lo = desc_lo(b0 + c.bs.i * b_bytes, NP * D8 * 128);
+      if (NP > 1 && g.wide) {
 #pragma unroll
-      for (int q = 0; q < plane_products(NP); ++q) {
-        const int pa = plane_of_a(NP, q);
-        const bool main = q + 1 == plane_products(NP);
-        const uint32_t to = ACCS == 2 && !main ? dst + D : dst;
-        const uint32_t bq = b_lo + plane_of_b(NP, q) * D8 * 8;
+        for (int pa = 0; pa < NP; ++pa) {
+          const uint32_t to = NP == 3 ? dst + pa * D : dst;
+          const uint32_t id = instr_desc(NP == 3 ? (3 - pa) * D : 2 * D, true);
 #pragma unroll
-        for (int k = 0; k < TN / 16; ++k)
-          mma_ts(leader, to, p + p_column(TN, 16 * k, pa), bq + k * step, hi, idesc,
-                 k > 0 || (q > 0 && !(ACCS == 2 && main)) || !first);
+          for (int k = 0; k < TN / 16; ++k)
+            mma_ts(leader, to, p + p_column(TN, 16 * k, pa), b_lo + k * step, hi, id,
+                   !first || k > 0 || pa > 0);
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < plane_products(NP); ++q) {
+          const int pa = plane_of_a(NP, q);
+          const bool main = q + 1 == plane_products(NP);
+          const uint32_t to = NP == 3 && !main ? dst + D : dst;
+          const uint32_t bq = b_lo + plane_of_b(NP, q) * D8 * 8;
+#pragma unroll
+          for (int k = 0; k < TN / 16; ++k)
+            mma_ts(leader, to, p + p_column(TN, 16 * k, pa), bq + k * step, hi, idesc,
+                   k > 0 || (q > 0 && !(NP == 3 && main)) || !first);
+        }
       }
       mma_commit(leader, &bar->b_empty[c.bs.i]);
       mma_commit(leader, &bar->s_free[b]);
@@ -720,7 +740,7 @@ __device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, 
         ok = warp_wait(&bar->acc_full[acc.i], acc.phase, stop);
         if (!ok) break;
         fence_after();
-        const uint32_t src = tmem + lanes + ACC0 + acc.i * ACCS * D;
+        const uint32_t src = tmem + lanes + ACC0 + acc.i * accs * D;
         if (!direct && !g.part_acc) {  // only the bias is wanted
           fence_before();
           __syncwarp();
@@ -735,17 +755,14 @@ __device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, 
 #pragma unroll
             for (int i = 0; i < 4; ++i) old[i] = at[i * TILE];
           }
-          uint32_t main[16];
+          // the smallest group first
+          uint32_t part[16];
           float v[16];
-          tmem_load(src + c, main);
-          tmem_load_wait(main);
+          for (int k = accs - 1; k >= 0; --k) {
+            tmem_load(src + k * D + c, part);
+            tmem_load_wait(part);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(main[i]);
-          if (ACCS == 2) {
-            tmem_load(src + D + c, main);
-            tmem_load_wait(main);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] += __uint_as_float(main[i]);
+            for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(part[i]) + (k == accs - 1 ? 0.f : v[i]);
           }
           if (c + 16 >= D) {
             fence_before();
@@ -786,10 +803,19 @@ __global__ void __launch_bounds__(stream_threads<FWD>(), 1) forward_kernel(const
   stream_pass<FWD, NP, TN>(g, smem, blockIdx.x, gridDim.x);
 }
 
-// Both gradients in one launch: dW's CTAs follow dX's without a gap.
+template <int MODE, int NP, int TN>
+__global__ void __launch_bounds__(stream_threads<MODE>(), 1) gradient_kernel(const StreamArgs g) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  stream_pass<MODE, NP, TN>(g, smem, blockIdx.x, gridDim.x);
+}
+
+// Both gradients in one launch, for calls whose CTAs have one unit each: dW's
+// CTAs then start on the SMs that dX leaves idle (8191 x 8200 x 65 fp32 313 ->
+// 269 us).  With more units the two kernels are faster apart (1080p, 256
+// classes, 16 channels: 708 us, together 785).
 template <int NP, int TN>
 __global__ void __launch_bounds__(stream_threads<DX>(), 1)
-    backward_kernel(const StreamArgs gx, const StreamArgs gw, const int x_ctas) {
+    gradients_kernel(const StreamArgs gx, const StreamArgs gw, const int x_ctas) {
   extern __shared__ __align__(1024) uint8_t smem[];
   if ((int)blockIdx.x < x_ctas) stream_pass<DX, NP, TN>(gx, smem, blockIdx.x, x_ctas);
   else stream_pass<DW, NP, TN>(gw, smem, blockIdx.x - x_ctas, gridDim.x - x_ctas);
@@ -1102,13 +1128,16 @@ size_t plan_pass(StreamArgs* g) {
   const size_t a_bytes = (size_t)NP * g->D8 * 2048;
   const size_t stage = (size_t)NP * g->D8 * TN * 16 + meta_floats<MODE>(TN) * 4;
   const size_t fixed = sizeof(Barriers) + 128;
-  constexpr int SBUF = z_columns<MODE>(NP, TN), ACCS = accumulators(NP);
+  constexpr int SBUF = z_columns<MODE>(NP, TN);
   static_assert(GROUPS * SBUF <= TMEM_COLUMNS, "z buffers");
+  const int D = g->D8 * 8;
+  g->wide = MODE != FWD && NP > 1 && NP * D <= 256 && GROUPS * SBUF + NP * D <= TMEM_COLUMNS;
+  g->accs = g->wide ? NP : accumulators(NP);
   g->flush = chain_products(NP) / (TN / 16);
   for (g->a_slots = MAX_A_SLOTS; g->a_slots > 1; --g->a_slots)
     if (g->a_slots * a_bytes + 6 * stage + fixed <= SMEM_MAX) break;
   g->stages = (int)std::min<size_t>(MAX_STAGES, (SMEM_MAX - fixed - g->a_slots * a_bytes) / stage);
-  const int acc = MODE == FWD ? 0 : ACCS * g->D8 * 8;
+  const int acc = MODE == FWD ? 0 : g->accs * D;
   g->acc_slots = GROUPS * SBUF + 2 * acc <= TMEM_COLUMNS ? 2 : 1;
   return std::max(SMEM_MIN, g->a_slots * a_bytes + g->stages * stage + fixed);
 }
@@ -1123,10 +1152,22 @@ int launch_forward(StreamArgs g, cudaStream_t s) {
 }
 template <int NP, int TN>
 int launch_backward(StreamArgs gx, StreamArgs gw, cudaStream_t s) {
-  const size_t smem = std::max(plan_pass<DX, NP, TN>(&gx), plan_pass<DW, NP, TN>(&gw));
-  cudaFuncSetAttribute(backward_kernel<NP, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  const int x_ctas = pass_ctas(gx);
-  backward_kernel<NP, TN><<<x_ctas + pass_ctas(gw), stream_threads<DX>(), smem, s>>>(gx, gw, x_ctas);
+  const size_t x_smem = plan_pass<DX, NP, TN>(&gx), w_smem = plan_pass<DW, NP, TN>(&gw);
+  const int x_units = gx.a_tiles * gx.splits, w_units = gw.a_tiles * gw.splits;
+  if (x_units && w_units && x_units <= SMS && w_units <= SMS) {
+    const size_t smem = std::max(x_smem, w_smem);
+    cudaFuncSetAttribute(gradients_kernel<NP, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    gradients_kernel<NP, TN><<<x_units + w_units, stream_threads<DX>(), smem, s>>>(gx, gw, x_units);
+    return check_launch("class loss backward");
+  }
+  if (x_units) {
+    cudaFuncSetAttribute(gradient_kernel<DX, NP, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)x_smem);
+    gradient_kernel<DX, NP, TN><<<pass_ctas(gx), stream_threads<DX>(), x_smem, s>>>(gx);
+  }
+  if (w_units) {
+    cudaFuncSetAttribute(gradient_kernel<DW, NP, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)w_smem);
+    gradient_kernel<DW, NP, TN><<<pass_ctas(gw), stream_threads<DW>(), w_smem, s>>>(gw);
+  }
   return check_launch("class loss backward");
 }
 
