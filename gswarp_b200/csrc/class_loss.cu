@@ -50,12 +50,32 @@ __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 
-__device__ __forceinline__ void store_elem(void* p, long long i, int dtype, float v) {
-  if (dtype == GSB_TYPE_FP32) ((float*)p)[i] = v;
-  else if (dtype == GSB_TYPE_BF16) ((__nv_bfloat16*)p)[i] = __float2bfloat16_rn(v);
-  else ((__half*)p)[i] = __float2half_rn(v);
-}
+template <typename T>
+__device__ __forceinline__ T from_float(float x);
+template <>
+__device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 
+// The features' type behind a number of planes.
+template <int NP>
+struct PlanesType;
+template <>
+struct PlanesType<1> {
+  using type = __nv_bfloat16;
+};
+template <>
+struct PlanesType<2> {
+  using type = __half;
+};
+template <>
+struct PlanesType<3> {
+  using type = float;
+};
+
+// What forward leaves for backward.
 struct Kept {
   uint4 *packed_x, *packed_w;
   float *class_bias2, *row_lse2;  // base 2; classes and rows rounded up to whole tiles
@@ -190,53 +210,42 @@ struct GradOut {
   const float* inv_count;  // null: upstream has one factor per row
   const int* y;            // rows without a gradient are zero (null: every row has one)
   long long rows, S;       // S > 0: n = b * S + s, written as (b, c, s); S = 0: (n, c)
-  int C, dtype;
+  int C;
 };
 __device__ __forceinline__ float grad_scale(const GradOut& o, long long n) {
-  if (o.y && o.y[n] < 0) return 0.f;
-  return o.inv_count ? o.upstream[0] * o.inv_count[0] : o.upstream ? o.upstream[n] : 1.f;
+  const int y = o.y ? o.y[n] : 0;  // loads side by side
+  const float u = o.inv_count ? o.upstream[0] * o.inv_count[0] : o.upstream ? o.upstream[n] : 1.f;
+  return y < 0 ? 0.f : u;
 }
 // Columns c .. c + COUNT - 1 of row n; u from grad_scale.
-template <int COUNT>
-__device__ __forceinline__ void write_grad(const GradOut& o, long long n, int c, const float (&v)[COUNT], float u) {
-  long long at, step = 1;
+template <typename T, int COUNT>
+__device__ __forceinline__ void write_grad(const GradOut& o, long long n, int c, float (&v)[COUNT], float u) {
+#pragma unroll
+  for (int i = 0; i < COUNT; ++i) v[i] = u == 0.f ? 0.f : v[i] * u;
   if (o.S > 0) {
     const unsigned b = (unsigned)n / (unsigned)o.S;
-    at = ((long long)b * o.C + c) * o.S + (n - b * o.S);
-    step = o.S;
+    T* at = (T*)o.out + ((long long)b * o.C + c) * o.S + (n - b * o.S);
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i)
+      if (c + i < o.C) at[i * o.S] = from_float<T>(v[i]);
   } else {
-    at = n * o.C + c;
-    const int size = o.dtype == GSB_TYPE_FP32 ? 4 : 2;
-    if (c + COUNT <= o.C && (at * size + (long long)(uintptr_t)o.out) % 16 == 0 && COUNT * size % 16 == 0) {
-      if (o.dtype == GSB_TYPE_FP32) {
+    T* at = (T*)o.out + n * o.C + c;
+    constexpr int PER = 16 / (int)sizeof(T);
+    if (COUNT % PER == 0 && c + COUNT <= o.C && (uintptr_t)at % 16 == 0) {
 #pragma unroll
-        for (int i = 0; i < COUNT / 4; ++i)
-          reinterpret_cast<float4*>((float*)o.out + at)[i] =
-              make_float4(u == 0.f ? 0.f : v[4 * i] * u, u == 0.f ? 0.f : v[4 * i + 1] * u,
-                          u == 0.f ? 0.f : v[4 * i + 2] * u, u == 0.f ? 0.f : v[4 * i + 3] * u);
-      } else {
-        uint32_t h[COUNT / 2];
+      for (int i = 0; i < COUNT / PER; ++i) {
+        uint4 raw;
+        T* e = reinterpret_cast<T*>(&raw);
 #pragma unroll
-        for (int i = 0; i < COUNT / 2; ++i) {
-          const float p = u == 0.f ? 0.f : v[2 * i] * u, q = u == 0.f ? 0.f : v[2 * i + 1] * u;
-          if (o.dtype == GSB_TYPE_BF16) {
-            const __nv_bfloat162 w = __floats2bfloat162_rn(p, q);
-            h[i] = *reinterpret_cast<const uint32_t*>(&w);
-          } else {
-            const __half2 w = __floats2half2_rn(p, q);
-            h[i] = *reinterpret_cast<const uint32_t*>(&w);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < COUNT / 8; ++i)
-          reinterpret_cast<uint4*>((uint16_t*)o.out + at)[i] = make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+        for (int k = 0; k < PER; ++k) e[k] = from_float<T>(v[i * PER + k]);
+        reinterpret_cast<uint4*>(at)[i] = raw;
       }
-      return;
+    } else {
+#pragma unroll
+      for (int i = 0; i < COUNT; ++i)
+        if (c + i < o.C) at[i] = from_float<T>(v[i]);
     }
   }
-#pragma unroll
-  for (int i = 0; i < COUNT; ++i)
-    if (c + i < o.C) store_elem(o.out, at + i * step, o.dtype, u == 0.f ? 0.f : v[i] * u);
 }
 
 struct StreamArgs {
@@ -250,7 +259,6 @@ struct StreamArgs {
   int a_slots, stages, acc_slots;
   int slots;               // partial results a unit leaves: its groups that had a tile
   int flush;               // tiles per accumulator
-  int wide, accs;          // second product: planes of B side by side; column groups of an accumulator
   float* part_m;           // FWD: [split][slot][row]
   float* part_s;
   float* t_label;          // FWD: [row]
@@ -281,15 +289,8 @@ __host__ __device__ constexpr int z_columns(int np, int tn) {
 // additions and added up with rounding.  fp32 features: 16 additions of the
 // leading planes' product; the other five products, 2^-8 of it and less, have
 // columns of their own, so that they do not lengthen the chain (5e-7).
-// fp16 (up to four products): 256 additions, 8e-6; bf16: 512, 1.5e-5; both far
+// fp16 (four products): 256 additions, 8e-6; bf16: 512, 1.5e-5; both far
 // below the half step of the gradients' type.
-//
-// A matrix instruction takes 45 cycles or more however few columns it has, so
-// few channels waste most of it.  Where tensor memory has room, one
-// instruction therefore multiplies a plane of P with all the planes of B that
-// it meets, side by side (B's planes are neighbours in the tile): columns
-// [h h | h m | h l], then [m h | m m] from the second group on, then [l h] in
-// the third: three instructions instead of six (fp16: two instead of four).
 __host__ __device__ constexpr int accumulators(int np) { return np == 3 ? 2 : 1; }
 __host__ __device__ constexpr int chain_products(int np) { return np == 3 ? 16 : np == 2 ? 64 : 512; }
 
@@ -347,6 +348,11 @@ struct Cursor {
   }
 };
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 // Packed pairs of fp32 (sm_100a issues both halves at once).
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
@@ -382,7 +388,7 @@ __device__ __forceinline__ void store_p(uint32_t buffer, int c, const float2 (&p
       h[i] = *reinterpret_cast<const uint32_t*>(&v);
       if (k + 1 < NP) {
         const float2 f = make_float2(__uint_as_float(h[i] << 16), __uint_as_float(h[i] & 0xffff0000u));
-        rest[i] = add2(rest[i], make_float2(-f.x, -f.y));
+        rest[i] = fma2(f, make_float2(-1.f, -1.f), rest[i]);  // exact
       }
     }
     tc::tmem_store(buffer + p_column(TN, c, k), h);
@@ -403,7 +409,7 @@ __device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int units = g.a_tiles * g.splits;
   constexpr int SBUF = z_columns<MODE>(NP, TN);
-  const int accs = g.accs;
+  constexpr int ACCS = accumulators(NP);
   constexpr uint32_t ACC0 = GROUPS * SBUF;          // first accumulator column
 
   if (threadIdx.x == 0) {
@@ -525,30 +531,18 @@ __device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, 
            warp_wait(&bar->p_full[b], (c.t / GROUPS) & 1, stop);
       if (!ok) break;
       fence_after();
-      const uint32_t dst = tmem + ACC0 + c.acc.i * accs * D, p = tmem + b * SBUF;
+      const uint32_t dst = tmem + ACC0 + c.acc.i * ACCS * D, p = tmem + b * SBUF;
       const uint32_t b_lo = desc_lo(b0 + c.bs.i * b_bytes, NP * D8 * 128);
-      if (NP > 1 && g.wide) {
 #pragma unroll
-        for (int pa = 0; pa < NP; ++pa) {
-          const uint32_t to = NP == 3 ? dst + pa * D : dst;
-          const uint32_t id = instr_desc(NP == 3 ? (3 - pa) * D : 2 * D, true);
+      for (int q = 0; q < plane_products(NP); ++q) {
+        const int pa = plane_of_a(NP, q);
+        const bool main = q + 1 == plane_products(NP);
+        const uint32_t to = NP == 3 && !main ? dst + D : dst;
+        const uint32_t bq = b_lo + plane_of_b(NP, q) * D8 * 8;
 #pragma unroll
-          for (int k = 0; k < TN / 16; ++k)
-            mma_ts(leader, to, p + p_column(TN, 16 * k, pa), b_lo + k * step, hi, id,
-                   !first || k > 0 || pa > 0);
-        }
-      } else {
-#pragma unroll
-        for (int q = 0; q < plane_products(NP); ++q) {
-          const int pa = plane_of_a(NP, q);
-          const bool main = q + 1 == plane_products(NP);
-          const uint32_t to = NP == 3 && !main ? dst + D : dst;
-          const uint32_t bq = b_lo + plane_of_b(NP, q) * D8 * 8;
-#pragma unroll
-          for (int k = 0; k < TN / 16; ++k)
-            mma_ts(leader, to, p + p_column(TN, 16 * k, pa), bq + k * step, hi, idesc,
-                   k > 0 || (q > 0 && !(NP == 3 && main)) || !first);
-        }
+        for (int k = 0; k < TN / 16; ++k)
+          mma_ts(leader, to, p + p_column(TN, 16 * k, pa), bq + k * step, hi, idesc,
+                 k > 0 || (q > 0 && !(NP == 3 && main)) || !first);
       }
       mma_commit(leader, &bar->b_empty[c.bs.i]);
       mma_commit(leader, &bar->s_free[b]);
@@ -564,7 +558,7 @@ __device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, 
     }
   } else if (warp < LOADER) {
     // ---- z -> row statistics, or P ----
-    constexpr int CH = MODE == FWD ? 32 : 16;  // columns in registers at a time
+    constexpr int CH = MODE != FWD && NP == 3 ? 16 : 32;  // columns in registers at a time
     const int group = warp / 4;
     const uint32_t buffer = tmem + lanes + group * SBUF;
     const int step = ctas;
@@ -598,11 +592,24 @@ __device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, 
         fence_after();
         const float* meta = sMeta + bs.i * META;
         const int col0 = bt * TN;
+        // whether a label of this warp's rows is among the tile's classes
+        bool labelled;
+        if (MODE == DW) {
+          const int* ym = reinterpret_cast<const int*>(meta + TN);
+          const unsigned wrow = row - lane;
+          labelled = false;
+#pragma unroll
+          for (int k = 0; k < TN / 32; ++k) labelled |= (unsigned)ym[32 * k + lane] - wrow < 32u;
+        } else {
+          labelled = y >= 0 && (unsigned)(y - col0) < (unsigned)TN;
+        }
+        labelled = __any_sync(0xffffffffu, labelled);
         uint32_t z[CH];
-        tmem_load(buffer, z);
         float2 tile_s[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        if (MODE == FWD) tmem_load(buffer, z);
 #pragma unroll 1
         for (int c = 0; c < TN; c += CH) {
+          if (MODE != FWD) tmem_load(buffer + c, z);  // four warps a scheduler hide it; registers are scarce
           tmem_load_wait(z);
           if (MODE == FWD && c + CH == TN) {
             fence_before();
@@ -611,15 +618,15 @@ __device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, 
           }
           // t of the columns: z log2(e) + bias, less the row's or the column's log-sum in the gradients
           float2 x[CH / 2];
-          const float2 l2e = make_float2(LOG2E, LOG2E), cst = make_float2(row_c, row_c);
+          const float2 l2e = make_float2(LOG2E, LOG2E), cst = make_float2(row_c, row_c), neg = make_float2(-1.f, -1.f);
 #pragma unroll
           for (int i = 0; i < CH / 2; i += 2) {
             const float4 w = *reinterpret_cast<const float4*>(meta + c + 2 * i);
             const float2 z0 = make_float2(__uint_as_float(z[2 * i]), __uint_as_float(z[2 * i + 1]));
             const float2 z1 = make_float2(__uint_as_float(z[2 * i + 2]), __uint_as_float(z[2 * i + 3]));
             if (MODE == DW) {
-              x[i] = add2(fma2(z0, l2e, cst), make_float2(-w.x, -w.y));
-              x[i + 1] = add2(fma2(z1, l2e, cst), make_float2(-w.z, -w.w));
+              x[i] = fma2(make_float2(w.x, w.y), neg, fma2(z0, l2e, cst));
+              x[i + 1] = fma2(make_float2(w.z, w.w), neg, fma2(z1, l2e, cst));
             } else {
               x[i] = fma2(z0, l2e, make_float2(w.x, w.y));
               x[i + 1] = fma2(z1, l2e, make_float2(w.z, w.w));
@@ -629,10 +636,10 @@ __device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, 
               }
             }
           }
-          if (c + CH < TN) tmem_load(buffer + c + CH, z);
+          if (MODE == FWD && c + CH < TN) tmem_load(buffer + c + CH, z);
           if (MODE == FWD) {
             const int rel = y - (col0 + c);
-            if (__any_sync(0xffffffffu, y >= 0 && rel >= 0 && rel < CH)) {
+            if (labelled) {
               float tl = 0.f;
 #pragma unroll
               for (int i = 0; i < CH / 2; ++i) {
@@ -641,10 +648,9 @@ __device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, 
               }
               if (y >= 0 && rel >= 0 && rel < CH) g.t_label[row] = tl;
             }
-            float cm[2] = {fmaxf(x[0].x, x[0].y), fmaxf(x[1].x, x[1].y)};
+            float top = x[0].x;
 #pragma unroll
-            for (int i = 2; i < CH / 2; ++i) cm[i & 1] = fmaxf(cm[i & 1], fmaxf(x[i].x, x[i].y));
-            const float top = fmaxf(cm[0], cm[1]);
+            for (int i = 0; i < CH / 2; ++i) top = max3(top, x[i].x, x[i].y);
             // The sums' base follows the maximum only when it is left behind by 2^8: fp32 has the range,
             // and the rescaling is rare.
             if (top > m + 8.f) {
@@ -666,38 +672,47 @@ __device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, 
           } else {
 #pragma unroll
             for (int i = 0; i < CH / 2; ++i) x[i] = make_float2(ex2(x[i].x), ex2(x[i].y));
-            if (MODE == DX) {
-              const int rel = y - (col0 + c);
-              if (__any_sync(0xffffffffu, y >= 0 && rel >= 0 && rel < CH)) {
+            if (labelled) {
+              if (MODE == DX) {
+                const int rel = y >= 0 ? y - (col0 + c) : -1;
 #pragma unroll
                 for (int i = 0; i < CH / 2; ++i) {
-                  if (y >= 0 && rel == 2 * i) x[i].x -= 1.f;
-                  if (y >= 0 && rel == 2 * i + 1) x[i].y -= 1.f;
+                  if (rel == 2 * i) x[i].x -= 1.f;
+                  if (rel == 2 * i + 1) x[i].y -= 1.f;
                 }
-              }
-            } else {
-              const int* ym = reinterpret_cast<const int*>(meta + TN) + c;
-              const int wrow = row - lane;
-              const int yl = ym[lane % CH];
-              if (__any_sync(0xffffffffu, yl >= wrow && yl < wrow + 32)) {
-#pragma unroll
-                for (int i = 0; i < CH / 2; ++i) {
-                  if (ym[2 * i] == row) x[i].x -= 1.f;
-                  if (ym[2 * i + 1] == row) x[i].y -= 1.f;
-                }
-              }
-              if (g.row_u) {
+              } else {
+                const int4* ym = reinterpret_cast<const int4*>(meta + TN + c);
 #pragma unroll
                 for (int i = 0; i < CH / 2; i += 2) {
-                  const float4 w = *reinterpret_cast<const float4*>(meta + 2 * TN + c + 2 * i);
-                  x[i] = make_float2(x[i].x * w.x, x[i].y * w.y);
-                  x[i + 1] = make_float2(x[i + 1].x * w.z, x[i + 1].y * w.w);
+                  const int4 l = ym[i / 2];
+                  if (l.x == row) x[i].x -= 1.f;
+                  if (l.y == row) x[i].y -= 1.f;
+                  if (l.z == row) x[i + 1].x -= 1.f;
+                  if (l.w == row) x[i + 1].y -= 1.f;
                 }
               }
+            }
+            if (MODE == DW && g.row_u) {
+#pragma unroll
+              for (int i = 0; i < CH / 2; i += 2) {
+                const float4 w = *reinterpret_cast<const float4*>(meta + 2 * TN + c + 2 * i);
+                x[i] = make_float2(x[i].x * w.x, x[i].y * w.y);
+                x[i + 1] = make_float2(x[i + 1].x * w.z, x[i + 1].y * w.w);
+              }
+            }
+            if (MODE == DW && g.part_bias) {
 #pragma unroll
               for (int i = 0; i < CH / 2; ++i) tile_s[i & 1] = add2(tile_s[i & 1], x[i]);
             }
-            if constexpr (MODE != FWD) store_p<NP, TN>(buffer, c, x);
+            if constexpr (MODE != FWD) {
+#pragma unroll
+              for (int h = 0; h < CH / 16; ++h) {
+                float2 half[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) half[i] = x[8 * h + i];
+                store_p<NP, TN>(buffer, c + 16 * h, half);
+              }
+            }
           }
         }
         if (MODE != FWD) {
@@ -720,7 +735,7 @@ __device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, 
           g.part_m[at] = m;
           g.part_s[at] = s;
         }
-        if (MODE == DW) g.part_bias[at] = bias_sum.x + bias_sum.y;
+        if (MODE == DW && g.part_bias) g.part_bias[at] = bias_sum.x + bias_sum.y;
       }
     }
   } else if (MODE != FWD) {
@@ -728,19 +743,27 @@ __device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, 
     // all of the streamed axis) straight into the gradient ----
     Ring acc;
     bool ok = true;
+    const int row = (warp & 3) * 32 + lane;
+    float scale_next = 0.f;
+    auto fetch = [&](int u) {  // the row's factor, one unit ahead: its loads would hold up every unit
+      if (u >= units || !g.grad.out) return;
+      const long long n = (long long)unit_range(g, u).tile * TILE + row;
+      scale_next = n < g.grad.rows ? grad_scale(g.grad, n) : 0.f;
+    };
+    fetch(cta);
     for (int u = cta; u < units && ok; u += ctas) {
       const Range r = unit_range(g, u);
       const size_t tile = (size_t)r.split * g.a_tiles + r.tile;
-      const int row = (warp & 3) * 32 + lane;
+      const float scale = scale_next;
+      fetch(u + ctas);
       const long long n = (long long)r.tile * TILE + row;
       float4* const dst = reinterpret_cast<float4*>(g.part_acc) + tile * (D / 4) * TILE + row;
       const bool direct = g.grad.out != nullptr, inside = direct && n < g.grad.rows;
-      const float scale = inside ? grad_scale(g.grad, n) : 0.f;
       for (int bt = r.lo; bt < r.hi; bt += g.flush) {
         ok = warp_wait(&bar->acc_full[acc.i], acc.phase, stop);
         if (!ok) break;
         fence_after();
-        const uint32_t src = tmem + lanes + ACC0 + acc.i * accs * D;
+        const uint32_t src = tmem + lanes + ACC0 + acc.i * ACCS * D;
         if (!direct && !g.part_acc) {  // only the bias is wanted
           fence_before();
           __syncwarp();
@@ -748,6 +771,7 @@ __device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, 
           acc.next(g.acc_slots);
           continue;
         }
+#pragma unroll 1
         for (int c = 0; c < D; c += 16) {
           float4* at = dst + (size_t)(c / 4) * TILE;
           float4 old[4];
@@ -758,11 +782,12 @@ __device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, 
           // the smallest group first
           uint32_t part[16];
           float v[16];
-          for (int k = accs - 1; k >= 0; --k) {
+#pragma unroll
+          for (int k = ACCS - 1; k >= 0; --k) {
             tmem_load(src + k * D + c, part);
             tmem_load_wait(part);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(part[i]) + (k == accs - 1 ? 0.f : v[i]);
+            for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(part[i]) + (k == ACCS - 1 ? 0.f : v[i]);
           }
           if (c + 16 >= D) {
             fence_before();
@@ -779,7 +804,7 @@ __device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, 
             }
           }
           if (direct && bt + g.flush >= r.hi) {
-            if (inside) write_grad(g.grad, n, c, v, scale);
+            if (inside) write_grad<typename PlanesType<NP>::type>(g.grad, n, c, v, scale);
           } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) at[i * TILE] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
@@ -940,6 +965,7 @@ struct Joins {
   Join x, w, bias;
 };
 
+template <typename T>
 __global__ void __launch_bounds__(THREADS) join_grads_kernel(const Joins j, int D) {
   __shared__ float4 s_part[8][32];
   const int lane = threadIdx.x % 32, sub = threadIdx.x / 32;
@@ -972,8 +998,8 @@ __global__ void __launch_bounds__(THREADS) join_grads_kernel(const Joins j, int 
   const long long strip = q / TILE;
   const long long n = strip / (D / 4) * TILE + q % TILE;
   if (n >= in.out.rows) return;
-  const float v[4] = {sum.x, sum.y, sum.z, sum.w};
-  write_grad(in.out, n, (int)(strip % (D / 4)) * 4, v, grad_scale(in.out, n));
+  float v[4] = {sum.x, sum.y, sum.z, sum.w};
+  write_grad<T>(in.out, n, (int)(strip % (D / 4)) * 4, v, grad_scale(in.out, n));
 }
 
 // ---------------------------------------------------------------------------
@@ -1130,14 +1156,12 @@ size_t plan_pass(StreamArgs* g) {
   const size_t fixed = sizeof(Barriers) + 128;
   constexpr int SBUF = z_columns<MODE>(NP, TN);
   static_assert(GROUPS * SBUF <= TMEM_COLUMNS, "z buffers");
-  const int D = g->D8 * 8;
-  g->wide = MODE != FWD && NP > 1 && NP * D <= 256 && GROUPS * SBUF + NP * D <= TMEM_COLUMNS;
-  g->accs = g->wide ? NP : accumulators(NP);
+
   g->flush = chain_products(NP) / (TN / 16);
   for (g->a_slots = MAX_A_SLOTS; g->a_slots > 1; --g->a_slots)
     if (g->a_slots * a_bytes + 6 * stage + fixed <= SMEM_MAX) break;
   g->stages = (int)std::min<size_t>(MAX_STAGES, (SMEM_MAX - fixed - g->a_slots * a_bytes) / stage);
-  const int acc = MODE == FWD ? 0 : g->accs * D;
+  const int acc = MODE == FWD ? 0 : accumulators(NP) * g->D8 * 8;
   g->acc_slots = GROUPS * SBUF + 2 * acc <= TMEM_COLUMNS ? 2 : 1;
   return std::max(SMEM_MIN, g->a_slots * a_bytes + g->stages * stage + fixed);
 }
@@ -1294,7 +1318,6 @@ GSB_EXPORT int gsb_class_loss_bwd(const gsb_class_loss_args* a, void* stream) {
     o.rows = d.N;
     o.S = a->stride_c == 1 ? 0 : a->S;
     o.C = a->C;
-    o.dtype = a->dtype;
     gx.a = kept.packed_x;
     gx.b = kept.packed_w;
     gx.a_tiles = (int)d.x_tiles;
@@ -1316,7 +1339,6 @@ GSB_EXPORT int gsb_class_loss_bwd(const gsb_class_loss_args* a, void* stream) {
     o.inv_count = per_row ? nullptr : kept.inv_count;
     o.rows = a->V;
     o.C = a->C;
-    o.dtype = a->dtype;
     joins.bias.out = o;
     gw.a = kept.packed_w;
     gw.b = kept.packed_x;
@@ -1325,7 +1347,7 @@ GSB_EXPORT int gsb_class_loss_bwd(const gsb_class_loss_args* a, void* stream) {
     gw.splits = d.dw_splits;
     gw.slots = d.dw_slots;
     gw.part_acc = a->grad_weight ? w.part_w : nullptr;
-    gw.part_bias = w.part_bias;
+    gw.part_bias = a->grad_bias ? w.part_bias : nullptr;
     if (d.dw_splits == 1) {
       gw.grad = o;
     } else if (a->grad_weight) {
@@ -1356,6 +1378,12 @@ GSB_EXPORT int gsb_class_loss_bwd(const gsb_class_loss_args* a, void* stream) {
   }
   if (r != GSB_OK) return r;
   const long long blocks = (joins.x.count + joins.w.count + joins.bias.count) / 32;
-  if (blocks > 0) join_grads_kernel<<<(unsigned)blocks, THREADS, 0, s>>>(joins, d.D);
+  if (blocks > 0) {
+    switch (a->dtype) {
+      case GSB_TYPE_BF16: join_grads_kernel<__nv_bfloat16><<<(unsigned)blocks, THREADS, 0, s>>>(joins, d.D); break;
+      case GSB_TYPE_FP16: join_grads_kernel<__half><<<(unsigned)blocks, THREADS, 0, s>>>(joins, d.D); break;
+      default: join_grads_kernel<float><<<(unsigned)blocks, THREADS, 0, s>>>(joins, d.D); break;
+    }
+  }
   return check_launch("gsb_class_loss_bwd");
 }
