@@ -559,6 +559,7 @@ __device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, 
   } else if (warp < LOADER) {
     // ---- z -> row statistics, or P ----
     constexpr int CH = MODE != FWD && NP == 3 ? 16 : 32;  // columns in registers at a time
+    constexpr bool AHEAD = MODE == FWD || CH == 16;       // the next ones are loaded meanwhile, registers permitting
     const int group = warp / 4;
     const uint32_t buffer = tmem + lanes + group * SBUF;
     const int step = ctas;
@@ -606,10 +607,10 @@ __device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, 
         labelled = __any_sync(0xffffffffu, labelled);
         uint32_t z[CH];
         float2 tile_s[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        if (MODE == FWD) tmem_load(buffer, z);
+        if (AHEAD) tmem_load(buffer, z);
 #pragma unroll 1
         for (int c = 0; c < TN; c += CH) {
-          if (MODE != FWD) tmem_load(buffer + c, z);  // four warps a scheduler hide it; registers are scarce
+          if (!AHEAD) tmem_load(buffer + c, z);
           tmem_load_wait(z);
           if (MODE == FWD && c + CH == TN) {
             fence_before();
@@ -636,10 +637,10 @@ __device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, 
               }
             }
           }
-          if (MODE == FWD && c + CH < TN) tmem_load(buffer + c + CH, z);
+          if (AHEAD && c + CH < TN) tmem_load(buffer + c + CH, z);
           if (MODE == FWD) {
             const int rel = y - (col0 + c);
-            if (labelled) {
+            if (labelled && __any_sync(0xffffffffu, y >= 0 && (unsigned)rel < (unsigned)CH)) {
               float tl = 0.f;
 #pragma unroll
               for (int i = 0; i < CH / 2; ++i) {
@@ -675,6 +676,7 @@ __device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, 
             if (labelled) {
               if (MODE == DX) {
                 const int rel = y >= 0 ? y - (col0 + c) : -1;
+                if (__any_sync(0xffffffffu, (unsigned)rel < (unsigned)CH))
 #pragma unroll
                 for (int i = 0; i < CH / 2; ++i) {
                   if (rel == 2 * i) x[i].x -= 1.f;
