@@ -59,6 +59,7 @@ import torch
 from . import _lib, _pipeline as pl
 from ._autograd import _camera
 from ._runtime import resolve_execution_options
+from .codebook import lookup_backward, lookup_forward
 from .view_sharding import GradientBuffer
 
 NUM_CHANNELS = 3
@@ -160,10 +161,18 @@ class FusedViewStep:
     process group when one is initialised.  The step ends with one host read
     of the device error word (a synchronisation), so an error flagged by any
     of its kernels raises ``RuntimeError`` from this call.
+
+    With ``sh_codes`` (P,) the scene's SH rows are shared: ``sh`` is a codebook
+    (rows, K, 3) and Gaussian p renders row ``sh_codes[p]`` (-1: zero SH).  Each
+    step expands the rows, trains them as above and sums their gradients by
+    code into the codebook's block of the flat buffer, before the all-reduce
+    (which then carries the codebook instead of P rows).  Views run view by
+    view; the range-ordered backward is not available.
     """
 
     def __init__(self, params: Sequence[torch.Tensor], settings: Sequence, l1_weight: float = 1.0,
-                 ssim_weight: float = 0.2, group=None, densify_stats: bool = False, batch_sh: bool | None = None):
+                 ssim_weight: float = 0.2, group=None, densify_stats: bool = False, batch_sh: bool | None = None,
+                 sh_codes: torch.Tensor | None = None):
         if len(params) != 5:
             raise ValueError("params must be (means, scales, rotations, opacities, sh)")
         means, scales, rots, opac, sh = params
@@ -171,11 +180,20 @@ class FusedViewStep:
         for t, shape in ((means, (P, 3)), (scales, (P, 3)), (rots, (P, 4)), (opac, (P, 1))):
             if tuple(t.shape) != shape or t.dtype != torch.float32 or not t.is_contiguous():
                 raise ValueError(f"parameter of shape {tuple(t.shape)} must be contiguous fp32 {shape}")
-        if sh.ndim != 3 or sh.shape[0] != P or sh.shape[2] != NUM_CHANNELS or sh.dtype != torch.float32 \
-                or not sh.is_contiguous():
-            raise ValueError("sh must be contiguous fp32 (P, K, 3)")
+        if sh.ndim != 3 or (sh_codes is None and sh.shape[0] != P) or sh.shape[2] != NUM_CHANNELS \
+                or sh.dtype != torch.float32 or not sh.is_contiguous():
+            raise ValueError("sh must be contiguous fp32 (P, K, 3)" if sh_codes is None else
+                             "sh must be a contiguous fp32 codebook (rows, K, 3)")
         if not settings:
             raise ValueError("no views")
+        self.sh_codes = None
+        if sh_codes is not None:
+            if sh_codes.shape != (P,) or sh_codes.dtype not in (torch.int32, torch.int64) \
+                    or sh_codes.device != means.device:
+                raise ValueError(f"sh_codes must be an int32 or int64 tensor of shape ({P},) on {means.device}")
+            self.sh_codes = sh_codes.contiguous()
+            self._sh_rows = torch.empty((P, *sh.shape[1:]), dtype=torch.float32, device=means.device)
+            self._grad_sh_rows = torch.zeros_like(self._sh_rows)
         self.params = list(params)
         self.settings = list(settings)
         self.cams = [_camera(rs) for rs in self.settings]
@@ -250,8 +268,18 @@ class FusedViewStep:
     def concurrent_views(self, on: bool) -> None:
         self.num_streams = 2 if on else 1
 
+    @property
+    def _sh(self) -> torch.Tensor:
+        """The SH rows the views render."""
+        return self.params[4] if self.sh_codes is None else self._sh_rows
+
+    @property
+    def _grad_sh(self) -> torch.Tensor:
+        return self.grads.views[4] if self.sh_codes is None else self._grad_sh_rows
+
     def _gaussians(self, rs) -> pl.Gaussians:
-        means, scales, rots, opac, sh = self.params
+        means, scales, rots, opac, _ = self.params
+        sh = self._sh
         return pl.make_gaussians(means, opac, scales, rots, None, sh, None, rs.scale_modifier, rs.sh_degree)
 
     def _staging_buffer(self, i: int, t: torch.Tensor) -> torch.Tensor:
@@ -318,10 +346,10 @@ class FusedViewStep:
             self._grad_acc[lane] = acc_buf
         grad_acc = pl.render_backward(pre.records, binned, cam, bg, ren.alpha, ren.n_contrib, grad_img, None, None,
                                       False, P, grad_acc=acc_buf)
-        v_means, v_scales, v_rots, v_opac, v_sh = self.grads.views
+        v_means, v_scales, v_rots, v_opac, _ = self.grads.views
         out = pl.PreprocessGrads(grad_means3D=v_means, grad_means2D=None, grad_opacity=v_opac,
                                  grad_scales=v_scales, grad_rotations=v_rots, grad_cov3D=None,
-                                 grad_sh=None if self.batch_sh else v_sh,
+                                 grad_sh=None if self.batch_sh else self._grad_sh,
                                  grad_colors=self._grad_colors[i] if self.batch_sh else None)
         if before_accumulate is not None:
             torch.cuda.current_stream(self.device).wait_event(before_accumulate)
@@ -379,20 +407,26 @@ class FusedViewStep:
         range, each range all-reduced while the next is computed."""
         if len(targets) != len(self.settings):
             raise ValueError(f"expected {len(self.settings)} targets, got {len(targets)}")
+        if self.sh_codes is not None and (self.range_backward or self.deferred_views):
+            raise ValueError("the range-ordered backward is not available with sh_codes")
         n_streams = max(1, int(self.num_streams))
         with torch.cuda.device(self.device):
             main = torch.cuda.current_stream(self.device)
             while len(self._side) < n_streams - 1:
                 self._side.append(torch.cuda.Stream(self.device))
             streams = [main] + self._side[: n_streams - 1]
-            means, _, _, _, sh = self.params
+            means, sh = self.params[0], self._sh
+            if self.sh_codes is not None:
+                lookup_forward(self.params[4].detach(), self.sh_codes, out=sh)
             if self.batch_sh:
                 # the SH block is stored whole by the SH backward; only the rest needs zeroing
-                self.grads.flat[: self.grads.flat.numel() - sh.numel()].zero_()
+                self.grads.flat[: self.grads.flat.numel() - self.params[4].numel()].zero_()
                 self.grads.attach()
                 pl.sh_colors_views(means, sh, self._sh_degree, self._campos, out=self._colors)
             else:
                 self.grads.zero_()
+                if self.sh_codes is not None:
+                    self._grad_sh.zero_()
             P, V = means.shape[0], len(targets)
             deferred = 0
             if self.batch_sh:
@@ -440,12 +474,15 @@ class FusedViewStep:
                 # the last view's event follows every earlier one (each view's accumulation waits for the
                 # previous)
                 main.wait_event(prev)
-                if self.batch_sh and _distributed(self.group) and self.sh_reduce_chunks > 0:
+                if self.batch_sh and self.sh_codes is None and _distributed(self.group) and self.sh_reduce_chunks > 0:
                     self._sh_backward_and_reduce()
                 else:
                     if self.batch_sh:
                         pl.sh_backward_views(means, sh, self._sh_degree, self._campos, self._grad_colors,
-                                             self.grads.views[4], self.grads.views[0])
+                                             self._grad_sh, self.grads.views[0])
+                    if self.sh_codes is not None:
+                        lookup_backward(self.params[4].detach(), self.sh_codes, 1.0, None, self._grad_sh,
+                                        out=self.grads.views[4])
                     self.grads.all_reduce(self.group)
             # errors flagged by the last view's emit and sort (earlier views' are read by the next
             # view's binning): raised by this call, before anyone uses its gradients

@@ -264,3 +264,66 @@ def test_rows_are_rendered_and_the_codebook_gets_the_scenes_gradient(cuda):
     (1 - gs.fused_ssim(color[None], target)).backward()
     assert float(sh.grad.abs().max()) > 0
     _check(table, codes, gain, sh.grad, sh.detach(), table.grad, gain.grad)
+
+
+def _shared_scene(dev, n, rows, views):
+    from gswarp_b200 import workloads as wl
+
+    sc = wl.config2_scene(seed=5, n=n)
+    cams = wl.ring_views(views, seed=5, width=320, height=192)
+    g = torch.Generator().manual_seed(3)
+    table = (0.3 * torch.randn(rows, 16, 3, generator=g)).to(dev)
+    codes = torch.randint(-1, rows, (n,), generator=g).to(dev)
+    params = [t.to(dev).contiguous() for t in (sc.means, sc.scales, sc.rotations, sc.opacities)]
+    settings = [gs.GaussianRasterizationSettings(
+        image_height=v.height, image_width=v.width, tanfovx=v.tanfovx, tanfovy=v.tanfovy,
+        bg=torch.zeros(3, device=dev), scale_modifier=1.0, viewmatrix=v.viewmatrix.to(dev),
+        projmatrix=v.projmatrix.to(dev), sh_degree=3, campos=v.campos.to(dev), prefiltered=False) for v in cams]
+    targets = [wl.target_image(100 + i, 192, 320).to(dev) for i in range(views)]
+    return params, table, codes, settings, targets
+
+
+@pytest.mark.parametrize("views, batch_sh", [(1, None), (3, True), (3, False)])
+@pytest.mark.parametrize("n", [20_000, 20_003])
+def test_fused_step_trains_shared_sh_rows(cuda, views, batch_sh, n):
+    from gswarp_b200.training import FusedViewStep
+
+    params, table, codes, settings, targets = _shared_scene(cuda, n, 700, views)
+    step = FusedViewStep(params + [table], settings, batch_sh=batch_sh, sh_codes=codes)
+    rows = torch.where((codes >= 0)[:, None, None], table[codes.clamp(min=0)], 0.0).contiguous()
+    dense = FusedViewStep([p.clone() for p in params] + [rows], settings, batch_sh=batch_sh)
+    for _ in range(2):  # a second step starts from zero again
+        losses, want = step.step(targets), dense.step(targets)
+        # the same rows give the same images
+        assert torch.equal(losses, want)
+        # the codebook's gradient is the sum of this step's row gradients
+        _check(table, codes, 1.0, step._grad_sh_rows, rows, step.grads.views[4], None)
+        assert table.grad.data_ptr() == step.grads.views[4].data_ptr()
+        # the render backward adds with atomics: blocks of the two runs agree by norm, as between any two runs
+        for a, b in zip(step.grads.views[:4], dense.grads.views[:4]):
+            assert float((a - b).norm()) <= 1e-4 * float(b.norm()) + 1e-7
+        assert float((step._grad_sh_rows - dense.grads.views[4]).norm()) <= 1e-4 * float(dense.grads.views[4].norm())
+
+
+def test_fused_step_refuses_bad_codes(cuda):
+    from gswarp_b200.training import FusedViewStep
+
+    params, table, codes, settings, targets = _shared_scene(cuda, 3000, 50, 2)
+    for bad in (codes[:-1], codes.float(), codes.cpu()):
+        with pytest.raises(ValueError, match="sh_codes"):
+            FusedViewStep(params + [table], settings, sh_codes=bad)
+    with pytest.raises(ValueError, match="codebook"):
+        FusedViewStep(params + [table[..., :2]], settings, sh_codes=codes)
+    with pytest.raises(ValueError, match="fp32 \\(P, K, 3\\)"):
+        FusedViewStep(params + [table], settings)
+    step = FusedViewStep(params + [table], settings, sh_codes=codes)
+    step.deferred_views = 1
+    with pytest.raises(ValueError, match="range-ordered"):
+        step.step(targets)
+    step.deferred_views = 0
+    step.step(targets)
+    step.sh_codes[5] = 50
+    with pytest.raises(RuntimeError, match="code"):
+        step.step(targets)
+    step.sh_codes[5] = 3
+    step.step(targets)
