@@ -179,7 +179,7 @@ class CodebookArgs(ctypes.Structure):
 class ClassLossArgs(ctypes.Structure):
     _fields_ = [
         ("B", c_ll), ("S", c_ll), ("V", c_ll), ("C", c_int), ("dtype", c_int),
-        ("reduction", c_int), ("labels64", c_int),
+        ("reduction", c_int), ("labels64", c_int), ("train", c_int),
         ("stride_b", c_ll), ("stride_c", c_ll), ("stride_s", c_ll), ("ignore_index", c_ll),
         ("features", vp), ("weight", vp), ("bias", vp), ("labels", vp), ("loss", vp), ("kept", vp),
         ("upstream", vp), ("grad_features", vp), ("grad_weight", vp), ("grad_bias", vp),

@@ -78,7 +78,7 @@ def _rows(features):
     return x, B, H * W, C, (sb, max(sc, 2) if C == 1 else sc, sw)
 
 
-def _forward(features, weight, labels, bias, ignore_index, reduction):
+def _forward(features, weight, labels, bias, ignore_index, reduction, train=True):
     """``(loss, args, kept, bytes of the backward workspace)``: the argument block with its sizes, and the
     buffer that backward reads."""
     x, B, S, C, (sb, sc, ss) = _rows(features)
@@ -88,7 +88,7 @@ def _forward(features, weight, labels, bias, ignore_index, reduction):
     b = bias.contiguous() if bias is not None else None
     y = labels.contiguous()
     a = _lib.ClassLossArgs(B, S, w.shape[0], C, _lib.DTYPES[x.dtype], _REDUCTIONS[reduction],
-                           labels.dtype == torch.int64, sb, sc, ss, ignore_index,
+                           labels.dtype == torch.int64, train, sb, sc, ss, ignore_index,
                            x.data_ptr(), w.data_ptr(), None if b is None else b.data_ptr(), y.data_ptr())
     sizes = _SIZES()
     _lib.call("gsb_class_loss_sizes", a, sizes)
@@ -171,5 +171,5 @@ def class_cross_entropy(features, weight, labels, bias=None, ignore_index=-100, 
     _validate(features, weight, labels, bias, ignore_index, reduction, train)
     if not train:
         with torch.no_grad():
-            return _forward(features, weight, labels, bias, ignore_index, reduction)[0]
+            return _forward(features, weight, labels, bias, ignore_index, reduction, False)[0]
     return _ClassCrossEntropy.apply(features, weight, labels, bias, ignore_index, reduction)

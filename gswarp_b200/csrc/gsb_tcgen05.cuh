@@ -123,9 +123,9 @@ __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::
 // `stride` along M or N.  Adding bytes / 16 to the low half moves the operand.
 __device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lead) { return addr >> 4 | (lead >> 4) << 16; }
 __device__ __forceinline__ uint32_t desc_hi(uint32_t stride) { return stride >> 4 | 1u << 14; }
-// bf16 operands, fp32 accumulator, M = 128.
-__device__ __forceinline__ uint32_t instr_desc(int n, bool b_mn_major) {
-  return 1u << 4 | 1u << 7 | 1u << 10 | (b_mn_major ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (128u >> 4) << 24;
+// bf16 (or fp16) operands, fp32 accumulator, M = 128.
+__device__ __forceinline__ uint32_t instr_desc(int n, bool b_mn_major, bool fp16 = false) {
+  return 1u << 4 | (fp16 ? 0u : 1u << 7 | 1u << 10) | (b_mn_major ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (128u >> 4) << 24;
 }
 // The issuing warp runs these with all lanes, so that operands stay in uniform
 // registers; `leader` picks the lane (one, the same every time) that issues.

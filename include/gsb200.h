@@ -497,6 +497,7 @@ typedef struct {
   long long B, S, V;      /* B * S and V < 2^31 - 128 */
   int C, dtype;           /* channels; GSB_TYPE_* of features, weight and their gradients */
   int reduction, labels64;
+  int train;              /* gsb_class_loss_bwd will follow (it refuses otherwise) */
   long long stride_b, stride_c, stride_s;
   long long ignore_index;
   const void* features;

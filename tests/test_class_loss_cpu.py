@@ -72,7 +72,7 @@ def test_rows_address_every_element_of_a_strided_map(shape, strides, copied):
 
 def _args(**kw):
     a = _lib.ClassLossArgs()
-    a.B, a.S, a.V, a.C, a.reduction = 1, 10, 4, 3, 2
+    a.B, a.S, a.V, a.C, a.reduction, a.train = 1, 10, 4, 3, 2, 1
     for k in ("kept", "error_word", "workspace", "features", "weight", "labels", "loss", "upstream"):
         setattr(a, k, 256)  # refused before anything reads them
     a.workspace_bytes = 1 << 40
@@ -100,6 +100,7 @@ def test_c_abi_refuses_missing_inputs():
     for k in ("features", "weight", "labels", "loss"):
         assert L.gsb_class_loss_fwd(ctypes.byref(_args(**{k: None})), None) == _lib.GSB_ERR_INVALID
     assert L.gsb_class_loss_bwd(ctypes.byref(_args(upstream=None)), None) == _lib.GSB_ERR_INVALID
+    assert L.gsb_class_loss_bwd(ctypes.byref(_args(train=0)), None) == _lib.GSB_ERR_INVALID
     assert L.gsb_class_loss_fwd(None, None) == _lib.GSB_ERR_INVALID
 
 
