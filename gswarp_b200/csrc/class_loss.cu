@@ -22,7 +22,6 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
-#include <type_traits>
 
 #include "gsb_common.cuh"
 #include "gsb_tcgen05.cuh"
@@ -183,6 +182,7 @@ __global__ void __launch_bounds__(THREADS) pack_kernel(const gsb_class_loss_args
   }
   const bool contiguous = stride == 1 && (uintptr_t)at % 16 == 0;
   uint4* const out = (classes ? kept.packed_w : kept.packed_x) + (size_t)tile * PLANES * D8 * TILE;
+#pragma unroll(PLANES == 1 ? 4 : 1)
   for (int d8 = threadIdx.x / TILE; d8 < D8; d8 += THREADS / TILE) {
     float x[8];
     if (used) {
@@ -1025,7 +1025,7 @@ __global__ void __launch_bounds__(THREADS) join_grads_kernel(const Joins j, int 
 // Host side.
 // ---------------------------------------------------------------------------
 constexpr int SMS = 148;
-constexpr int JOIN_BLOCKS = SMS * 4;
+constexpr int JOIN_BLOCKS = SMS * 8;
 
 // Pieces of the streamed axis: the number for which the waves of work units
 // over the SMs take the least time, in tiles.  A unit costs `unit` tiles

@@ -208,6 +208,19 @@ def test_only_the_wanted_gradients(cuda):
     assert torch.equal(loss.detach(), full["loss"])
 
 
+@pytest.mark.parametrize("N, C, V", SIZES + [(300, 256, 700), (40_000, 16, 513)])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_a_forward_alone(cuda, N, C, V, dtype, reduction):
+    if C > 128 and dtype == torch.float32:
+        pytest.skip("fp32 features have at most 128 channels")
+    x, w, y, b = _inputs(N, C, V, dtype, bias=(N + V) % 2 == 0, seed=N + C + V)
+    x, w = x.requires_grad_(True), w.requires_grad_(True)
+    loss = gs.class_cross_entropy(x, w, y, b, reduction=reduction, train=False)
+    assert not loss.requires_grad
+    _compare({"loss": loss}, reference(x, w, y, b, -100, reduction))
+
+
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
 def test_no_row_left(cuda, reduction):
     x, w, y, b = _inputs(300, 16, 150, torch.float32)
