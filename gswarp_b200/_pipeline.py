@@ -55,6 +55,9 @@ def sticky_error_word(device: torch.device) -> torch.Tensor:
     idx = device.index if device.index is not None else torch.cuda.current_device()
     t = _STICKY.get(idx)
     if t is None:
+        if torch.cuda.is_current_stream_capturing():
+            # it would live in the graph's memory and be cleared by every replay
+            raise RuntimeError("gswarp_b200: make one call on this device before capturing a graph")
         t = torch.zeros(1, dtype=torch.int64, device=device)
         _STICKY[idx] = t
     return t

@@ -156,8 +156,8 @@ def class_cross_entropy(features, weight, labels, bias=None, ignore_index=-100, 
     ``features`` is a map (C, H, W) or (B, C, H, W), or rows (N, C); ``labels`` (int32 or int64) has its shape
     without C.  ``weight`` (V, C) shares the features' type: float32 with up to 128 channels, bfloat16 or float16
     with up to 256.  ``bias`` (V,) is float32.  Logits, softmax and sums are float32 and gradients are rounded
-    once to their input's type; for 16-bit inputs the softmax's probabilities are rounded to bfloat16 (bfloat16
-    inputs) or to 16 bits of precision (float16) before the gradients' products.
+    once to their input's type; for 16-bit inputs the softmax's probabilities are rounded to 16 bits of precision
+    before the gradients' products (to bfloat16's 8 for bfloat16 inputs of more than 8 channels and 128 classes).
 
     Returns a float32 scalar ("mean" over the rows that count, "sum") or the rows' losses in ``labels``' shape
     ("none").  Rows labelled ``ignore_index`` have loss 0 and no gradient, whatever their features hold; with no

@@ -32,8 +32,8 @@ def _validate(table, codes, scale) -> None:
     if not table.is_cuda or codes.device != table.device:
         raise ValueError("table and codes must be on the same CUDA device")
     row = math.prod(table.shape[1:])
-    if row < 1 or row > 1 << 24:
-        raise ValueError(f"table rows must have 1 to {1 << 24} elements, got {row}")
+    if row < 1 or row > 1 << 22:
+        raise ValueError(f"table rows must have 1 to {1 << 22} elements, got {row}")
     if table.shape[0] >= (1 << 31) - 1 or codes.numel() >= (1 << 31) - 4096:
         raise ValueError("table and codes must have fewer than 2**31 - 4096 rows")
     if isinstance(scale, torch.Tensor):

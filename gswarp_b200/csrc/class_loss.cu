@@ -82,6 +82,7 @@ struct PlanesType<3> {
 struct Kept {
   uint4 *packed_x, *packed_w;
   float *class_bias2, *row_lse2;  // base 2; classes and rows rounded up to whole tiles
+  float* row_exact;               // 2^(row_lse2 - the row's log-sum before it was rounded to fp32)
   int* row_y;                     // labels, -1 where a row has no gradient
   float* inv_count;
 };
@@ -226,13 +227,15 @@ struct GradOut {
   const float* upstream;
   const float* inv_count;  // null: upstream has one factor per row
   const int* y;            // rows without a gradient are zero (null: every row has one)
+  const float* row_exact;  // dX: what P was computed too small by (null: nothing)
   long long rows, S;       // S > 0: n = b * S + s, written as (b, c, s); S = 0: (n, c)
   int C;
 };
 __device__ __forceinline__ float grad_scale(const GradOut& o, long long n) {
   const int y = o.y ? o.y[n] : 0;  // loads side by side
   const float u = o.inv_count ? o.upstream[0] * o.inv_count[0] : o.upstream ? o.upstream[n] : 1.f;
-  return y < 0 ? 0.f : u;
+  const float e = o.row_exact ? o.row_exact[n] : 1.f;
+  return y < 0 ? 0.f : u * e;
 }
 // Columns c .. c + COUNT - 1 of row n; u from grad_scale.
 template <typename T, int COUNT>
@@ -270,6 +273,7 @@ struct StreamArgs {
   const uint4* b;          // streamed operand, packed
   const float* b2;         // bias of the classes, base 2
   const float* lse2;       // rows (DX, DW)
+  const float* row_exact;  // rows (DX)
   const int* y;            // rows
   const float* row_u;      // per-row upstream (DW, reduction none) or NULL
   int a_tiles, b_tiles, splits, D8;
@@ -412,7 +416,8 @@ __device__ __forceinline__ void store_p(uint32_t buffer, int c, const float2 (&p
   }
 }
 
-template <int MODE, int NP, int TN, bool FP16 = false>
+// PP: planes of P in the gradients, NP or (for NP = 1) 2.
+template <int MODE, int NP, int TN, int PP = NP, bool FP16 = false>
 __device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, const int cta, const int ctas) {
   using namespace tc;
   const int D8 = g.D8, D = D8 * 8;
@@ -551,11 +556,11 @@ __device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, 
       const uint32_t dst = tmem + ACC0 + c.acc.i * ACCS * D, p = tmem + b * SBUF;
       const uint32_t b_lo = desc_lo(b0 + c.bs.i * b_bytes, NP * D8 * 128);
 #pragma unroll
-      for (int q = 0; q < plane_products(NP); ++q) {
-        const int pa = plane_of_a(NP, q);
+      for (int q = 0; q < (NP == 1 ? PP : plane_products(NP)); ++q) {
+        const int pa = NP == 1 ? PP - 1 - q : plane_of_a(NP, q);
         const bool main = q + 1 == plane_products(NP);
         const uint32_t to = NP == 3 && !main ? dst + D : dst;
-        const uint32_t bq = b_lo + plane_of_b(NP, q) * D8 * 8;
+        const uint32_t bq = b_lo + (NP == 1 ? 0 : plane_of_b(NP, q)) * D8 * 8;
 #pragma unroll
         for (int k = 0; k < TN / 16; ++k)
           mma_ts(leader, to, p + p_column(TN, 16 * k, pa), bq + k * step, hi, idesc,
@@ -584,12 +589,12 @@ __device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, 
     uint32_t t = 0;
     bool ok = true;
     int y_next = 0;
-    float c_next = 0.f;
+    float c_next = 0.f, e_next = 1.f;
     auto fetch = [&](int u) {  // the row's constants, one unit ahead
       if (u >= units) return;
       const int row = unit_range(g, u).tile * TILE + (warp & 3) * 32 + lane;
       if (MODE != DW) y_next = g.y[row];
-      if (MODE == DX) c_next = -g.lse2[row];
+      if (MODE == DX) c_next = -g.lse2[row], e_next = g.row_exact[row];
       if (MODE == DW) c_next = g.b2[row];
     };
     fetch(cta);
@@ -598,6 +603,9 @@ __device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, 
       const int row = r.tile * TILE + (warp & 3) * 32 + lane;
       const int y = y_next;
       const float row_c = c_next;  // -lse2 (DX) or the class's bias (DW)
+      // dX: the row is scaled by row_exact at its end, which makes up for the rounding of lse2 to fp32 (at 2^17
+      // classes 6e-7 of every p of the row, which shows where P W cancels); the label's 1 is scaled back
+      const float one = MODE == DX ? 1.f / e_next : 1.f;
       fetch(u + step);
       const int slot = (int)((group - t) % GROUPS);  // this group's first tile in the unit
       float m = -INFINITY, s = 0.f;
@@ -696,8 +704,8 @@ __device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, 
                 if (__any_sync(0xffffffffu, (unsigned)rel < (unsigned)CH))
 #pragma unroll
                 for (int i = 0; i < CH / 2; ++i) {
-                  if (rel == 2 * i) x[i].x -= 1.f;
-                  if (rel == 2 * i + 1) x[i].y -= 1.f;
+                  if (rel == 2 * i) x[i].x -= one;
+                  if (rel == 2 * i + 1) x[i].y -= one;
                 }
               } else {
                 const int4* ym = reinterpret_cast<const int4*>(meta + TN + c);
@@ -729,7 +737,7 @@ __device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, 
                 float2 half[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) half[i] = x[8 * h + i];
-                store_p<NP, TN>(buffer, c + 16 * h, half);
+                store_p<PP, TN>(buffer, c + 16 * h, half);
               }
             }
           }
@@ -844,25 +852,25 @@ __device__ __forceinline__ void stream_pass(const StreamArgs& g, uint8_t* smem, 
 template <int NP, int TN, bool FP16>
 __global__ void __launch_bounds__(stream_threads<FWD>(), 1) forward_kernel(const StreamArgs g) {
   extern __shared__ __align__(1024) uint8_t smem[];
-  stream_pass<FWD, NP, TN, FP16>(g, smem, blockIdx.x, gridDim.x);
+  stream_pass<FWD, NP, TN, NP, FP16>(g, smem, blockIdx.x, gridDim.x);
 }
 
-template <int MODE, int NP, int TN>
+template <int MODE, int NP, int TN, int PP>
 __global__ void __launch_bounds__(stream_threads<MODE>(), 1) gradient_kernel(const StreamArgs g) {
   extern __shared__ __align__(1024) uint8_t smem[];
-  stream_pass<MODE, NP, TN>(g, smem, blockIdx.x, gridDim.x);
+  stream_pass<MODE, NP, TN, PP>(g, smem, blockIdx.x, gridDim.x);
 }
 
 // Both gradients in one launch, for calls whose CTAs have one unit each: dW's
 // CTAs then start on the SMs that dX leaves idle (8191 x 8200 x 65 fp32 313 ->
 // 269 us).  With more units the two kernels are faster apart (1080p, 256
 // classes, 16 channels: 708 us, together 785).
-template <int NP, int TN>
+template <int NP, int TN, int PP>
 __global__ void __launch_bounds__(stream_threads<DX>(), 1)
     gradients_kernel(const StreamArgs gx, const StreamArgs gw, const int x_ctas) {
   extern __shared__ __align__(1024) uint8_t smem[];
-  if ((int)blockIdx.x < x_ctas) stream_pass<DX, NP, TN>(gx, smem, blockIdx.x, x_ctas);
-  else stream_pass<DW, NP, TN>(gw, smem, blockIdx.x - x_ctas, gridDim.x - x_ctas);
+  if ((int)blockIdx.x < x_ctas) stream_pass<DX, NP, TN, PP>(gx, smem, blockIdx.x, x_ctas);
+  else stream_pass<DW, NP, TN, PP>(gw, smem, blockIdx.x - x_ctas, gridDim.x - x_ctas);
 }
 
 // ---------------------------------------------------------------------------
@@ -916,7 +924,7 @@ __global__ void __launch_bounds__(THREADS) join_rows_kernel(const gsb_class_loss
       m = top;
     }
     if (sub == 0 && inside) {
-      float l2 = INFINITY, l = 0.f;
+      float l2 = INFINITY, l = 0.f, exact = 1.f;
       if (y >= 0) {
         const float t = t_label[n];
         count += 1.0;
@@ -928,10 +936,12 @@ __global__ void __launch_bounds__(THREADS) join_rows_kernel(const gsb_class_loss
           const float ls = log2f(s);
           l = (float)(((double)(m - t) + (double)ls) * LN2);
           l2 = m + ls;
+          exact = exp2f((l2 - m) - ls);  // l2 - m is exact or nearly so: the part of ls that l2 holds
         }
         loss += l;
       }
       kept.row_lse2[n] = l2;
+      kept.row_exact[n] = exact;
       if (a.reduction == GSB_REDUCE_NONE && n < N) a.loss[n] = l;
     }
   }
@@ -1025,6 +1035,7 @@ __global__ void __launch_bounds__(THREADS) join_grads_kernel(const Joins j, int 
 // Host side.
 // ---------------------------------------------------------------------------
 constexpr int SMS = 148;
+constexpr int FEW_CLASSES = 128, FEW_CHANNELS = 8;
 constexpr int JOIN_BLOCKS = SMS * 8;
 
 // Pieces of the streamed axis: the number for which the waves of work units
@@ -1113,6 +1124,7 @@ inline size_t carve_kept(void* base, const Dims& d, Kept* k) {
   k->packed_w = c.take<uint4>((size_t)d.w_tiles * TILE * d.planes * d.D8);
   k->class_bias2 = c.take<float>((size_t)d.w_tiles * TILE);
   k->row_lse2 = c.take<float>((size_t)d.x_tiles * TILE);
+  k->row_exact = c.take<float>((size_t)d.x_tiles * TILE);
   k->row_y = c.take<int>((size_t)d.x_tiles * TILE);
   k->inv_count = c.take<float>(1);
   return c.off;
@@ -1208,23 +1220,23 @@ int launch_forward(StreamArgs g, cudaStream_t s) {
   forward_kernel<NP, TN, FP16><<<pass_ctas(g), stream_threads<FWD>(), smem, s>>>(g);
   return check_launch("class loss forward");
 }
-template <int NP, int TN>
+template <int NP, int TN, int PP = NP>
 int launch_backward(StreamArgs gx, StreamArgs gw, cudaStream_t s) {
   const size_t x_smem = plan_pass<DX, NP, TN>(&gx), w_smem = plan_pass<DW, NP, TN>(&gw);
   const int x_units = gx.a_tiles * gx.splits, w_units = gw.a_tiles * gw.splits;
   if (x_units && w_units && x_units <= SMS && w_units <= SMS) {
     const size_t smem = std::max(x_smem, w_smem);
-    cudaFuncSetAttribute(gradients_kernel<NP, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    gradients_kernel<NP, TN><<<x_units + w_units, stream_threads<DX>(), smem, s>>>(gx, gw, x_units);
+    cudaFuncSetAttribute(gradients_kernel<NP, TN, PP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    gradients_kernel<NP, TN, PP><<<x_units + w_units, stream_threads<DX>(), smem, s>>>(gx, gw, x_units);
     return check_launch("class loss backward");
   }
   if (x_units) {
-    cudaFuncSetAttribute(gradient_kernel<DX, NP, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)x_smem);
-    gradient_kernel<DX, NP, TN><<<pass_ctas(gx), stream_threads<DX>(), x_smem, s>>>(gx);
+    cudaFuncSetAttribute(gradient_kernel<DX, NP, TN, PP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)x_smem);
+    gradient_kernel<DX, NP, TN, PP><<<pass_ctas(gx), stream_threads<DX>(), x_smem, s>>>(gx);
   }
   if (w_units) {
-    cudaFuncSetAttribute(gradient_kernel<DW, NP, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)w_smem);
-    gradient_kernel<DW, NP, TN><<<pass_ctas(gw), stream_threads<DW>(), w_smem, s>>>(gw);
+    cudaFuncSetAttribute(gradient_kernel<DW, NP, TN, PP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)w_smem);
+    gradient_kernel<DW, NP, TN, PP><<<pass_ctas(gw), stream_threads<DW>(), w_smem, s>>>(gw);
   }
   return check_launch("class loss backward");
 }
@@ -1340,6 +1352,7 @@ GSB_EXPORT int gsb_class_loss_bwd(const gsb_class_loss_args* a, void* stream) {
   StreamArgs g{};
   g.b2 = kept.class_bias2;
   g.lse2 = kept.row_lse2;
+  g.row_exact = kept.row_exact;
   g.y = kept.row_y;
   g.error_word = a->error_word;
   g.D8 = d.D8;
@@ -1353,6 +1366,7 @@ GSB_EXPORT int gsb_class_loss_bwd(const gsb_class_loss_args* a, void* stream) {
     o.upstream = a->upstream;
     o.inv_count = per_row ? nullptr : kept.inv_count;
     o.y = kept.row_y;
+    o.row_exact = kept.row_exact;
     o.rows = d.N;
     o.S = a->stride_c == 1 ? 0 : a->S;
     o.C = a->C;
@@ -1407,7 +1421,14 @@ GSB_EXPORT int gsb_class_loss_bwd(const gsb_class_loss_args* a, void* stream) {
   }
   int r = GSB_ERR_INVALID;
   switch (d.planes * 1000 + d.grad_tn) {
-    case 1064: r = launch_backward<1, 64>(gx, gw, s); break;
+    case 1064:
+      // P's rounding to bf16 averages out over classes and channels. With few of either it does not, and a second
+      // plane of P costs little there (the passes are bound by the map's rows). Error of dX in units of that of
+      // its own rounding to bf16, one plane: 831,000 x 15 classes x 5 channels 1.65, 788,000 x 149 x 2 1.69,
+      // 239,000 x 627 x 9 1.35, 640,000 x 1000 x 32 1.25; two planes 1.0 everywhere, but 26% longer passes in
+      // the last, so one stays there.
+      r = a->V <= FEW_CLASSES || a->C <= FEW_CHANNELS ? launch_backward<1, 64, 2>(gx, gw, s) : launch_backward<1, 64>(gx, gw, s);
+      break;
     case 2064: r = launch_backward<2, 64>(gx, gw, s); break;
     case 2032: r = launch_backward<2, 32>(gx, gw, s); break;
     case 3064: r = launch_backward<3, 64>(gx, gw, s); break;

@@ -35,6 +35,7 @@ namespace {
 constexpr int THREADS = launch::CODEBOOK;
 constexpr int SEG_UNROLL = 4;       // rows in flight per group of lanes
 constexpr long long MAX_ROWS = (1ll << 31) - 4096;
+constexpr int MAX_COLS = 1 << 22;   // 65,535 column blocks of 128 or more
 
 template <typename T>
 struct Vec16 {
@@ -685,7 +686,7 @@ int check_args(const gsb_codebook_args* a, const char* what) {
     set_error("%s: null arguments", what);
     return GSB_ERR_INVALID;
   }
-  if (a->P < 0 || a->P >= MAX_ROWS || a->K < 0 || a->K >= (1ll << 31) - 1 || a->D < 1 || a->D > (1 << 24)) {
+  if (a->P < 0 || a->P >= MAX_ROWS || a->K < 0 || a->K >= (1ll << 31) - 1 || a->D < 1 || a->D > MAX_COLS) {
     set_error("%s: sizes out of range (P %lld, K %lld, D %d)", what, a->P, a->K, a->D);
     return GSB_ERR_INVALID;
   }

@@ -456,7 +456,7 @@ int gsb_knn(const gsb_knn_args* a, void* stream);
 typedef struct {
   long long P;            /* rows, < 2^31 - 4096 */
   long long K;            /* codebook rows, < 2^31 - 1 */
-  int D;                  /* elements per row */
+  int D;                  /* elements per row, <= 2^22 */
   int dtype;              /* GSB_TYPE_* of table, out, grad_out, grad_table */
   int codes64;            /* codes are int64 (else int32) */
   float scale;

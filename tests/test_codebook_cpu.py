@@ -29,7 +29,7 @@ def test_bad_arguments_are_value_errors(args, message):
 
 @pytest.mark.parametrize("table, codes, scale, message", [
     ((4, 0), (5,), 1.0, "elements"),
-    ((4, 1 << 25), (5,), 1.0, "elements"),
+    ((4, (1 << 22) + 1), (5,), 1.0, "elements"),
     (((1 << 31) - 1, 1), (5,), 1.0, "rows"),
     ((4, 3), ((1 << 31) - 4096,), 1.0, "rows"),
     ((4, 3), (5,), "2", "number"),
@@ -57,7 +57,7 @@ def _args(**kw):
 
 
 @pytest.mark.parametrize("kw", [dict(P=-1), dict(P=(1 << 31) - 4096), dict(K=-1), dict(K=(1 << 31) - 1), dict(D=0),
-                                dict(D=(1 << 24) + 1), dict(dtype=3), dict(dtype=-1), dict()])
+                                dict(D=(1 << 22) + 1), dict(dtype=3), dict(dtype=-1), dict()])
 def test_c_abi_refuses(kw):
     L = _lib.load()
     for fn in (L.gsb_codebook_fwd, L.gsb_codebook_bwd):

@@ -417,6 +417,28 @@ def test_captured_and_replayed(cuda):
             assert all(torch.equal(out[k], want[k]) for k in want)
 
 
+@pytest.mark.parametrize("rows", [False, True])
+def test_offsets_past_32_bits(cuda, rows):
+    C, H, W, V = 256, 2900, 2900, 40  # 2.15e9 elements; the last 3 image rows count
+    g = torch.Generator(device="cuda").manual_seed(0)
+    N, tail = H * W, 3 * W
+    x = torch.zeros((N, C) if rows else (C, H, W), dtype=torch.bfloat16, device=cuda)
+    last = torch.randn(tail, C, generator=g, device="cuda").bfloat16()
+    if rows:
+        x[N - tail:] = last
+    else:
+        x[:, H - 3:] = last.t().reshape(C, 3, W)
+    w = (torch.randn(V, C, generator=g, device="cuda") / 16).bfloat16()
+    y = torch.full((N,), -100, device=cuda)
+    y[N - tail:] = torch.randint(0, V, (tail,), generator=g, device="cuda")
+    up = torch.ones((), device=cuda)
+    got = _run(x, w, y if rows else y.view(H, W), None, "mean", up)
+    gx = got["grad_features"]
+    head, end = (gx[:N - tail], gx[N - tail:]) if rows else (gx[:, :H - 3], gx[:, H - 3:].reshape(C, tail).t())
+    assert not head.any()
+    _compare({**got, "grad_features": end}, reference(last, w, y[N - tail:], None, -100, "mean", up))
+
+
 def test_a_scene_with_shared_feature_rows_is_trained_through_both(cuda):
     """Codebook rows -> rasterizer -> class loss, and back to the codebook."""
     from gswarp_b200 import workloads as wl

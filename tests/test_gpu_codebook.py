@@ -242,6 +242,32 @@ def test_captured_and_replayed(cuda):
             assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+def test_offsets_past_32_bits(cuda):
+    P, D, K = 46_000_003, 48, 5000  # 2.2e9 elements
+    g = torch.Generator(device="cuda").manual_seed(0)
+    table = torch.randn(K, D, generator=g, device="cuda").bfloat16()
+    codes = torch.randint(0, K, (P,), generator=g, device="cuda", dtype=torch.int32)
+    out = codebook.lookup_forward(table, codes, 2.0)
+    for lo in (0, 44_739_242 - 5, P - 1000):  # the element 2^31 is in row 44,739,242
+        n = min(1000, P - lo)
+        assert torch.equal(out[lo:lo + n], table[codes[lo:lo + n].long()] * 2)
+    # a gradient that is zero but in the last rows
+    out.zero_()
+    out[P - 1000:] = torch.randn(1000, D, generator=g, device="cuda").bfloat16()
+    gt, _ = codebook.lookup_backward(table, codes, 2.0, None, out)
+    _check(table, codes[P - 1000:], 2.0, out[P - 1000:],
+           codebook.lookup_forward(table, codes[P - 1000:].contiguous(), 2.0), gt, None)
+
+
+def test_the_first_call_on_a_device_is_not_captured(cuda, monkeypatch):
+    monkeypatch.setattr(pl, "_STICKY", {})
+    table, codes, s, _ = _inputs(100, 5, 3, torch.float32)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="before capturing"):
+        with torch.cuda.graph(graph):
+            codebook.lookup_forward(table, codes, 1.0, s)
+
+
 def test_rows_are_rendered_and_the_codebook_gets_the_scenes_gradient(cuda):
     """As it is used: shared SH rows expanded, rendered and trained through the rasterizer."""
     from gswarp_b200 import workloads as wl
