@@ -43,10 +43,12 @@ def _validate(table, codes, scale) -> None:
         raise ValueError("scale must be a number or a float32 tensor")
 
 
-def _args(table, codes, scale, gain) -> _lib.CodebookArgs:
-    return _lib.CodebookArgs(codes.numel(), table.shape[0], math.prod(table.shape[1:]), _lib.DTYPES[table.dtype],
-                             codes.dtype == torch.int64, scale, table.data_ptr(), codes.data_ptr(),
-                             None if gain is None else gain.data_ptr())
+def _args(shape, dtype, table, codes, scale, gain, device) -> _lib.CodebookArgs:
+    a = _lib.CodebookArgs(codes.numel(), shape[0], math.prod(shape[1:]), _lib.DTYPES[dtype],
+                          codes.dtype == torch.int64, scale, None if table is None else table.data_ptr(),
+                          codes.data_ptr(), None if gain is None else gain.data_ptr())
+    a.error_word = _pipeline.sticky_error_word(device).data_ptr()
+    return a
 
 
 def lookup_forward(table: torch.Tensor, codes: torch.Tensor, scale: float = 1.0,
@@ -55,25 +57,24 @@ def lookup_forward(table: torch.Tensor, codes: torch.Tensor, scale: float = 1.0,
     dev = table.device
     if out is None:
         out = torch.empty(codes.shape + table.shape[1:], dtype=table.dtype, device=dev)
-    a = _args(table, codes, scale, gain)
+    a = _args(table.shape, table.dtype, table, codes, scale, gain, dev)
     a.out = out.data_ptr()
-    a.error_word = _pipeline.sticky_error_word(dev).data_ptr()
     with _pipeline._stage_timer("codebook_fwd", {"rows": a.P, "kernels": 1}):
         _lib.call_on(dev, "gsb_codebook_fwd", a)
     return out
 
 
-def lookup_backward(table: torch.Tensor, codes: torch.Tensor, scale: float, gain: torch.Tensor | None,
-                    grad_out: torch.Tensor, want_table: bool = True, want_gain: bool = False,
-                    out: torch.Tensor | None = None):
-    """``(grad_table, grad_gain)`` of contiguous tensors; ``grad_table`` into ``out`` if given."""
-    dev = table.device
-    a = _args(table, codes, scale, gain)
+def lookup_backward(shape, dtype, table: torch.Tensor | None, codes: torch.Tensor, scale: float,
+                    gain: torch.Tensor | None, grad_out: torch.Tensor, want_table: bool = True,
+                    want_gain: bool = False, out: torch.Tensor | None = None):
+    """``(grad_table, grad_gain)`` of contiguous tensors, for a table of ``shape`` and ``dtype`` (read only for the
+    gains' gradient); ``grad_table`` into ``out`` if given."""
+    dev = grad_out.device
+    a = _args(shape, dtype, table, codes, scale, gain, dev)
     a.grad_out = grad_out.data_ptr()
-    a.error_word = _pipeline.sticky_error_word(dev).data_ptr()
     grad_table = grad_gain = None
     if want_table:
-        grad_table = torch.empty_like(table) if out is None else out
+        grad_table = torch.empty(shape, dtype=dtype, device=dev) if out is None else out
         a.grad_table = grad_table.data_ptr()
         n = _lib.load().gsb_codebook_bwd_workspace_bytes(a.P, a.K, a.D)
         if n:
@@ -92,19 +93,24 @@ class _CodebookLookup(torch.autograd.Function):
     def forward(ctx, table, codes, scale, gain):
         t = table.contiguous()
         c = codes.contiguous()
-        g = gain.contiguous() if gain is not None else None
-        ctx.scale = scale
-        ctx.save_for_backward(t, c, g)
+        ctx.scale, ctx.shape, ctx.dtype = scale, table.shape, table.dtype
+        if gain is None:
+            ctx.save_for_backward(c)  # the table's gradient does not need the table
+            return lookup_forward(t, c, scale)
+        g = gain.contiguous()
+        ctx.save_for_backward(c, g, t)
         return lookup_forward(t, c, scale, g)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        t, c, g = ctx.saved_tensors
-        want_table, want_gain = ctx.needs_input_grad[0], ctx.needs_input_grad[3]
+        want_table, _, _, want_gain = ctx.needs_input_grad
         if not (want_table or want_gain):
             return None, None, None, None
-        grad_table, grad_gain = lookup_backward(t, c, ctx.scale, g, grad.contiguous(), want_table, want_gain)
+        saved = ctx.saved_tensors
+        c, g, t = saved if len(saved) == 3 else (saved[0], None, None)
+        grad_table, grad_gain = lookup_backward(ctx.shape, ctx.dtype, t, c, ctx.scale, g, grad.contiguous(), want_table,
+                                                want_gain)
         return grad_table, None, None, grad_gain
 
 

@@ -694,7 +694,7 @@ int check_args(const gsb_codebook_args* a, const char* what) {
     set_error("%s: unknown dtype %d", what, a->dtype);
     return GSB_ERR_INVALID;
   }
-  if (a->P > 0 && (!a->codes || !a->error_word || (a->K > 0 && !a->table))) {
+  if (a->P > 0 && (!a->codes || !a->error_word)) {
     set_error("%s: null pointer", what);
     return GSB_ERR_INVALID;
   }
@@ -709,7 +709,7 @@ GSB_EXPORT int gsb_codebook_fwd(const gsb_codebook_args* a, void* stream) {
   const int st = check_args(a, "gsb_codebook_fwd");
   if (st != GSB_OK) return st;
   if (a->P == 0) return GSB_OK;
-  if (!a->out) {
+  if (!a->out || (a->K > 0 && !a->table)) {
     set_error("gsb_codebook_fwd: null pointer");
     return GSB_ERR_INVALID;
   }
@@ -734,8 +734,8 @@ GSB_EXPORT int gsb_codebook_bwd(const gsb_codebook_args* a, void* stream) {
     set_error("gsb_codebook_bwd: null pointer");
     return GSB_ERR_INVALID;
   }
-  if (a->grad_gain && !a->gain) {
-    set_error("gsb_codebook_bwd: grad_gain without gain");
+  if (a->grad_gain && (!a->gain || (a->K > 0 && !a->table))) {
+    set_error("gsb_codebook_bwd: grad_gain without gain or table");
     return GSB_ERR_INVALID;
   }
   const size_t need = a->grad_table ? gsb_codebook_bwd_workspace_bytes(a->P, a->K, a->D) : 0;

@@ -481,8 +481,9 @@ class FusedViewStep:
                         pl.sh_backward_views(means, sh, self._sh_degree, self._campos, self._grad_colors,
                                              self._grad_sh, self.grads.views[0])
                     if self.sh_codes is not None:
-                        lookup_backward(self.params[4].detach(), self.sh_codes, 1.0, None, self._grad_sh,
-                                        out=self.grads.views[4])
+                        table = self.grads.views[4]
+                        lookup_backward(table.shape, table.dtype, None, self.sh_codes, 1.0, None, self._grad_sh,
+                                        out=table)
                     self.grads.all_reduce(self.group)
             # errors flagged by the last view's emit and sort (earlier views' are read by the next
             # view's binning): raised by this call, before anyone uses its gradients

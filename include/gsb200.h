@@ -460,7 +460,7 @@ typedef struct {
   int dtype;              /* GSB_TYPE_* of table, out, grad_out, grad_table */
   int codes64;            /* codes are int64 (else int32) */
   float scale;
-  const void* table;      /* (K,D) contiguous */
+  const void* table;      /* (K,D) contiguous; backward: only with grad_gain */
   const void* codes;      /* (P) */
   const float* gain;      /* (P) or NULL */
   void* out;              /* forward: (P,D) */

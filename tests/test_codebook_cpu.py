@@ -73,6 +73,9 @@ def test_c_abi_refuses_missing_buffers():
     assert L.gsb_codebook_bwd(ctypes.byref(_args(**full)), None) == _lib.GSB_ERR_INVALID  # no grad_out
     full["grad_out"] = p
     assert L.gsb_codebook_bwd(ctypes.byref(_args(grad_gain=p, **full)), None) == _lib.GSB_ERR_INVALID  # no gain
+    bare = {**full, "table": None, "out": p, "gain": p}
+    assert L.gsb_codebook_bwd(ctypes.byref(_args(grad_gain=p, **bare)), None) == _lib.GSB_ERR_INVALID  # no table
+    assert L.gsb_codebook_fwd(ctypes.byref(_args(**bare)), None) == _lib.GSB_ERR_INVALID
     need = L.gsb_codebook_bwd_workspace_bytes(100_000, 400, 3)
     assert need > 0
     short = _args(P=100_000, K=400, grad_table=p, workspace=p, workspace_bytes=need - 1, **full)

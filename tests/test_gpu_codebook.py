@@ -222,14 +222,14 @@ def test_captured_and_replayed(cuda):
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
-        codebook.lookup_backward(table, codes, 1.0, s, up, want_gain=True)
+        codebook.lookup_backward(table.shape, table.dtype, table, codes, 1.0, s, up, want_gain=True)
     torch.cuda.current_stream().wait_stream(side)
     graphs = []
     for _ in range(2):  # two graphs, each with its own workspace
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
             out = (codebook.lookup_forward(table, codes, 1.0, s),
-                   *codebook.lookup_backward(table, codes, 1.0, s, up, want_gain=True))
+                   *codebook.lookup_backward(table.shape, table.dtype, table, codes, 1.0, s, up, want_gain=True))
         graphs.append((g, out))
     for seed in (11, 12):
         t2, c2, s2, u2 = _inputs(3000, 40, 48, torch.float32, seed=seed)
@@ -254,7 +254,7 @@ def test_offsets_past_32_bits(cuda):
     # a gradient that is zero but in the last rows
     out.zero_()
     out[P - 1000:] = torch.randn(1000, D, generator=g, device="cuda").bfloat16()
-    gt, _ = codebook.lookup_backward(table, codes, 2.0, None, out)
+    gt, _ = codebook.lookup_backward(table.shape, table.dtype, None, codes, 2.0, None, out)
     _check(table, codes[P - 1000:], 2.0, out[P - 1000:],
            codebook.lookup_forward(table, codes[P - 1000:].contiguous(), 2.0), gt, None)
 
