@@ -33,7 +33,6 @@ namespace gsb {
 namespace {
 
 constexpr int THREADS = launch::CODEBOOK;
-constexpr int SEG_UNROLL = 4;       // rows in flight per group of lanes
 constexpr long long MAX_ROWS = (1ll << 31) - 4096;
 constexpr int MAX_COLS = 1 << 22;   // 65,535 column blocks of 128 or more
 
@@ -86,7 +85,7 @@ __device__ __forceinline__ long long read_code(const void* codes, int codes64, l
 // ---------------------------------------------------------------------------
 // Forward.  A CTA owns ROWS consecutive rows (a multiple of 16, which keeps
 // CTAs 16-byte aligned); their codes and factors go through shared memory, and
-// the threads walk the CTA's flat output in 16-byte pieces, several in flight.
+// the threads walk the CTA's flat output in 16-byte pieces.
 // ALIGNED: rows are whole 16-byte pieces and both pointers are aligned, so a
 // piece is one load; otherwise a piece may cross rows and is gathered element
 // by element (the rows come from L1/L2), while its store still is one when the
@@ -95,7 +94,7 @@ __device__ __forceinline__ long long read_code(const void* codes, int codes64, l
 template <typename T, bool ALIGNED, int ROWS>
 __global__ void __launch_bounds__(THREADS) codebook_gather_kernel(const gsb_codebook_args a, int out_aligned) {
   constexpr int VW = Vec16<T>::N;
-  constexpr int UNROLL = ALIGNED ? 4 : 2;
+  constexpr int UNROLL = ALIGNED ? 1 : 2;
   __shared__ int s_code[ROWS];
   __shared__ float s_scale[ROWS];
   const long long base = (long long)blockIdx.x * ROWS;
@@ -312,6 +311,9 @@ struct SegArgs {
 
 template <typename T, int VW, int NV, bool DGAIN>
 __global__ void __launch_bounds__(THREADS) segment_sum_kernel(const SegArgs a) {
+  // Rows in flight: registers against occupancy (300,000 x 77 fp16 40 us with 2, 52 with 4; 1M x 48 bf16 56 and 65;
+  // 300,000 x 77 fp32 37 and 33; 6M x 48 fp32 with gains 433 and 411, 577 with 8).
+  constexpr int SEG_UNROLL = sizeof(T) == 2 ? 2 : 4;
   const int G = 1 << a.gshift;
   const int lane = threadIdx.x & (G - 1);
   const long long chunk = ((long long)blockIdx.x * THREADS + threadIdx.x) >> a.gshift;
@@ -425,7 +427,7 @@ __global__ void __launch_bounds__(THREADS) segment_sum_kernel(const SegArgs a) {
 // starts there and leaves to the right, it adds up that run's partial rows.
 // Runs of more than LONG_RUN chunks are left to the whole CTA, whose warps
 // take every eighth partial row.
-constexpr int LONG_RUN = 32;
+constexpr int LONG_RUN = 8;
 
 template <typename T>
 __global__ void __launch_bounds__(THREADS) run_join_kernel(const SegArgs a) {
@@ -452,15 +454,15 @@ __global__ void __launch_bounds__(THREADS) run_join_kernel(const SegArgs a) {
   auto sum_rows = [&](int start, int end, int c, int from, int step) {
     float sum = 0.f;
     if (c < a.D) {
-      for (int k = start + from; k <= end; k += 4 * step) {
-        float v[4];
+      for (int k = start + from; k <= end; k += 8 * step) {
+        float v[8];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < 8; ++u) {
           const long long r = (long long)k + u * step;
           v[u] = r <= end ? a.part_rows[(2 * r + (r == start ? 1 : 0)) * a.D + c] : 0.f;
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) sum += v[u];
+        for (int u = 0; u < 8; ++u) sum += v[u];
       }
     }
     return sum;
@@ -514,7 +516,7 @@ __global__ void __launch_bounds__(THREADS) gain_dot_kernel(const gsb_codebook_ar
 // ---------------------------------------------------------------------------
 // Chunk length: long chunks leave few partial rows to write and read again,
 // short ones keep enough groups in flight when there are few rows.
-inline int chunk_len(long long P) { return P >= (1 << 20) ? 128 : P >= (1 << 17) ? 32 : 16; }
+inline int chunk_len(long long P) { return P >= (1 << 20) ? 128 : P >= (1 << 19) ? 64 : P >= (1 << 17) ? 32 : 16; }
 
 inline long long chunks_of(long long n, int len) { return (n + len - 1) / len; }
 
@@ -534,15 +536,16 @@ struct Shape {
   int vw, nv, gshift, col_blocks;
 };
 
-// Lanes and pieces that cover a row with the least waste.
+// Lanes and pieces that cover a row with the least waste, of those that hold at
+// most 12 elements of a row per lane if there are any.
 inline Shape pick_shape(int D, int vw) {
   const int pieces = (D + vw - 1) / vw;
   Shape best{vw, 4, 5, 0};
   int best_slots = 1 << 30;
   for (int g = 0; g <= 5; ++g)
     for (int nv = 1; nv <= 4; ++nv) {
-      const int slots = nv << g;
-      if (slots >= pieces && slots <= best_slots) {  // ties: more lanes, fewer pieces
+      const int slots = (nv << g) + (nv * vw > 12 ? 1 << 20 : 0);
+      if (nv << g >= pieces && slots <= best_slots) {  // ties: more lanes, fewer pieces
         best = Shape{vw, nv, g, 1};
         best_slots = slots;
       }
@@ -672,10 +675,10 @@ void launch_gather(const gsb_codebook_args* a, cudaStream_t s) {
 
 template <typename T>
 int run_fwd(const gsb_codebook_args* a, cudaStream_t s) {
-  // Longer CTAs spend less of their time on reading codes; short rows or few
-  // of them need shorter ones to fill the SMs.  About 16 KB of output each.
-  const long long bytes = (long long)a->D * sizeof(T);
-  if (a->P >= 148 * 8 * 256 && bytes <= 128) launch_gather<T, 256>(a, s);
+  // Longer CTAs spend less of their time on reading codes, few rows need
+  // shorter ones to fill the SMs (6M x 48 fp32: 64 rows 280 us, 128 217,
+  // 256 192, 512 201).
+  if (a->P >= 148 * 8 * 256) launch_gather<T, 256>(a, s);
   else if (a->P >= 148 * 8 * 128) launch_gather<T, 128>(a, s);
   else launch_gather<T, 32>(a, s);
   return check_launch("gsb_codebook_fwd");
