@@ -160,19 +160,31 @@ __global__ void __launch_bounds__(THREADS) codebook_gather_kernel(const gsb_code
 }
 
 // ---------------------------------------------------------------------------
-// Backward of few rows: P * K and P below the bounds of small_case().  A code
-// belongs to `wpc` warps of a CTA, each of which scans its part of the codes
-// and adds up the rows it finds, in order; the parts are then added in order.
-// One more "code" takes the rows without one (their gains' gradient is zero).
+// Backward of few rows, in one scan of all the codes by every warp.
+// BY_ROW false (few codes): a code belongs to `wpc` warps of a CTA, each of
+// which scans its part of the codes and adds up the rows it finds, in order;
+// the parts are then added in order.  One more "code" takes the rows without
+// one (their gains' gradient is zero).
+// BY_ROW true (very few rows): a warp takes the code of one row and gives up
+// when it meets the code before that row; the first row's warp adds them all.
 // ---------------------------------------------------------------------------
 constexpr int SMALL_COLS = 128;  // columns a warp sums at a time, four per lane
 
-template <typename T>
+template <typename T, bool BY_ROW>
 __global__ void __launch_bounds__(THREADS) code_scan_kernel(const gsb_codebook_args a, int wpc) {
   __shared__ float s_sum[THREADS / 32][SMALL_COLS];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int per_cta = THREADS / 32 / wpc, part = warp % wpc;
-  const long long code = (long long)blockIdx.x * per_cta + warp / wpc;
+  const long long index = (long long)blockIdx.x * per_cta + warp / wpc;  // a code, or a row
+  long long code = index;
+  if (BY_ROW) {
+    if (index >= a.P) return;
+    code = read_code(a.codes, a.codes64, index);
+    if (code < 0 || code >= a.K) {
+      if (a.grad_gain && blockIdx.y == 0 && lane == 0) a.grad_gain[index] = 0.f;
+      return;
+    }
+  }
   const int lo = (int)(a.P * part / wpc), hi = (int)(a.P * (part + 1) / wpc);
   const int c0 = blockIdx.y * SMALL_COLS;
   const T* grad = (const T*)a.grad_out;
@@ -194,6 +206,7 @@ __global__ void __launch_bounds__(THREADS) code_scan_kernel(const gsb_codebook_a
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       unsigned hit = __ballot_sync(0xffffffffu, c[u] == code);
+      if (BY_ROW && hit && p0 + 32 * u + __ffs(hit) - 1 < index) return;  // an earlier row's warp adds this code up
       if (code == a.K) {
         if (a.grad_gain && blockIdx.y == 0 && c[u] == code) a.grad_gain[p0 + 32 * u + lane] = 0.f;
         continue;
@@ -235,17 +248,23 @@ __global__ void __launch_bounds__(THREADS) code_scan_kernel(const gsb_codebook_a
       }
     }
   }
+  if constexpr (BY_ROW) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) s_sum[warp][lane + 32 * j] = acc[j];
-  __syncthreads();
-  if (part != 0 || code >= a.K || !a.grad_table) return;
+    for (int j = 0; j < 4; ++j)
+      if (c0 + lane + 32 * j < a.D) ((T*)a.grad_table)[code * a.D + c0 + lane + 32 * j] = from_f<T>(acc[j]);
+  } else {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int col = c0 + lane + 32 * j;
-    if (col >= a.D) continue;
-    float sum = s_sum[warp][lane + 32 * j];
-    for (int w = 1; w < wpc; ++w) sum += s_sum[warp + w][lane + 32 * j];
-    ((T*)a.grad_table)[code * a.D + col] = from_f<T>(sum);
+    for (int j = 0; j < 4; ++j) s_sum[warp][lane + 32 * j] = acc[j];
+    __syncthreads();
+    if (part != 0 || code >= a.K || !a.grad_table) return;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int col = c0 + lane + 32 * j;
+      if (col >= a.D) continue;
+      float sum = s_sum[warp][lane + 32 * j];
+      for (int w = 1; w < wpc; ++w) sum += s_sum[warp + w][lane + 32 * j];
+      ((T*)a.grad_table)[code * a.D + col] = from_f<T>(sum);
+    }
   }
 }
 
@@ -527,10 +546,13 @@ inline int key_bits(long long K) {
   return b;
 }
 
-// Warps per code of the scan, and when it is taken: it reads every code K / 8 *
-// wpc times (from L2), so it stops paying once that is tens of microseconds.
+// The scans.  By code: every code is read K / 8 * wpc times (from L2), so it
+// stops paying once that is tens of microseconds (10,000 x 256 codes x 3 fp32:
+// 22 us, the sort's eight launches 45).  By row: P * P / 32 reads at most,
+// whatever K is, and a fill of the table's gradient.
 inline int scan_warps(long long P) { return P > 4096 ? 8 : P > 2048 ? 4 : P > 1024 ? 2 : 1; }
-inline bool small_case(long long P, long long K) { return P <= (1 << 15) && P * K <= (1 << 23); }
+inline bool scan_by_code(long long P, long long K) { return P <= (1 << 14) && P * K <= (1 << 23); }
+inline bool small_case(long long P, long long K) { return P <= (1 << 12) || scan_by_code(P, K); }
 
 struct Shape {
   int vw, nv, gshift, col_blocks;
@@ -617,8 +639,14 @@ int run_bwd(const gsb_codebook_args* a, cudaStream_t s) {
   if (scan) {
     gsb_codebook_args b = *a;
     if (!fused_gain) b.grad_gain = nullptr;
-    const int wpc = scan_warps(P), per_cta = THREADS / 32 / wpc;
-    code_scan_kernel<T><<<dim3(div_up(K + 1, per_cta), div_up(a->D, SMALL_COLS)), THREADS, 0, s>>>(b, wpc);
+    const int cols = div_up(a->D, SMALL_COLS);
+    if (scan_by_code(P, K)) {
+      const int wpc = scan_warps(P), per_cta = THREADS / 32 / wpc;
+      code_scan_kernel<T, false><<<dim3(div_up(K + 1, per_cta), cols), THREADS, 0, s>>>(b, wpc);
+    } else {
+      cudaMemsetAsync(a->grad_table, 0, (size_t)K * a->D * sizeof(T), s);
+      code_scan_kernel<T, true><<<dim3(div_up(P, THREADS / 32), cols), THREADS, 0, s>>>(b, 1);
+    }
     return check_launch("gsb_codebook_bwd");
   }
 

@@ -85,6 +85,7 @@ def _run(table, codes, scale, up):
     (1, 1, 1), (1, 7, 3), (2, 1, 48), (31, 2, 3), (32, 5, 4), (33, 5, 45), (64, 64, 16), (65, 3, 8), (127, 255, 12),
     (128, 256, 20), (1000, 257, 45), (1025, 1, 48), (4097, 65_537, 3), (10_000, 256, 3), (3841, 700, 77),
     (300, 9, 128), (300, 9, 129), (77, 5, 513), (50, 4, 2001),
+    (300, 40_000, 45), (4096, 5000, 8), (3000, 100_000, 140), (1, 9_000_000, 1), (40_000, 900, 12),
 ])
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("gain", [False, True])
