@@ -18,6 +18,14 @@
 // takes care of every stride, tail and ignored row, so the passes see whole
 // tiles: rows past the end and ignored rows are zero, classes past the end
 // have the bias -inf.
+//
+// What bounds it: an exponential per row and class in each pass (16 a clock
+// and SM) while channels are few, the matrix products from about 256 channels
+// (16 bits) or 64 (fp32, six products), and below both the issue of the
+// instructions around the exponential.  On a B200, forward / dX / dW:
+//   2,073,600 x 256 classes x 16 channels fp32    245 / 378 / 312 us
+//     640,000 x 1,000 x 32 bf16                   229 / 229 / 209 us
+//      16,384 x 32,768 x 256 bf16                 286 / 406 / 430 us
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
