@@ -92,7 +92,8 @@ __device__ __forceinline__ long long read_code(const void* codes, int codes64, l
 // output is aligned.
 // ---------------------------------------------------------------------------
 template <typename T, bool ALIGNED, int ROWS>
-__global__ void __launch_bounds__(THREADS) codebook_gather_kernel(const gsb_codebook_args a, int out_aligned) {
+__global__ void __launch_bounds__(THREADS) codebook_gather_kernel(const gsb_codebook_args a, int out_aligned,
+                                                                  unsigned magic) {
   constexpr int VW = Vec16<T>::N;
   constexpr int UNROLL = ALIGNED ? 1 : 2;
   __shared__ int s_code[ROWS];
@@ -121,11 +122,23 @@ __global__ void __launch_bounds__(THREADS) codebook_gather_kernel(const gsb_code
 #pragma unroll
       for (int i = 0; i < VW; ++i) v[u][i] = 0.f;
       if (e >= total) continue;
-      unsigned r = e / D, col = e - r * D;
+      unsigned r = magic ? __umulhi(e, magic) : e / D, col = e - r * D;
       if constexpr (ALIGNED) {
         const int c = s_code[r];
         s[u] = s_scale[r];
         if (c >= 0) load_vec<T, VW>(table + (long long)c * D + col, v[u]);
+      } else if (D >= VW) {
+        // at most one row ends inside the piece
+        const unsigned r1 = min(r + 1, (unsigned)rows - 1);
+        const int c0 = s_code[r], c1 = s_code[r1];
+        const float f0 = s_scale[r], f1 = s_scale[r1];
+        const T* p0 = table + (long long)c0 * D + col;
+        const T* p1 = table + (long long)c1 * D + col - D;
+#pragma unroll
+        for (int i = 0; i < VW; ++i) {
+          const bool next = col + i >= D;
+          if ((next ? c1 : c0) >= 0 && e + i < total) v[u][i] = (next ? f1 : f0) * to_f((next ? p1 : p0)[i]);
+        }
       } else {
 #pragma unroll
         for (int i = 0; i < VW; ++i) {
@@ -697,8 +710,12 @@ void launch_gather(const gsb_codebook_args* a, cudaStream_t s) {
   const bool out_aligned = (uintptr_t)a->out % 16 == 0;
   const bool aligned = out_aligned && (long long)a->D * sizeof(T) % 16 == 0 && (uintptr_t)a->table % 16 == 0;
   const int blocks = div_up(a->P, ROWS);
-  if (aligned) codebook_gather_kernel<T, true, ROWS><<<blocks, THREADS, 0, s>>>(*a, 1);
-  else codebook_gather_kernel<T, false, ROWS><<<blocks, THREADS, 0, s>>>(*a, out_aligned);
+  // e / D is the high word of e * ceil(2^32 / D) while e * D < 2^32 (the excess of the factor, below D, then adds
+  // less than 1 / D): e < ROWS * D
+  const unsigned long long D = (unsigned long long)a->D;
+  const unsigned magic = D > 1 && ROWS * D * D < (1ull << 32) ? (unsigned)(((1ull << 32) + D - 1) / D) : 0u;
+  if (aligned) codebook_gather_kernel<T, true, ROWS><<<blocks, THREADS, 0, s>>>(*a, 1, magic);
+  else codebook_gather_kernel<T, false, ROWS><<<blocks, THREADS, 0, s>>>(*a, out_aligned, magic);
 }
 
 template <typename T>
