@@ -5,10 +5,10 @@ Tolerances count roundings.  A row element is scale * gain (one rounding of
 step).  A gradient element is a sum of n products s * g: each product carries
 at most three roundings of 2^-24, and each summand passes through at most
 min(n, DEPTH) additions (chunks of at most 128 rows, then the chunks of a run,
-which eight warps share: at most 160 of each here, the longest run being 1,251
-chunks), each one rounding of the running sum, which the sum of magnitudes
-bounds.  A gain's gradient is a dot product
-of D terms times scale.
+which eight warps share: at most 340 of each here, the longest run being a
+third of 1.06M rows in chunks of 128), each one rounding of the running sum,
+which the sum of magnitudes bounds.  A gain's gradient is a dot product of D
+terms times scale.
 """
 
 import pytest
@@ -21,7 +21,7 @@ from gswarp_b200 import codebook
 pytestmark = pytest.mark.gpu
 
 U = 2.0 ** -24
-DEPTH = 128 + 160
+DEPTH = 128 + 340
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
 
 
