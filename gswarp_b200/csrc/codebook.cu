@@ -106,7 +106,8 @@ __global__ void __launch_bounds__(THREADS) codebook_gather_kernel(const gsb_code
     const bool ok = c >= 0 && c < a.K;
     if (c < -1 || c >= a.K) atomicOr((unsigned long long*)a.error_word, (unsigned long long)ERR_BAD_CODE);
     s_code[i] = ok ? (int)c : -1;
-    s_scale[i] = a.gain ? a.scale * a.gain[base + i] : a.scale;
+    // a row without a code is zero, whatever its gain holds
+    s_scale[i] = !ok ? 0.f : a.gain ? a.scale * a.gain[base + i] : a.scale;
   }
   __syncthreads();
   const T* table = (const T*)a.table;

@@ -355,3 +355,23 @@ def test_fused_step_refuses_bad_codes(cuda):
         step.step(targets)
     step.sh_codes[5] = 3
     step.step(targets)
+
+
+@pytest.mark.parametrize("D", [3, 45, 48])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("P", [300, 20_011])
+def test_rows_without_a_code_are_zero_whatever_their_gain_holds(cuda, D, dtype, P):
+    table, codes, s, up = _inputs(P, 90, D, dtype, unassigned=0.3, seed=D)
+    gone = torch.nonzero(codes == -1)[:, 0]
+    s[gone[::3]], s[gone[1::3]] = float("nan"), float("inf")
+    rows, gt, gg = _run(table, codes, s, up)
+    assert (rows[gone] == 0).all() and (gg[gone] == 0).all()
+    clean = torch.where(codes == -1, 1.0, s)
+    _check(table, codes, clean, up, rows, gt, gg)
+    for number in (float("nan"), float("inf")):
+        assert (codebook.lookup_forward(table, codes, number)[gone] == 0).all()
+    # a code out of range is no code either
+    codes[gone[:3]] = 90
+    assert (codebook.lookup_forward(table, codes, 1.0, s)[gone] == 0).all()
+    with pytest.raises(RuntimeError, match="code"):
+        pl.raise_device_errors(cuda)
