@@ -411,7 +411,8 @@ __global__ void __launch_bounds__(THREADS) segment_sum_kernel(const SegArgs a) {
     for (int u = 0; u < SEG_UNROLL; ++u) {
       key[u] = next_key[u];
       id[u] = next_id[u];
-      s[u] = a.gain && !(id[u] & SKIP) ? a.scale * a.gain[id[u]] : a.scale;
+      // rows without a code and positions past the end add 0, not scale * 0
+      s[u] = id[u] & SKIP ? 0.f : a.gain ? a.scale * a.gain[id[u]] : a.scale;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
 #pragma unroll

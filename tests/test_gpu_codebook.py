@@ -375,3 +375,14 @@ def test_rows_without_a_code_are_zero_whatever_their_gain_holds(cuda, D, dtype, 
     assert (codebook.lookup_forward(table, codes, 1.0, s)[gone] == 0).all()
     with pytest.raises(RuntimeError, match="code"):
         pl.raise_device_errors(cuda)
+
+
+@pytest.mark.parametrize("D", [3, 48])
+@pytest.mark.parametrize("P", [300, 20_011])
+def test_an_infinite_scale_stays_with_the_rows_that_have_a_code(cuda, D, P):
+    table, codes, _, _ = _inputs(P, 4100, D, torch.float32, unassigned=0.5, seed=1)
+    up = torch.ones(P, D, device="cuda")  # every sum of a code that has rows is +inf
+    gt, _ = codebook.lookup_backward(table.shape, table.dtype, None, codes, float("inf"), None, up)
+    has = torch.zeros(4100, dtype=torch.bool, device="cuda")
+    has[codes[codes >= 0]] = True
+    assert (gt[has] == float("inf")).all() and (gt[~has] == 0).all()
