@@ -900,7 +900,8 @@ __device__ __forceinline__ double block_sum(double v) {
 // Joins the slots' (maximum, sum) pairs of every row: LANES threads per row
 // take every LANES-th slot and are joined in a fixed order (8 where a few rows
 // have hundreds of slots: 37 rows of 50,001 classes 63 -> 11 us).  A label whose
-// class takes no part (bias -inf) has the loss +inf and no gradient.  The last
+// class takes no part (bias -inf) has the loss +inf and no gradient; one whose
+// logit overflowed to -inf has its gradient, with the probability 0.  The last
 // CTA to finish adds up the CTAs' sums in their order.
 template <int LANES>
 __global__ void __launch_bounds__(THREADS) join_rows_kernel(const gsb_class_loss_args a, const Kept kept, const float* __restrict__ part_m,
@@ -936,7 +937,7 @@ __global__ void __launch_bounds__(THREADS) join_rows_kernel(const gsb_class_loss
       if (y >= 0) {
         const float t = t_label[n];
         count += 1.0;
-        if (t == -INFINITY) {
+        if (t == -INFINITY && kept.class_bias2[y] == -INFINITY) {
           l = INFINITY;
           kept.row_y[n] = -1;
         } else {

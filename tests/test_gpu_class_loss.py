@@ -474,3 +474,29 @@ def test_a_scene_with_shared_feature_rows_is_trained_through_both(cuda):
     mag.index_add_(0, codes, feats.grad.double().abs())
     assert float(mag.max()) > 0
     assert ((table.grad.double() - ref).abs() <= 300 * U * mag + 2.0 ** -149).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES[:2])
+def test_a_label_whose_logit_overflows_keeps_its_gradient(cuda, dtype):
+    # z[17, 130] = -2^200 is -inf in fp32; the class takes part, so P[17, 130] is softmax 0 less 1
+    x, w, y, b = _inputs(200, 16, 140, dtype, ignore=0.0, seed=19)
+    x[:, 0], w[:, 0] = 0.0, 0.0
+    x[17, 0], w[130, 0], y[17] = 2.0 ** 100, -2.0 ** 100, 130
+    up = _upstream("none", 200)
+    got = _run(x, w, y, b, "none", up)
+    assert got["loss"][17] == float("inf")
+    z = x[17].double() @ w.double().T + b.double()
+    p = torch.softmax(z, 0)
+    p[130] -= 1.0
+    u = up[17].double()
+    # a logit of at most 10 in magnitude: (C + 8) * 2 U * 40 for the products' magnitudes and the chain of the row's
+    # sum, 2 (64 + 10) U; P's rounding; half a step of the result; 140 products added up
+    err = (24 * 2 * U * 40 + 150 * U + P_ROUNDING[dtype] + 2 * 140 * U)
+    mag = (p.abs() @ w.double().abs()) * u
+    tol = 1.01 * (err * mag + torch.finfo(dtype).eps / 2 * ((p @ w.double()) * u).abs())
+    assert ((got["grad_features"][17].double() - (p @ w.double()) * u).abs() <= tol).all()
+    assert float(got["grad_features"][17].abs().max()) > 0
+    # the class's gradient has the row: -u x[17, 0] and nothing else in that column
+    want = -u * 2.0 ** 100
+    assert abs(float(got["grad_weight"][130, 0].double() - want)) <= 1.01 * (
+        P_ROUNDING[dtype] + 2 * U + torch.finfo(dtype).eps / 2) * abs(float(want)) * 2
