@@ -1222,11 +1222,18 @@ size_t plan_pass(StreamArgs* g) {
 }
 inline int pass_ctas(const StreamArgs& g) { return std::min(g.a_tiles * g.splits, SMS); }
 
+// A kernel's limit of shared memory belongs to the kernel, whose launches need different sizes, and host threads
+// launch side by side: every launch sets the same limit.
+template <typename... Args>
+void launch_pass(void (*kernel)(Args...), int ctas, int threads, size_t smem, cudaStream_t s, const Args&... args) {
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_MAX) == cudaSuccess)
+    kernel<<<ctas, threads, smem, s>>>(args...);
+}
+
 template <int NP, int TN, bool FP16 = false>
 int launch_forward(StreamArgs g, cudaStream_t s) {
   const size_t smem = plan_pass<FWD, NP, TN>(&g);
-  cudaFuncSetAttribute(forward_kernel<NP, TN, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  forward_kernel<NP, TN, FP16><<<pass_ctas(g), stream_threads<FWD>(), smem, s>>>(g);
+  launch_pass(forward_kernel<NP, TN, FP16>, pass_ctas(g), stream_threads<FWD>(), smem, s, g);
   return check_launch("class loss forward");
 }
 template <int NP, int TN, int PP = NP>
@@ -1234,19 +1241,12 @@ int launch_backward(StreamArgs gx, StreamArgs gw, cudaStream_t s) {
   const size_t x_smem = plan_pass<DX, NP, TN>(&gx), w_smem = plan_pass<DW, NP, TN>(&gw);
   const int x_units = gx.a_tiles * gx.splits, w_units = gw.a_tiles * gw.splits;
   if (x_units && w_units && x_units <= SMS && w_units <= SMS) {
-    const size_t smem = std::max(x_smem, w_smem);
-    cudaFuncSetAttribute(gradients_kernel<NP, TN, PP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    gradients_kernel<NP, TN, PP><<<x_units + w_units, stream_threads<DX>(), smem, s>>>(gx, gw, x_units);
+    launch_pass(gradients_kernel<NP, TN, PP>, x_units + w_units, stream_threads<DX>(), std::max(x_smem, w_smem), s, gx,
+                gw, x_units);
     return check_launch("class loss backward");
   }
-  if (x_units) {
-    cudaFuncSetAttribute(gradient_kernel<DX, NP, TN, PP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)x_smem);
-    gradient_kernel<DX, NP, TN, PP><<<pass_ctas(gx), stream_threads<DX>(), x_smem, s>>>(gx);
-  }
-  if (w_units) {
-    cudaFuncSetAttribute(gradient_kernel<DW, NP, TN, PP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)w_smem);
-    gradient_kernel<DW, NP, TN, PP><<<pass_ctas(gw), stream_threads<DW>(), w_smem, s>>>(gw);
-  }
+  if (x_units) launch_pass(gradient_kernel<DX, NP, TN, PP>, pass_ctas(gx), stream_threads<DX>(), x_smem, s, gx);
+  if (w_units) launch_pass(gradient_kernel<DW, NP, TN, PP>, pass_ctas(gw), stream_threads<DW>(), w_smem, s, gw);
   return check_launch("class loss backward");
 }
 

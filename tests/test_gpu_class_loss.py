@@ -20,10 +20,14 @@ u = 2^-24 and sums of magnitudes in place of sums:
   type (and at most one subnormal step).
 """
 
+import ctypes
+import threading
+
 import pytest
 import torch
 
 import gswarp_b200 as gs
+from gswarp_b200 import _lib
 from gswarp_b200 import _pipeline as pl
 
 pytestmark = pytest.mark.gpu
@@ -500,3 +504,49 @@ def test_a_label_whose_logit_overflows_keeps_its_gradient(cuda, dtype):
     want = -u * 2.0 ** 100
     assert abs(float(got["grad_weight"][130, 0].double() - want)) <= 1.01 * (
         P_ROUNDING[dtype] + 2 * U + torch.finfo(dtype).eps / 2) * abs(float(want)) * 2
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_two_host_threads_with_different_channels(cuda, dtype):
+    """Calls of the C ABI side by side: one kernel instantiation, two plans of shared memory."""
+    up = _upstream("mean", 1)
+    calls, want, held = [], [], []
+    for C, seed in ((16, 20), (64, 21)):
+        x, w, y, b = _inputs(300, C, 200, dtype, seed=seed)
+        want.append(_run(x, w, y, b, "mean", up))
+        a = _lib.ClassLossArgs(1, 300, 200, C, _lib.DTYPES[dtype], 2, 1, 1, 0, 1, C, -100, x.data_ptr(), w.data_ptr(),
+                               b.data_ptr(), y.data_ptr())
+        sizes = (ctypes.c_size_t * 3)()
+        _lib.call("gsb_class_loss_sizes", a, sizes)
+        kept, ws = (torch.empty(n, dtype=torch.uint8, device=cuda) for n in (sizes[0], max(sizes[1], sizes[2])))
+        out = {"loss": torch.empty(1, device=cuda), "grad_features": torch.empty_like(x),
+               "grad_weight": torch.empty_like(w), "grad_bias": torch.empty_like(b)}
+        a.kept, a.workspace, a.workspace_bytes = kept.data_ptr(), ws.data_ptr(), ws.numel()
+        a.loss, a.upstream, a.error_word = out["loss"].data_ptr(), up.data_ptr(), pl.sticky_error_word(cuda).data_ptr()
+        a.grad_features, a.grad_weight = out["grad_features"].data_ptr(), out["grad_weight"].data_ptr()
+        a.grad_bias = out["grad_bias"].data_ptr()
+        calls.append((a, out))
+        held.append((x, w, y, b, kept, ws))
+    torch.cuda.synchronize()
+    failed, start = [], threading.Barrier(2)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    L = _lib.load()
+
+    def work(k):
+        a, stream = calls[k][0], streams[k].cuda_stream
+        torch.cuda.set_device(cuda)
+        start.wait(30)
+        for _ in range(1000):
+            if L.gsb_class_loss_fwd(a, stream) or L.gsb_class_loss_bwd(a, stream):
+                failed.append((k, L.gsb_last_error()))
+                return
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed
+    for (_, out), ref in zip(calls, want):
+        assert all(torch.equal(out[n].view_as(ref[n]), ref[n]) for n in ref)
