@@ -58,8 +58,8 @@ def sticky_error_word(device: torch.device) -> torch.Tensor:
         if torch.cuda.is_current_stream_capturing():
             # it would live in the graph's memory and be cleared by every replay
             raise RuntimeError("gswarp_b200: make one call on this device before capturing a graph")
-        t = torch.zeros(1, dtype=torch.int64, device=device)
-        _STICKY[idx] = t
+        # of two host threads' first calls, both get the word that stays
+        t = _STICKY.setdefault(idx, torch.zeros(1, dtype=torch.int64, device=device))
     return t
 
 

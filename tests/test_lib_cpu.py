@@ -91,3 +91,31 @@ def test_block_dims_are_the_launched_shapes():
         assert _lib.load().gsb_block_dim(name.encode()) > 0, name
     assert _lib.load().gsb_block_dim(b"no_such_kernel") == 0
     assert _runtime.get_tuned_block_dim("no_such_kernel") == 256
+
+
+def test_the_error_word_of_two_host_threads_is_one(monkeypatch):
+    """A first call's kernels may still write to the word that the other thread's call got."""
+    import threading
+
+    import torch
+    from gswarp_b200 import _pipeline as pl
+
+    monkeypatch.setattr(pl, "_STICKY", {})
+    both, zeros, got = threading.Barrier(2), torch.zeros, [None, None]
+
+    def slow(*args, **kw):
+        t = zeros(*args, **kw)
+        both.wait(30)  # both threads have found no word
+        return t
+
+    monkeypatch.setattr(torch, "zeros", slow)
+
+    def first(k):
+        got[k] = pl.sticky_error_word(torch.device("cpu", 0))
+
+    threads = [threading.Thread(target=first, args=(k,)) for k in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert got[0] is got[1] is pl._STICKY[0]
