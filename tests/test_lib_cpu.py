@@ -101,6 +101,7 @@ def test_the_error_word_of_two_host_threads_is_one(monkeypatch):
     from gswarp_b200 import _pipeline as pl
 
     monkeypatch.setattr(pl, "_STICKY", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     both, zeros, got = threading.Barrier(2), torch.zeros, [None, None]
 
     def slow(*args, **kw):
