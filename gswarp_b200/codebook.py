@@ -67,8 +67,8 @@ def lookup_forward(table: torch.Tensor, codes: torch.Tensor, scale: float = 1.0,
 def lookup_backward(shape, dtype, table: torch.Tensor | None, codes: torch.Tensor, scale: float,
                     gain: torch.Tensor | None, grad_out: torch.Tensor, want_table: bool = True,
                     want_gain: bool = False, out: torch.Tensor | None = None):
-    """``(grad_table, grad_gain)`` of contiguous tensors, for a table of ``shape`` and ``dtype`` (read only for the
-    gains' gradient); ``grad_table`` into ``out`` if given."""
+    """``(grad_table, grad_gain)`` of contiguous tensors, for a table of ``shape`` and ``dtype``; ``grad_table`` into
+    ``out`` if given.  The table is read only for the gains' gradient, the gains only for the table's."""
     dev = grad_out.device
     a = _args(shape, dtype, table, codes, scale, gain, dev)
     a.grad_out = grad_out.data_ptr()
@@ -81,8 +81,10 @@ def lookup_backward(shape, dtype, table: torch.Tensor | None, codes: torch.Tenso
             ws = torch.empty(n, dtype=torch.uint8, device=dev)
             a.workspace, a.workspace_bytes = ws.data_ptr(), n
     if want_gain:
-        grad_gain = torch.empty_like(gain)
+        grad_gain = torch.empty(codes.shape, dtype=torch.float32, device=dev)
         a.grad_gain = grad_gain.data_ptr()
+        if gain is None:
+            a.gain = a.grad_gain  # there have to be gains, but their own gradient does not read them
     with _pipeline._stage_timer("codebook_bwd", {"rows": a.P}):
         _lib.call_on(dev, "gsb_codebook_bwd", a)
     return grad_table, grad_gain
@@ -94,11 +96,10 @@ class _CodebookLookup(torch.autograd.Function):
         t = table.contiguous()
         c = codes.contiguous()
         ctx.scale, ctx.shape, ctx.dtype = scale, table.shape, table.dtype
-        if gain is None:
-            ctx.save_for_backward(c)  # the table's gradient does not need the table
-            return lookup_forward(t, c, scale)
-        g = gain.contiguous()
-        ctx.save_for_backward(c, g, t)
+        g = gain.contiguous() if gain is not None else None
+        # what no gradient reads may change before backward: the table's reads the gains, the gains' the table
+        want_table, _, _, want_gain = ctx.needs_input_grad
+        ctx.save_for_backward(c, g if want_table else None, t if want_gain else None)
         return lookup_forward(t, c, scale, g)
 
     @staticmethod
@@ -107,8 +108,7 @@ class _CodebookLookup(torch.autograd.Function):
         want_table, _, _, want_gain = ctx.needs_input_grad
         if not (want_table or want_gain):
             return None, None, None, None
-        saved = ctx.saved_tensors
-        c, g, t = saved if len(saved) == 3 else (saved[0], None, None)
+        c, g, t = ctx.saved_tensors
         grad_table, grad_gain = lookup_backward(ctx.shape, ctx.dtype, t, c, ctx.scale, g, grad.contiguous(), want_table,
                                                 want_gain)
         return grad_table, None, None, grad_gain

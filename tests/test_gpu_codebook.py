@@ -386,3 +386,35 @@ def test_an_infinite_scale_stays_with_the_rows_that_have_a_code(cuda, D, P):
     has = torch.zeros(4100, dtype=torch.bool, device="cuda")
     has[codes[codes >= 0]] = True
     assert (gt[has] == float("inf")).all() and (gt[~has] == 0).all()
+
+
+def test_a_table_that_backward_does_not_need_may_change(cuda):
+    table, codes, s, up = _inputs(500, 11, 6, torch.float32, seed=6)
+    want = _run(table, codes, s, up)[1]
+    t = table.clone().requires_grad_(True)
+    out = gs.codebook_lookup(t, codes, s)       # the gains are fixed: no gradient reads the table
+    with torch.no_grad():
+        t.add_(1.0)
+    got, = torch.autograd.grad(out, t, up)
+    assert torch.equal(got, want)
+    gain = s.clone().requires_grad_(True)       # the gains' gradient does read it
+    out = gs.codebook_lookup(t, codes, gain)
+    with torch.no_grad():
+        t.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out, gain, up)
+    out = gs.codebook_lookup(table, codes, gain)   # and not the gains
+    want, = torch.autograd.grad(out, gain, up, retain_graph=True)
+    with torch.no_grad():
+        gain.add_(1.0)
+    got, = torch.autograd.grad(out, gain, up)
+    assert torch.equal(got, want)
+
+
+def test_gains_of_a_frozen_table(cuda):
+    for P, K, D in ((1, 1, 1), (300, 9, 48), (300, 9, 129), (20_011, 700, 45)):
+        table, codes, s, up = _inputs(P, K, D, torch.float32, seed=P)
+        gain = s.clone().requires_grad_(True)
+        out = gs.codebook_lookup(table, codes, gain)
+        gg, = torch.autograd.grad(out, gain, up)
+        _check(table, codes, s, up, out.detach(), None, gg)
