@@ -188,9 +188,11 @@ class FusedViewStep:
             raise ValueError("no views")
         self.sh_codes = None
         if sh_codes is not None:
-            if sh_codes.shape != (P,) or sh_codes.dtype not in (torch.int32, torch.int64) \
-                    or sh_codes.device != means.device:
+            if not isinstance(sh_codes, torch.Tensor) or sh_codes.shape != (P,) \
+                    or sh_codes.dtype not in (torch.int32, torch.int64) or sh_codes.device != means.device:
                 raise ValueError(f"sh_codes must be an int32 or int64 tensor of shape ({P},) on {means.device}")
+            if sh.device != means.device:
+                raise ValueError(f"the sh codebook must be on {means.device}, got {sh.device}")
             self.sh_codes = sh_codes.contiguous()
             self._sh_rows = torch.empty((P, *sh.shape[1:]), dtype=torch.float32, device=means.device)
             self._grad_sh_rows = torch.zeros_like(self._sh_rows)

@@ -89,3 +89,16 @@ def test_workspace_grows_with_the_rows_and_their_width():
     assert ws(1_000_000, 4096, 45) >= 16 * 1_000_000
     assert ws(2_000_000, 4096, 45) > ws(1_000_000, 4096, 45)
     assert ws(1_000_000, 4096, 96) > ws(1_000_000, 4096, 45)
+
+
+@pytest.mark.parametrize("sh, codes, message", [
+    (torch.empty(4, 1, 3, device="meta"), torch.zeros(7, dtype=torch.int64), "sh codebook must be on cpu"),
+    (torch.zeros(4, 1, 3), [0] * 7, "sh_codes must be"),
+    (torch.zeros(4, 1, 3), torch.zeros(7, dtype=torch.int64, device="meta"), "sh_codes must be"),
+])
+def test_fused_step_refuses_codebooks_and_codes_elsewhere(sh, codes, message):
+    from gswarp_b200.training import FusedViewStep
+
+    params = [torch.zeros(7, n) for n in (3, 3, 4, 1)] + [sh]
+    with pytest.raises(ValueError, match=message):
+        FusedViewStep(params, ["a view"], sh_codes=codes)
