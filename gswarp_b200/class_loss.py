@@ -166,10 +166,12 @@ def class_cross_entropy(features, weight, labels, bias=None, ignore_index=-100, 
     not read); a row labelled with it has the loss +inf and no gradient.
 
     With ``train`` the loss is differentiable in ``features``, ``weight`` and ``bias``; the call then keeps a
-    packed copy of the features and the classifier instead of the tensors themselves.
+    packed copy of the features and the classifier instead of the tensors themselves.  Where no gradient can be
+    asked for (none of them requires one, or gradients are off) the call is a forward alone, as with ``train=False``.
     """
     _validate(features, weight, labels, bias, ignore_index, reduction, train)
-    if not train:
+    if not (train and torch.is_grad_enabled()
+            and (features.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad))):
         with torch.no_grad():
             return _forward(features, weight, labels, bias, ignore_index, reduction, False)[0]
     return _ClassCrossEntropy.apply(features, weight, labels, bias, ignore_index, reduction)

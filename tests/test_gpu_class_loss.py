@@ -550,3 +550,26 @@ def test_two_host_threads_with_different_channels(cuda, dtype):
     assert not failed
     for (_, out), ref in zip(calls, want):
         assert all(torch.equal(out[n].view_as(ref[n]), ref[n]) for n in ref)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_no_gradient_wanted_is_a_forward_alone(cuda, dtype, monkeypatch):
+    x, w, y, b = _inputs(300, 20, 150, dtype, seed=22)
+    want = reference(x, w, y, b, -100, "mean")
+    trained, call_on = [], _lib.call_on
+
+    def spy(dev, name, a):
+        trained.append(a.train)
+        call_on(dev, name, a)
+
+    monkeypatch.setattr(_lib, "call_on", spy)
+    losses = [gs.class_cross_entropy(x, w, y, b)]
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    with torch.no_grad():
+        losses.append(gs.class_cross_entropy(leaves[0], leaves[1], y, leaves[2]))
+    for k in range(3):  # one leaf is enough
+        a, c, d = (leaves[i] if i == k else t for i, t in enumerate((x, w, b)))
+        losses.append(gs.class_cross_entropy(a, c, y, d))
+    assert trained == [0, 0, 1, 1, 1] and [t.requires_grad for t in losses] == [False, False, True, True, True]
+    for loss in losses:
+        _compare({"loss": loss.detach()}, want)
