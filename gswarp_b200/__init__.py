@@ -29,3 +29,4 @@ from .fused_ssim import fused_ssim  # noqa: F401
 from .knn import distCUDA2  # noqa: F401
 from .codebook import codebook_lookup  # noqa: F401
 from .class_loss import class_cross_entropy  # noqa: F401
+from ._pipeline import raise_device_errors  # noqa: F401

@@ -70,12 +70,14 @@ def _device_error(bits: int) -> RuntimeError:
     return RuntimeError(f"gswarp_b200 device error word {int(bits):#x} ({', '.join(what)})")
 
 
-def raise_device_errors(device: torch.device) -> None:
-    """Reads the sticky error word of ``device`` (a synchronisation of the
-    current stream) and raises if a kernel flagged an error since the last
-    check; the word is cleared before raising.  Binning checks it at its own
+def raise_device_errors(device: torch.device | str | int | None = None) -> None:
+    """Reads the sticky error word of ``device`` (default: the current CUDA
+    device; a synchronisation of the current stream) and raises a
+    ``RuntimeError`` if a kernel flagged an error since the last check; the
+    word is cleared before raising.  Binning checks it at its own
     host read of the pair count, which covers every earlier call; this
     covers the calls after it (the emit and sort of the last binning)."""
+    device = torch.device(torch.cuda.current_device() if device is None else device)
     sticky = sticky_error_word(device)
     bits = int(sticky.item())
     if bits:

@@ -120,7 +120,8 @@ def codebook_lookup(table, codes, scale=1.0):
 
     ``scale`` is a number, or a float32 tensor of ``codes``' shape (one gain per row).  Products are taken in
     float32 and rounded once.  Code -1 gives a zero row and no gradient; any other code outside ``[0, K)`` does
-    the same and is reported by the device error word (a ``RuntimeError`` at the next call that reads it).
+    the same and is reported by the device error word (a ``RuntimeError`` from
+    ``raise_device_errors``, or from the next rasterizer call, which reads it too).
     Differentiable in ``table`` and in a tensor ``scale``.
     """
     _validate(table, codes, scale)

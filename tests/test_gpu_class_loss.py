@@ -573,3 +573,16 @@ def test_no_gradient_wanted_is_a_forward_alone(cuda, dtype, monkeypatch):
     assert trained == [0, 0, 1, 1, 1] and [t.requires_grad for t in losses] == [False, False, True, True, True]
     for loss in losses:
         _compare({"loss": loss.detach()}, want)
+
+
+def test_a_program_of_the_loss_alone_learns_of_a_bad_label(cuda):
+    gs.raise_device_errors()
+    x, w, y, b = _inputs(300, 16, 150, torch.float32, seed=23)
+    y[7] = 150
+    gs.class_cross_entropy(x, w, y, b)
+    for device in (None, cuda, str(cuda), torch.cuda.current_device()):
+        y[7] = 150
+        gs.class_cross_entropy(x, w, y, b)
+        with pytest.raises(RuntimeError, match="class label out of range"):
+            gs.raise_device_errors(device)
+        gs.raise_device_errors(device)
