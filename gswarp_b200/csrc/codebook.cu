@@ -18,9 +18,12 @@
 // of K), the sorted positions are cut into chunks of equal length, and one
 // group of lanes sums each chunk's runs in registers in fp32.  A run that lies
 // inside its chunk is stored at once; the at most two that cross a chunk's
-// ends leave fp32 partial rows, which a second kernel adds up, a warp for each
-// such run (a CTA for the longest).  Few rows or codes: warps scan all the
-// codes for the ones they own, in one launch.
+// ends leave fp32 partial rows.  A CTA whose chunks all lie in one run adds
+// theirs up at its end; a second kernel adds up the rest, a warp for each run
+// that crosses chunks (a CTA for the longest), so that one code may have most
+// of the rows (6M x 48 fp32, 16,384 codes, times of the gradient: codes spread
+// 442 us, 60% in one 446, all in two 395).  Few rows or codes: teams of warps
+// scan all the codes for the ones they own, in one launch.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -77,6 +80,22 @@ __device__ __forceinline__ void store_vec(T* p, const float (&v)[VW]) {
     *reinterpret_cast<uint4*>(p) = raw;
   }
 }
+
+// The same, held as it is read.
+template <typename T, int VW>
+struct Piece {
+  uint4 raw;
+  __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void zero() { raw = make_uint4(0u, 0u, 0u, 0u); }
+  __device__ __forceinline__ float operator[](int i) const { return to_f(reinterpret_cast<const T*>(&raw)[i]); }
+};
+template <typename T>
+struct Piece<T, 1> {
+  float x;
+  __device__ __forceinline__ void load(const T* p) { x = to_f(*p); }
+  __device__ __forceinline__ void zero() { x = 0.f; }
+  __device__ __forceinline__ float operator[](int) const { return x; }
+};
 
 __device__ __forceinline__ long long read_code(const void* codes, int codes64, long long p) {
   return codes64 ? ((const long long*)codes)[p] : (long long)((const int*)codes)[p];
@@ -174,111 +193,192 @@ __global__ void __launch_bounds__(THREADS) codebook_gather_kernel(const gsb_code
 }
 
 // ---------------------------------------------------------------------------
-// Backward of few rows, in one scan of all the codes by every warp.
-// BY_ROW false (few codes): a code belongs to `wpc` warps of a CTA, each of
-// which scans its part of the codes and adds up the rows it finds, in order;
-// the parts are then added in order.  One more "code" takes the rows without
-// one (their gains' gradient is zero).
-// BY_ROW true (very few rows): a warp takes the code of one row and gives up
-// when it meets the code before that row; the first row's warp adds them all.
+// Backward of few rows, in one scan of all the codes.
+// A team of `wpc` warps of a CTA takes a code; each warp scans its part of the
+// codes, keeps the rows it finds in a queue and adds them up from there in
+// order, a batch at a time: 32 >> gshift rows side by side in groups of lanes,
+// UNROLL of them in flight per group, so that a code that most rows have is
+// bound by loads in flight and not by one latency per row.  The groups' and
+// then the warps' sums are added in a fixed order.
+// BY_ROW false (few codes): one team per code.  One more "code" takes the rows
+// without one (their gains' gradient is zero).
+// BY_ROW true (very few rows): a team takes the code of one row and gives up if
+// an earlier row has the same one; the first row's team adds them all.
 // ---------------------------------------------------------------------------
-constexpr int SMALL_COLS = 128;  // columns a warp sums at a time, four per lane
+constexpr int SCAN_COLS = 128;    // columns that a CTA sums
+constexpr int SCAN_QUEUE = 256;   // below a batch (at most 128 rows), and 128 rows more
+__host__ __device__ constexpr int scan_unroll(int vw, int nv) { return vw == 1 && nv == 1 ? 8 : 4; }
+constexpr size_t scan_smem(int warps) { return (size_t)warps * (SCAN_COLS * 4 + SCAN_QUEUE * 2); }
 
-template <typename T, bool BY_ROW>
-__global__ void __launch_bounds__(THREADS) code_scan_kernel(const gsb_codebook_args a, int wpc) {
-  __shared__ float s_sum[THREADS / 32][SMALL_COLS];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int per_cta = THREADS / 32 / wpc, part = warp % wpc;
-  const long long index = (long long)blockIdx.x * per_cta + warp / wpc;  // a code, or a row
-  long long code = index;
+// A lane's pieces of a row: NV of VW elements.
+template <typename T, int VW, int NV, bool BY_ROW, bool DGAIN>
+__global__ void __launch_bounds__(1024) code_scan_kernel(const gsb_codebook_args a, int wpc, int gshift) {
+  constexpr int UNROLL = scan_unroll(VW, NV);
+  extern __shared__ __align__(16) uint8_t scan_shared[];
+  __shared__ int s_earlier[32];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
+  float* const sums = reinterpret_cast<float*>(scan_shared) + warp * SCAN_COLS;
+  // rows are below 2^14
+  unsigned short* const queue =
+      reinterpret_cast<unsigned short*>(scan_shared + (size_t)warps * SCAN_COLS * 4) + warp * SCAN_QUEUE;
+  const int team = warp / wpc, part = warp % wpc;
+  const int G = 1 << gshift, groups = 32 >> gshift, sub = lane >> gshift;
+  const int P = (int)a.P, K = (int)a.K;
+  const long long index = (long long)blockIdx.x * (warps / wpc) + team;  // a code, or a row
+  auto code_of = [&](int p) {
+    const long long c = read_code(a.codes, a.codes64, p);
+    return c < 0 || c >= K ? K : (int)c;
+  };
+  int code = -1;  // none: nothing to do
   if (BY_ROW) {
-    if (index >= a.P) return;
-    code = read_code(a.codes, a.codes64, index);
-    if (code < 0 || code >= a.K) {
-      if (a.grad_gain && blockIdx.y == 0 && lane == 0) a.grad_gain[index] = 0.f;
-      return;
+    if (threadIdx.x < 32) s_earlier[threadIdx.x] = 0;
+    __syncthreads();
+    if (index < P) code = code_of((int)index);
+    if (code == K) {
+      if (DGAIN && blockIdx.y == 0 && part == 0 && lane == 0) a.grad_gain[index] = 0.f;
+      code = -1;
     }
-  }
-  const int lo = (int)(a.P * part / wpc), hi = (int)(a.P * (part + 1) / wpc);
-  const int c0 = blockIdx.y * SMALL_COLS;
-  const T* grad = (const T*)a.grad_out;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f}, trow[4] = {0.f, 0.f, 0.f, 0.f};
-  if (code < a.K && a.grad_gain) {
+    if (code >= 0) {
+      for (int p0 = part * 128; p0 < index; p0 += wpc * 128) {
+        bool same = false;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (c0 + lane + 32 * j < a.D) trow[j] = to_f(((const T*)a.table)[code * a.D + c0 + lane + 32 * j]);
+        for (int u = 0; u < 4; ++u) {
+          const int p = p0 + 32 * u + lane;
+          same |= p < index && code_of(p) == code;
+        }
+        if (same) s_earlier[team] = 1;
+        if (__any_sync(0xffffffffu, same || *(volatile int*)&s_earlier[team])) break;
+      }
+    }
+    __syncthreads();
+    if (s_earlier[team]) code = -1;
+  } else if (index <= K) {
+    code = (int)index;
   }
-  for (int p0 = lo; p0 < hi && code <= a.K; p0 += 32 * 4) {
-    // four codes per lane at a time: the loads are in flight together
-    long long c[4];
+
+  const int first = BY_ROW ? (int)index : 0;  // no row before it has the code
+  const int lo = first + (int)((long long)(P - first) * part / wpc);
+  const int hi = code < 0 ? lo : first + (int)((long long)(P - first) * (part + 1) / wpc);
+  const int c0 = blockIdx.y * SCAN_COLS + (lane & (G - 1)) * VW;  // and 32 further on, where NV is not 1 (G is 32)
+  const T* const grad = (const T*)a.grad_out + c0;
+  float acc[NV][VW], trow[NV][VW];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+#pragma unroll
+    for (int i = 0; i < VW; ++i) acc[j][i] = trow[j][i] = 0.f;
+    if (DGAIN && code >= 0 && code < K && c0 + 32 * j < a.D)
+      load_vec<T, VW>((const T*)a.table + (long long)code * a.D + c0 + 32 * j, trow[j]);
+  }
+  const int batch = groups * UNROLL;
+  // rows queue[from .. from + n - 1], n at most a batch
+  auto drain = [&](int from, int n) {
+    int r[UNROLL];
+    float s[UNROLL], sum[NV][VW];  // a batch's sum of its own: shorter chains of additions
+    Piece<T, VW> v[UNROLL][NV];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int i = u * groups + sub;
+      r[u] = i < n ? queue[from + i] : -1;
+      s[u] = r[u] < 0 ? 0.f : a.gain ? a.scale * a.gain[r[u]] : a.scale;
+      const T* const row = grad + (long long)r[u] * a.D;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (r[u] >= 0 && c0 + 32 * j < a.D) v[u][j].load(row + 32 * j);
+        else v[u][j].zero();
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < VW; ++i) sum[j][i] = 0.f;
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      float dot = 0.f;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < VW; ++i) {
+          const float x = v[u][j][i];
+          sum[j][i] += s[u] * x;
+          if (DGAIN) dot += x * trow[j][i];
+        }
+      if (DGAIN) {
+        for (int o = G >> 1; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        if (r[u] >= 0 && (lane & (G - 1)) == 0) a.grad_gain[r[u]] = a.scale * dot;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < VW; ++i) acc[j][i] += sum[j][i];
+  };
+  // four codes per lane, read a round ahead: the words as they are, so that nothing waits for them yet
+  int next_lo[4], next_hi[4];
+  auto fetch = [&](int p0) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int p = p0 + 32 * u + lane;
-      c[u] = p < hi ? read_code(a.codes, a.codes64, p) : -2;
-      if (p < hi && (c[u] < 0 || c[u] >= a.K)) c[u] = a.K;
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      unsigned hit = __ballot_sync(0xffffffffu, c[u] == code);
-      if (BY_ROW && hit && p0 + 32 * u + __ffs(hit) - 1 < index) return;  // an earlier row's warp adds this code up
-      if (code == a.K) {
-        if (a.grad_gain && blockIdx.y == 0 && c[u] == code) a.grad_gain[p0 + 32 * u + lane] = 0.f;
-        continue;
-      }
-      while (hit) {
-        // two rows in flight
-        const int i0 = __ffs(hit) - 1;
-        hit &= hit - 1;
-        const int i1 = hit ? __ffs(hit) - 1 : -1;
-        if (i1 >= 0) hit &= hit - 1;
-        const int r0 = p0 + 32 * u + i0, r1 = p0 + 32 * u + (i1 < 0 ? i0 : i1);
-        float v0[4], v1[4], dot0 = 0.f, dot1 = 0.f;
-        const float g0 = a.gain ? a.scale * a.gain[r0] : a.scale;
-        const float g1 = i1 < 0 ? 0.f : a.gain ? a.scale * a.gain[r1] : a.scale;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int col = c0 + lane + 32 * j;
-          v0[j] = col < a.D ? to_f(grad[(long long)r0 * a.D + col]) : 0.f;
-          v1[j] = col < a.D && i1 >= 0 ? to_f(grad[(long long)r1 * a.D + col]) : 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          acc[j] += g0 * v0[j];
-          acc[j] += g1 * v1[j];
-          dot0 += v0[j] * trow[j];
-          dot1 += v1[j] * trow[j];
-        }
-        if (a.grad_gain) {
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) {
-            dot0 += __shfl_xor_sync(0xffffffffu, dot0, o);
-            dot1 += __shfl_xor_sync(0xffffffffu, dot1, o);
-          }
-          if (lane == 0) {
-            a.grad_gain[r0] = a.scale * dot0;
-            if (i1 >= 0) a.grad_gain[r1] = a.scale * dot1;
-          }
+      next_lo[u] = -1, next_hi[u] = -1;
+      if (p < hi) {
+        if (a.codes64) {
+          const int2 w = ((const int2*)a.codes)[p];
+          next_lo[u] = w.x, next_hi[u] = w.y;
+        } else {
+          next_lo[u] = ((const int*)a.codes)[p], next_hi[u] = 0;
         }
       }
     }
+  };
+  fetch(lo);
+  int queued = 0;
+  for (int p0 = lo;; p0 += 32 * 4) {
+    const bool end = p0 >= hi;
+    if (!end) {
+      int c[4], high[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) c[u] = next_lo[u], high[u] = next_hi[u];
+      fetch(p0 + 32 * 4);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int p = p0 + 32 * u + lane;
+        if (code == K) {
+          if (DGAIN && blockIdx.y == 0 && p < hi && (high[u] != 0 || (unsigned)c[u] >= (unsigned)K)) a.grad_gain[p] = 0.f;
+          continue;
+        }
+        const bool mine = c[u] == code && high[u] == 0;
+        const unsigned hits = __ballot_sync(0xffffffffu, mine);
+        if (!hits) continue;
+        if (mine) queue[queued + __popc(hits & ((1u << lane) - 1u))] = (unsigned short)p;
+        queued += __popc(hits);
+      }
+      if (queued < batch) continue;
+    }
+    __syncwarp();
+    int from = 0;
+    for (; queued - from >= (end ? 1 : batch); from += batch) drain(from, min(batch, queued - from));
+    if (end) break;
+    // what is left, less than a batch, goes to the front
+    queued -= from;
+    unsigned short left[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) left[u] = lane + 32 * u < queued ? queue[from + lane + 32 * u] : 0;
+    __syncwarp();
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (lane + 32 * u < queued) queue[lane + 32 * u] = left[u];
   }
-  if constexpr (BY_ROW) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (c0 + lane + 32 * j < a.D) ((T*)a.grad_table)[code * a.D + c0 + lane + 32 * j] = from_f<T>(acc[j]);
-  } else {
+  for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s_sum[warp][lane + 32 * j] = acc[j];
-    __syncthreads();
-    if (part != 0 || code >= a.K || !a.grad_table) return;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int col = c0 + lane + 32 * j;
-      if (col >= a.D) continue;
-      float sum = s_sum[warp][lane + 32 * j];
-      for (int w = 1; w < wpc; ++w) sum += s_sum[warp + w][lane + 32 * j];
-      ((T*)a.grad_table)[code * a.D + col] = from_f<T>(sum);
+    for (int i = 0; i < VW; ++i) {
+      for (int o = G; o < 32; o <<= 1) acc[j][i] += __shfl_xor_sync(0xffffffffu, acc[j][i], o);
+      if (sub == 0) sums[(lane & (G - 1)) * VW + i + 32 * j] = acc[j][i];
     }
+  __syncthreads();
+  if (part != 0 || code < 0 || code >= K) return;
+  for (int c = lane; c < SCAN_COLS && blockIdx.y * SCAN_COLS + c < a.D; c += 32) {
+    float sum = sums[c];
+    for (int w = 1; w < wpc; ++w) sum += sums[w * SCAN_COLS + c];
+    ((T*)a.grad_table)[(long long)code * a.D + blockIdx.y * SCAN_COLS + c] = from_f<T>(sum);
   }
 }
 
@@ -327,6 +427,7 @@ __global__ void __launch_bounds__(THREADS) code_keys_kernel(const void* codes, i
 // right at 2c + 1 (a run that does both: its sum at 2c, both keys set).
 // ---------------------------------------------------------------------------
 constexpr unsigned NONE = 0xffffffffu;
+constexpr int LONG_RUN = 8;  // chunks
 
 struct SegArgs {
   const unsigned* keys;
@@ -455,16 +556,30 @@ __global__ void __launch_bounds__(THREADS) segment_sum_kernel(const SegArgs a) {
     a.part_keys[2 * chunk] = left_key;
     a.part_keys[2 * chunk + 1] = right_key;
   }
+  // A CTA whose chunks all lie inside one run adds their sums up, into row 2c + 1 of its first chunk, so that a run of
+  // most rows is not one CTA's to join.
+  if (a.chunks <= LONG_RUN) return;
+  __shared__ unsigned s_key;
+  const unsigned inside = left_key == right_key ? left_key : NONE;
+  if (threadIdx.x == 0) s_key = inside;
+  __syncthreads();
+  if (!__syncthreads_and(inside != NONE && inside == s_key)) return;
+  const int block = THREADS >> a.gshift, c = col0 + threadIdx.x;
+  float* const rows0 = a.part_rows + 2ll * blockIdx.x * block * a.D;
+  for (int cc = c; cc < min(a.D, col0 + G * NV * VW); cc += THREADS) {
+    float sum = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < block; ++k) sum += rows0[2ll * k * a.D + cc];
+    rows0[a.D + cc] = sum;
+  }
 }
 
 // Step 3: the runs that cross chunks.  A warp looks at one chunk; if a run
-// starts there and leaves to the right, it adds up that run's partial rows.
-// Runs of more than LONG_RUN chunks are left to the whole CTA, whose warps
-// take every eighth partial row.
-constexpr int LONG_RUN = 8;
-
+// starts there and leaves to the right, it adds up that run's partial rows, or
+// the sums of whole blocks of them.  Runs of more than LONG_RUN chunks are left
+// to the whole CTA, whose warps take every eighth partial row.
 template <typename T>
-__global__ void __launch_bounds__(THREADS) run_join_kernel(const SegArgs a) {
+__global__ void __launch_bounds__(THREADS, 8) run_join_kernel(const SegArgs a) {
   constexpr int WARPS = THREADS / 32;
   __shared__ int s_last[WARPS];
   __shared__ float s_sum[WARPS][128];
@@ -475,25 +590,30 @@ __global__ void __launch_bounds__(THREADS) run_join_kernel(const SegArgs a) {
   if (mine < a.chunks) {
     const unsigned key = a.part_keys[2 * mine + 1];
     if (key != NONE && a.part_keys[2 * mine] != key) {
-      for (int c = mine + 1;; c += 32) {
-        const unsigned stop = __ballot_sync(0xffffffffu, c + lane >= a.chunks || a.part_keys[2 * (c + lane) + 1] != key);
-        if (stop) {
-          last = c + __ffs(stop) - 1;
-          break;
-        }
+      // the first chunk that the run does not leave: among the next 32, then by 32 probes a round (keys are sorted, and
+      // no run leaves the last chunk)
+      int from = mine, step = 1;
+      last = a.chunks - 1;
+      while (last - from > 1) {
+        const unsigned stop =
+            __ballot_sync(0xffffffffu, a.part_keys[2 * min(from + (lane + 1) * step, last) + 1] != key);
+        const int f = stop ? __ffs(stop) - 1 : 32;
+        if (stop) last = min(last, from + (f + 1) * step);
+        from += f * step;
+        step = (last - from + 31) / 32;
       }
     }
   }
-  // rows of the run in chunk order: 2 * start + 1, 2 * (start + 1), 2 * (start + 2), ...
-  auto sum_rows = [&](int start, int end, int c, int from, int step) {
+  // column c of the partial rows row, row + stride, ..., n of them; every step-th from the from-th on
+  auto sum_rows = [&](long long row, int stride, int n, int c, int from, int step) {
     float sum = 0.f;
     if (c < a.D) {
-      for (int k = start + from; k <= end; k += 8 * step) {
+      for (int k = from; k < n; k += 8 * step) {
         float v[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-          const long long r = (long long)k + u * step;
-          v[u] = r <= end ? a.part_rows[(2 * r + (r == start ? 1 : 0)) * a.D + c] : 0.f;
+          const int i = k + u * step;
+          v[u] = i < n ? a.part_rows[(row + (long long)i * stride) * a.D + c] : 0.f;
         }
 #pragma unroll
         for (int u = 0; u < 8; ++u) sum += v[u];
@@ -501,10 +621,12 @@ __global__ void __launch_bounds__(THREADS) run_join_kernel(const SegArgs a) {
     }
     return sum;
   };
+  // a run's rows in chunk order: 2 * start + 1, 2 * (start + 1), 2 * (start + 2), ...
   const bool is_long = last - mine > LONG_RUN && last >= 0;
   if (last >= 0 && !is_long) {
     T* dst = (T*)a.grad_table + (long long)a.part_keys[2 * mine + 1] * a.D;
-    for (int c = lane; c < a.D; c += 32) dst[c] = from_f<T>(sum_rows(mine, last, c, 0, 1));
+    for (int c = lane; c < a.D; c += 32)
+      dst[c] = from_f<T>(a.part_rows[(2ll * mine + 1) * a.D + c] + sum_rows(2ll * mine + 2, 2, last - mine, c, 0, 1));
   }
   if (lane == 0) s_last[warp] = is_long ? last : -1;
   __syncthreads();
@@ -512,9 +634,19 @@ __global__ void __launch_bounds__(THREADS) run_join_kernel(const SegArgs a) {
     const int end = s_last[w];
     if (end < 0) continue;
     T* dst = (T*)a.grad_table + (long long)a.part_keys[2 * (first + w) + 1] * a.D;
+    // whole CTAs of the sums after start and before end, and the chunks around them
+    const int start = first + w, block = THREADS >> a.gshift;
+    const int b0 = start / block + 1, b1 = max(end / block, b0);
+    const int head = b1 > b0 ? b0 * block - start - 1 : end - start, tail = b1 > b0 ? end + 1 - b1 * block : 0;
     for (int c0 = 0; c0 < a.D; c0 += 128) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s_sum[warp][lane + 32 * j] = sum_rows(first + w, end, c0 + lane + 32 * j, warp, WARPS);
+#pragma unroll 1
+      for (int c = lane; c < 128; c += 32) {
+        float sum = sum_rows(2ll * start + 1, 1, 1, c0 + c, warp, WARPS);
+        sum += sum_rows(2ll * start + 2, 2, head, c0 + c, warp, WARPS);
+        sum += sum_rows(2ll * block * b0 + 1, 2 * block, b1 - b0, c0 + c, warp, WARPS);
+        sum += sum_rows(2ll * block * b1, 2, tail, c0 + c, warp, WARPS);
+        s_sum[warp][c] = sum;
+      }
       __syncthreads();
       const int c = threadIdx.x;
       if (c < 128 && c0 + c < a.D) {
@@ -561,11 +693,18 @@ inline int key_bits(long long K) {
   return b;
 }
 
-// The scans.  By code: every code is read K / 8 * wpc times (from L2), so it
-// stops paying once that is tens of microseconds (10,000 x 256 codes x 3 fp32:
-// 22 us, the sort's eight launches 45).  By row: P * P / 32 reads at most,
-// whatever K is, and a fill of the table's gradient.
-inline int scan_warps(long long P) { return P > 4096 ? 8 : P > 2048 ? 4 : P > 1024 ? 2 : 1; }
+// The scans.  By code: every code is read K times (from L2), so it stops
+// paying once that is tens of microseconds (16,384 x 512 codes x 48 fp32:
+// 18 us; the sort's eight launches take 45 and more).  By row: P * P reads at most, whatever
+// K is, and a fill of the table's gradient.
+// Warps of a team: more while they fit the SMs twice over, for the sake of codes
+// that most rows have (16,384 x 48 fp32, 512 codes, 60% in one: 8 warps 111 us,
+// 16 63; spread 16 and 18; a single code, 32 warps: 57).
+inline int scan_warps(long long P, long long teams) {
+  int w = P > 4096 ? 8 : P > 2048 ? 4 : P > 1024 ? 2 : 1;
+  while (w < 32 && P > 256 * w && teams * 2 * w <= 148 * 64) w *= 2;
+  return w;
+}
 inline bool scan_by_code(long long P, long long K) { return P <= (1 << 14) && P * K <= (1 << 23); }
 inline bool small_case(long long P, long long K) { return P <= (1 << 12) || scan_by_code(P, K); }
 
@@ -601,6 +740,24 @@ void launch_seg(const SegArgs& a, const Shape& sh, cudaStream_t s) {
     case 3: segment_sum_kernel<T, VW, 3, DGAIN><<<grid, THREADS, 0, s>>>(a); break;
     default: segment_sum_kernel<T, VW, 4, DGAIN><<<grid, THREADS, 0, s>>>(a); break;
   }
+}
+
+template <typename T, int VW, int NV, bool BY_ROW>
+void launch_scan(const gsb_codebook_args& a, long long teams, cudaStream_t s) {
+  // lanes that cover a row (of at most SCAN_COLS columns), and few enough rows side by side for the queue
+  const int pieces = (std::min(a.D, SCAN_COLS) + VW - 1) / VW;
+  int gshift = 0;
+  while ((1 << gshift < pieces && gshift < 5) || (32 >> gshift) * scan_unroll(VW, NV) > SCAN_QUEUE / 2) ++gshift;
+  const int wpc = scan_warps(a.P, teams), warps = std::max(wpc, 8);
+  const dim3 grid(div_up(teams * wpc, warps), div_up(a.D, SCAN_COLS));
+  if (a.grad_gain) code_scan_kernel<T, VW, NV, BY_ROW, true><<<grid, warps * 32, scan_smem(warps), s>>>(a, wpc, gshift);
+  else code_scan_kernel<T, VW, NV, BY_ROW, false><<<grid, warps * 32, scan_smem(warps), s>>>(a, wpc, gshift);
+}
+template <typename T, bool BY_ROW>
+void launch_scan(const gsb_codebook_args& a, long long teams, bool aligned, cudaStream_t s) {
+  if (aligned) launch_scan<T, Vec16<T>::N, 1, BY_ROW>(a, teams, s);
+  else if (a.D <= 32) launch_scan<T, 1, 1, BY_ROW>(a, teams, s);
+  else launch_scan<T, 1, 4, BY_ROW>(a, teams, s);
 }
 
 struct Workspace {
@@ -647,20 +804,18 @@ int run_bwd(const gsb_codebook_args* a, cudaStream_t s) {
                        (uintptr_t)a->table % 16 == 0 && (uintptr_t)a->grad_table % 16 == 0;
   const Shape sh = pick_shape(a->D, aligned ? VW : 1);
   const bool scan = a->grad_table && K > 0 && small_case(P, K);
-  const bool fused_gain = a->grad_gain && a->grad_table && K > 0 && (scan ? a->D <= SMALL_COLS : sh.col_blocks == 1);
+  const bool fused_gain = a->grad_gain && a->grad_table && K > 0 && (scan ? a->D <= SCAN_COLS : sh.col_blocks == 1);
   if (a->grad_gain && !fused_gain)
     gain_dot_kernel<T><<<div_up(P * 32, THREADS), THREADS, 0, s>>>(*a);
   if (!a->grad_table || K == 0) return check_launch("gsb_codebook_bwd");
   if (scan) {
     gsb_codebook_args b = *a;
     if (!fused_gain) b.grad_gain = nullptr;
-    const int cols = div_up(a->D, SMALL_COLS);
     if (scan_by_code(P, K)) {
-      const int wpc = scan_warps(P), per_cta = THREADS / 32 / wpc;
-      code_scan_kernel<T, false><<<dim3(div_up(K + 1, per_cta), cols), THREADS, 0, s>>>(b, wpc);
+      launch_scan<T, false>(b, K + 1, aligned, s);
     } else {
       cudaMemsetAsync(a->grad_table, 0, (size_t)K * a->D * sizeof(T), s);
-      code_scan_kernel<T, true><<<dim3(div_up(P, THREADS / 32), cols), THREADS, 0, s>>>(b, 1);
+      launch_scan<T, true>(b, P, aligned, s);
     }
     return check_launch("gsb_codebook_bwd");
   }

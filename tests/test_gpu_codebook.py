@@ -418,3 +418,29 @@ def test_gains_of_a_frozen_table(cuda):
         out = gs.codebook_lookup(table, codes, gain)
         gg, = torch.autograd.grad(out, gain, up)
         _check(table, codes, s, up, out.detach(), None, gg)
+
+
+@pytest.mark.parametrize("P, K, D", [
+    (1, 1, 4), (600, 1, 48), (5000, 3, 7), (16_384, 1, 3), (16_384, 512, 48), (16_001, 500, 129), (14_000, 599, 128),
+    (4096, 100_000, 45), (4000, 3000, 200), (4096, 2_200_000, 1), (129, 100_000, 16),
+    (40_011, 300, 1), (40_011, 300, 48), (40_011, 2, 513), (16_700, 1, 20), (140_003, 5000, 12), (300_000, 9, 8),
+])
+@pytest.mark.parametrize("dtype, gain", [(torch.float32, True), (torch.float32, False), (torch.bfloat16, True),
+                                         (torch.float16, False)])
+@pytest.mark.parametrize("codes", ["most in one", "two blocks", "sorted"])
+def test_codes_that_many_rows_have(cuda, P, K, D, dtype, gain, codes):
+    """Runs over many chunks and CTAs of the sorted sums, and full queues of the scans.  The longest chain of additions:
+    chunks of 16, CTAs of at most 256 chunks, and what a warp of the join takes of 2,501 chunks, below DEPTH."""
+    table, c, s, up = _inputs(P, K, D, dtype, torch.int32 if D % 2 else torch.int64, gain, seed=K + D)
+    i = torch.arange(P, device="cuda")
+    if codes == "most in one":
+        c = torch.where(i * 7919 % 10 < 7, K // 2, c)
+    elif codes == "two blocks":  # with runs that begin and end anywhere
+        c = torch.where(i < P // 3, 0, torch.where(i < P // 3 + 5, -1, K - 1))
+    else:
+        c = c.sort().values
+    args = (table, c.to(torch.int32 if D % 2 else torch.int64), s, up)
+    got = _run(*args)
+    _check(*args, *got)
+    again = _run(*args)
+    assert all(torch.equal(x, y) for x, y in zip(got, again) if x is not None)
