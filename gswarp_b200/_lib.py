@@ -299,15 +299,13 @@ def call(name: str, *args) -> None:
 
 def call_on(device: torch.device, name: str, args) -> None:
     """``call`` on ``device``'s current stream, with ``device`` made current
-    only if it is not: an operator of a few microseconds notices both the
-    context manager and a Stream object."""
+    only if it is not: an operator of a few microseconds notices the context
+    manager, a Stream object and every call on the way."""
     index = device.index
-    if torch.cuda.current_device() == index:
-        call(name, args, _raw_stream(index))
+    if torch._C._cuda_getDevice() == index:
+        status = getattr(_lib or load(), name)(args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
-            call(name, args, _raw_stream(index))
-
-
-def _raw_stream(index: int) -> int:
-    return torch._C._cuda_getCurrentRawStream(index)
+            status = getattr(_lib or load(), name)(args, torch._C._cuda_getCurrentRawStream(index))
+    if status != GSB_OK:
+        check(status, name)

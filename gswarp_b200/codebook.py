@@ -19,49 +19,86 @@ from . import _lib, _pipeline
 
 __all__ = ["codebook_lookup"]
 
+_INDEX_TYPES = (torch.int32, torch.int64)
+
+
+MAX_COLS = 1 << 22
+MAX_ROWS = (1 << 31) - 4096
+
 
 def _validate(table, codes, scale) -> None:
-    if not isinstance(table, torch.Tensor) or not isinstance(codes, torch.Tensor):
+    if not (isinstance(table, torch.Tensor) and isinstance(codes, torch.Tensor)):
         raise ValueError("table and codes must be torch.Tensor instances")
-    if table.ndim < 2:
-        raise ValueError(f"table must have shape (K, ...) with at least two dimensions, got {tuple(table.shape)}")
+    shape = table.shape
+    if len(shape) < 2:
+        raise ValueError(f"table must have shape (K, ...) with at least two dimensions, got {tuple(shape)}")
     if table.dtype not in _lib.DTYPES:
         raise ValueError(f"table must have dtype float32, bfloat16 or float16, got {table.dtype}")
-    if codes.dtype not in (torch.int32, torch.int64):
+    if codes.dtype not in _INDEX_TYPES:
         raise ValueError(f"codes must have dtype int32 or int64, got {codes.dtype}")
-    if not table.is_cuda or codes.device != table.device:
+    device = table.device
+    if not table.is_cuda or codes.device != device:
         raise ValueError("table and codes must be on the same CUDA device")
-    row = math.prod(table.shape[1:])
-    if row < 1 or row > 1 << 22:
-        raise ValueError(f"table rows must have 1 to {1 << 22} elements, got {row}")
-    if table.shape[0] >= (1 << 31) - 1 or codes.numel() >= (1 << 31) - 4096:
+    row = shape[1] if len(shape) == 2 else math.prod(shape[1:])
+    if not 1 <= row <= MAX_COLS:
+        raise ValueError(f"table rows must have 1 to {MAX_COLS} elements, got {row}")
+    if shape[0] >= (1 << 31) - 1 or codes.numel() >= MAX_ROWS:
         raise ValueError("table and codes must have fewer than 2**31 - 4096 rows")
+    if type(scale) is float:
+        return
     if isinstance(scale, torch.Tensor):
-        if scale.dtype != torch.float32 or scale.shape != codes.shape or scale.device != codes.device:
+        if scale.dtype != torch.float32 or scale.shape != codes.shape or scale.device != device:
             raise ValueError("a scale tensor must be float32 with the shape and device of codes")
     elif not isinstance(scale, Real) or isinstance(scale, bool):
         raise ValueError("scale must be a number or a float32 tensor")
 
 
-def _args(shape, dtype, table, codes, scale, gain, device) -> _lib.CodebookArgs:
-    a = _lib.CodebookArgs(codes.numel(), shape[0], math.prod(shape[1:]), _lib.DTYPES[dtype],
-                          codes.dtype == torch.int64, scale, None if table is None else table.data_ptr(),
-                          codes.data_ptr(), None if gain is None else gain.data_ptr())
-    a.error_word = _pipeline.sticky_error_word(device).data_ptr()
-    return a
+def _call(device, stage, name, a) -> None:
+    if _pipeline.TIMING_ENABLED:
+        with _pipeline._stage_timer(stage, {"rows": a.P}):
+            _lib.call_on(device, name, a)
+    else:
+        _lib.call_on(device, name, a)
+
+
+def _forward(table, codes, scale, gain, out):
+    """The rows, and the argument block, of contiguous tensors."""
+    dev, shape, P = table.device, table.shape, codes.numel()
+    K, *row = shape
+    D = row[0] if len(row) == 1 else math.prod(row)
+    if out is None:
+        out = table.new_empty((P, D) if codes.ndim == 1 and len(row) == 1 else codes.shape + shape[1:])
+    a = _lib.CodebookArgs(P, K, D, _lib.DTYPES[table.dtype], codes.dtype is torch.int64, scale, table.data_ptr(),
+                          codes.data_ptr(), None if gain is None else gain.data_ptr(), out.data_ptr(), None, None, None,
+                          _pipeline.sticky_error_word(dev).data_ptr())
+    _call(dev, "codebook_fwd", "gsb_codebook_fwd", a)
+    return out, a
 
 
 def lookup_forward(table: torch.Tensor, codes: torch.Tensor, scale: float = 1.0,
                    gain: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """``scale * gain * table[codes]`` of contiguous tensors, into ``out`` if given."""
-    dev = table.device
-    if out is None:
-        out = torch.empty(codes.shape + table.shape[1:], dtype=table.dtype, device=dev)
-    a = _args(table.shape, table.dtype, table, codes, scale, gain, dev)
-    a.out = out.data_ptr()
-    with _pipeline._stage_timer("codebook_fwd", {"rows": a.P, "kernels": 1}):
-        _lib.call_on(dev, "gsb_codebook_fwd", a)
-    return out
+    return _forward(table, codes, scale, gain, out)[0]
+
+
+def _backward(a, shape, codes, gain, grad_out, want_table, want_gain, out=None):
+    """Gradients for the argument block ``a``, whose table, codes and gains are set."""
+    a.grad_out = grad_out.data_ptr()
+    grad_table = grad_gain = None
+    if want_table:
+        grad_table = grad_out.new_empty(shape) if out is None else out
+        a.grad_table = grad_table.data_ptr()
+        n = _lib.load().gsb_codebook_bwd_workspace_bytes(a.P, a.K, a.D)
+        if n:
+            ws = torch.empty(n, dtype=torch.uint8, device=grad_out.device)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), n
+    if want_gain:
+        grad_gain = torch.empty(codes.shape, dtype=torch.float32, device=grad_out.device)
+        a.grad_gain = grad_gain.data_ptr()
+        if gain is None:
+            a.gain = a.grad_gain  # there have to be gains, but their own gradient does not read them
+    _call(grad_out.device, "codebook_bwd", "gsb_codebook_bwd", a)
+    return grad_table, grad_gain
 
 
 def lookup_backward(shape, dtype, table: torch.Tensor | None, codes: torch.Tensor, scale: float,
@@ -69,25 +106,24 @@ def lookup_backward(shape, dtype, table: torch.Tensor | None, codes: torch.Tenso
                     want_gain: bool = False, out: torch.Tensor | None = None):
     """``(grad_table, grad_gain)`` of contiguous tensors, for a table of ``shape`` and ``dtype``; ``grad_table`` into
     ``out`` if given.  The table is read only for the gains' gradient, the gains only for the table's."""
-    dev = grad_out.device
-    a = _args(shape, dtype, table, codes, scale, gain, dev)
-    a.grad_out = grad_out.data_ptr()
-    grad_table = grad_gain = None
-    if want_table:
-        grad_table = torch.empty(shape, dtype=dtype, device=dev) if out is None else out
-        a.grad_table = grad_table.data_ptr()
-        n = _lib.load().gsb_codebook_bwd_workspace_bytes(a.P, a.K, a.D)
-        if n:
-            ws = torch.empty(n, dtype=torch.uint8, device=dev)
-            a.workspace, a.workspace_bytes = ws.data_ptr(), n
-    if want_gain:
-        grad_gain = torch.empty(codes.shape, dtype=torch.float32, device=dev)
-        a.grad_gain = grad_gain.data_ptr()
-        if gain is None:
-            a.gain = a.grad_gain  # there have to be gains, but their own gradient does not read them
-    with _pipeline._stage_timer("codebook_bwd", {"rows": a.P}):
-        _lib.call_on(dev, "gsb_codebook_bwd", a)
-    return grad_table, grad_gain
+    a = _lib.CodebookArgs(codes.numel(), shape[0], math.prod(shape[1:]), _lib.DTYPES[dtype], codes.dtype is torch.int64,
+                          scale, None if table is None else table.data_ptr(), codes.data_ptr(),
+                          None if gain is None else gain.data_ptr())
+    a.error_word = _pipeline.sticky_error_word(grad_out.device).data_ptr()
+    return _backward(a, shape, codes, gain, grad_out, want_table, want_gain, out)
+
+
+def _gradients(ctx, grad):
+    want_table, _, _, want_gain = ctx.needs_input_grad
+    if not (want_table or want_gain):
+        return None, None, None, None
+    a = _lib.CodebookArgs.from_buffer_copy(ctx.args)
+    c, g, t = ctx.saved_tensors
+    a.codes = c.data_ptr()
+    a.gain = None if g is None else g.data_ptr()
+    a.table = None if t is None else t.data_ptr()
+    grad_table, grad_gain = _backward(a, ctx.shape, c, g, grad.contiguous(), want_table, want_gain)
+    return grad_table, None, None, grad_gain
 
 
 class _CodebookLookup(torch.autograd.Function):
@@ -95,23 +131,25 @@ class _CodebookLookup(torch.autograd.Function):
     def forward(ctx, table, codes, scale, gain):
         t = table.contiguous()
         c = codes.contiguous()
-        ctx.scale, ctx.shape, ctx.dtype = scale, table.shape, table.dtype
         g = gain.contiguous() if gain is not None else None
+        out, ctx.args = _forward(t, c, scale, g, None)
+        ctx.shape = table.shape
         # what no gradient reads may change before backward: the table's reads the gains, the gains' the table
         want_table, _, _, want_gain = ctx.needs_input_grad
         ctx.save_for_backward(c, g if want_table else None, t if want_gain else None)
-        return lookup_forward(t, c, scale, g)
+        return out
+
+    once = torch.autograd.function.once_differentiable(_gradients)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        want_table, _, _, want_gain = ctx.needs_input_grad
-        if not (want_table or want_gain):
-            return None, None, None, None
-        c, g, t = ctx.saved_tensors
-        grad_table, grad_gain = lookup_backward(ctx.shape, ctx.dtype, t, c, ctx.scale, g, grad.contiguous(), want_table,
-                                                want_gain)
-        return grad_table, None, None, grad_gain
+        # a second derivative is refused; without a graph of this pass there is nothing to refuse
+        return _CodebookLookup.once(ctx, grad) if torch.is_grad_enabled() else _gradients(ctx, grad)
+
+
+# The small calls' time is the host's (10,000 x 3 in training: 25 us of kernels).  Function.apply's part in Python takes
+# 4 us of their 80 and is there for functorch's transforms, which it refuses for this class.
+_apply = super(torch.autograd.Function, _CodebookLookup).apply
 
 
 def codebook_lookup(table, codes, scale=1.0):
@@ -127,7 +165,9 @@ def codebook_lookup(table, codes, scale=1.0):
     _validate(table, codes, scale)
     gain = scale if isinstance(scale, torch.Tensor) else None
     scale = 1.0 if gain is not None else float(scale)
-    if not torch.is_grad_enabled():
+    if not (torch.is_grad_enabled() and (table.requires_grad or (gain is not None and gain.requires_grad))):
         return lookup_forward(table.contiguous(), codes.contiguous(), scale,
                               None if gain is None else gain.contiguous())
-    return _CodebookLookup.apply(table, codes, scale, gain)
+    if torch._C._are_functorch_transforms_active():
+        return _CodebookLookup.apply(table, codes, scale, gain)
+    return _apply(table, codes, scale, gain)

@@ -444,3 +444,34 @@ def test_codes_that_many_rows_have(cuda, P, K, D, dtype, gain, codes):
     _check(*args, *got)
     again = _run(*args)
     assert all(torch.equal(x, y) for x, y in zip(got, again) if x is not None)
+
+
+def test_second_derivatives_and_transforms_are_refused(cuda):
+    table, codes, s, up = _inputs(300, 11, 6, torch.float32, seed=7)
+    t, gain = table.clone().requires_grad_(True), s.clone().requires_grad_(True)
+    want = _run(table, codes, s, up)
+    g = torch.autograd.grad(gs.codebook_lookup(t, codes, gain), (t, gain), up.requires_grad_(True), create_graph=True)
+    assert torch.equal(g[0].detach(), want[1]) and torch.equal(g[1].detach(), want[2])
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g[0].sum().backward()
+    with pytest.raises(RuntimeError, match="functorch"):
+        torch.func.grad(lambda x: gs.codebook_lookup(x, codes).sum())(table)
+
+
+def test_saved_tensors_that_moved(cuda):
+    args = _inputs(300, 11, 6, torch.float32, seed=7)
+    want = _run(*args)
+    with torch.autograd.graph.save_on_cpu():
+        t, gain = args[0].clone().requires_grad_(True), args[2].clone().requires_grad_(True)
+        out = gs.codebook_lookup(t, args[1], gain)
+        got = torch.autograd.grad(out, (t, gain), args[3])
+    assert torch.equal(got[0], want[1]) and torch.equal(got[1], want[2])
+
+
+def test_nothing_to_differentiate_keeps_nothing(cuda):
+    table, codes, s, _ = _inputs(300, 11, 6, torch.float32, seed=7)
+    assert not gs.codebook_lookup(table, codes, s).requires_grad
+    with torch.no_grad():
+        assert not gs.codebook_lookup(table.requires_grad_(True), codes, s).requires_grad
+    assert gs.codebook_lookup(table, codes, s).requires_grad
+    assert gs.codebook_lookup(table.detach(), codes, s.requires_grad_(True)).requires_grad
