@@ -318,8 +318,8 @@ __host__ __device__ constexpr int z_columns(int np, int tn) {
 // additions and added up with rounding.  fp32 features: 16 additions of the
 // leading planes' product; the other five products, 2^-8 of it and less, have
 // columns of their own, so that they do not lengthen the chain (5e-7).
-// fp16 (four products): 256 additions, 8e-6; bf16: 512, 1.5e-5; both far
-// below the half step of the gradients' type.
+// fp16 (four products): 256 additions, 8e-6; bf16: 512, 1.5e-5 (1,024 and 3e-5
+// where P has two planes); all far below the half step of the gradients' type.
 __host__ __device__ constexpr int accumulators(int np) { return np == 3 ? 2 : 1; }
 __host__ __device__ constexpr int chain_products(int np) { return np == 3 ? 16 : np == 2 ? 64 : 512; }
 
@@ -1073,7 +1073,8 @@ constexpr size_t SMEM_MIN = 118 * 1024, SMEM_MAX = 227 * 1024;
 
 // Columns of a streamed tile: the most of 128 (64 in the gradient passes,
 // whose tensor memory then has room for four z buffers), 64 and 32 with which
-// the resident tile and four stages fit.  Three planes of P take half as
+// the resident tile and four stages fit (three stages of 32 columns for fp16
+// in training with more than 224 channels).  Three planes of P take half as
 // much tensor memory again.
 template <int MODE>
 inline int tile_columns(int planes, int D8) {

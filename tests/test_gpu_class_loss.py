@@ -586,3 +586,91 @@ def test_a_program_of_the_loss_alone_learns_of_a_bad_label(cuda):
         with pytest.raises(RuntimeError, match="class label out of range"):
             gs.raise_device_errors(device)
         gs.raise_device_errors(device)
+
+
+def _exact(x, w, y):
+    """dX and dW of the summed loss in 64 bits, by pieces of rows."""
+    X, W = x.double(), w.double()
+    dX, dW = torch.empty_like(X), torch.zeros_like(W)
+    piece = max(1, 100_000_000 // W.shape[0])
+    for lo in range(0, X.shape[0], piece):
+        rows = X[lo:lo + piece]
+        p = torch.log_softmax(rows @ W.T, 1)
+        at = torch.arange(len(rows), device=x.device), y[lo:lo + piece]
+        label = torch.expm1(p[at])
+        p.exp_()
+        p[at] = label
+        dX[lo:lo + piece] = p @ W
+        dW += p.T @ rows
+    return dX, dW
+
+
+def _off(got, want):
+    return float((got.double() - want).norm() / want.norm())
+
+
+@pytest.mark.parametrize("N, C, V, dtype, most", [
+    (100_000, 5, 15, torch.bfloat16, 1.1), (100_000, 2, 149, torch.bfloat16, 1.1),     # two planes of P
+    (50_000, 32, 1000, torch.bfloat16, 1.8),                                           # one
+    (100_000, 16, 300, torch.float16, 1.1), (30_000, 200, 700, torch.float16, 1.1),
+])
+def test_gradients_are_off_by_little_more_than_their_own_rounding(cuda, N, C, V, dtype, most):
+    """Norms of the error over norms of the gradients' rounding to their type.  What comes before that rounding is
+    2^-16 of a product and less where P has two planes, which is 2^-8 of the rounding of bf16 and 2^-5 of that of fp16.
+    One plane of bf16 rounds each product as the result is rounded: sqrt(2) in all where products do not cancel, and
+    the label's term takes away up to as much again of the result."""
+    x, w, y, _ = _inputs(N, C, V, dtype, bias=False, ignore=0.0, seed=24, spread=1.0)
+    got = _run(x, w, y, None, "sum", torch.ones((), device=cuda))
+    for name, want in zip(("grad_features", "grad_weight"), _exact(x, w, y)):
+        assert _off(got[name], want) <= most * _off(want.to(dtype), want), name
+
+
+def test_the_error_of_fp32_gradients(cuda):
+    """Norm of the error over the norm of the gradients, 100,000 rows, logits of magnitude 1 and |t| below 16 in base
+    2.  Rounding the exponent twice and the row's log-sum once, 2^-20 / sqrt(12) ln 2 each: 3.3e-7 together; ex2 2^-23;
+    16 additions that truncate before a sum is taken out, half an ulp of 2^-23 on average: 16 * 2^-24; then sums that
+    are rounded, the logits' products and the planes, below 2^-24 each."""
+    x, w, y, _ = _inputs(100_000, 16, 256, torch.float32, bias=False, ignore=0.0, seed=25, spread=0.0)
+    w *= 0.3
+    got = _run(x, w, y, None, "sum", torch.ones((), device=cuda))
+    for name, want in zip(("grad_features", "grad_weight"), _exact(x, w, y)):
+        assert _off(got[name], want) <= 16 * U + 3.3e-7 + 2 * U + 3 * U, name
+
+
+@pytest.mark.parametrize("dtype, chain", [(torch.float32, 16), (torch.float16, 256), (torch.bfloat16, 512)])
+@pytest.mark.parametrize("which", ["grad_weight", "grad_features"])
+def test_long_sums_do_not_drift(cuda, dtype, chain, which):
+    """Sums of 50,000 to 300,000 products of one sign: a chain of additions that truncate loses half an ulp of 2^-23 of
+    its running sum each, always the same way, and is cut after `chain` of them.  The mean relative error of all
+    elements, from which their own rounding (half a step, uniform) goes as 1 / sqrt(n): five standard deviations of
+    it, the chain, and 3e-6 for the probabilities (ex2 2^-22, the truncated products of logits below 2 in magnitude)."""
+    g = torch.Generator(device="cuda").manual_seed(26)
+    if which == "grad_weight":
+        N, C, V = 300_000, 64, 512
+    else:
+        N, C, V = 148 * 128, 16, 200_000 if dtype == torch.bfloat16 else 50_000   # one unit per SM, over all classes
+    y = torch.zeros(N, dtype=torch.int64, device=cuda)
+    x, w = torch.randn(N, C, generator=g, device=cuda), torch.randn(V, C, generator=g, device=cuda)
+    if which == "grad_weight":
+        x, w = 0.1 + x.abs(), 0.05 * w
+    else:
+        x, w = 0.1 * x, 0.1 + w.abs()
+        w[0] = 0.0          # the label's class adds nothing
+    x, w = x.to(dtype), w.to(dtype)
+    got = _run(x, w, y, None, "sum", torch.ones((), device=cuda))[which].double()
+    want = _exact(x, w, y)[which == "grad_weight"]
+    if which == "grad_weight":
+        got, want = got[1:], want[1:]                       # the other classes' rows are positive
+    assert (want > 0).all()
+    drift = abs(float(((got - want) / want).mean()))
+    assert drift <= chain * U + 5 * torch.finfo(dtype).eps / 2 / 3 ** 0.5 / want.numel() ** 0.5 + 3e-6
+
+
+@pytest.mark.parametrize("dtype, scale", [(torch.float32, 1e4), (torch.float32, 100.0), (torch.bfloat16, 200.0),
+                                          (torch.bfloat16, 20.0), (torch.float16, 100.0), (torch.float16, 10.0)])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_gradients_at_large_logits(cuda, dtype, scale, reduction):
+    x, w, y, b = _inputs(200, 16, 300, dtype, seed=10)
+    x = (x.float() * scale).to(dtype)
+    up = _upstream(reduction, 200)
+    _compare(_run(x, w, y, b, reduction, up), reference(x, w, y, b, -100, reduction, up))
