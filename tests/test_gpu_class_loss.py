@@ -674,3 +674,15 @@ def test_gradients_at_large_logits(cuda, dtype, scale, reduction):
     x = (x.float() * scale).to(dtype)
     up = _upstream(reduction, 200)
     _compare(_run(x, w, y, b, reduction, up), reference(x, w, y, b, -100, reduction, up))
+
+
+@pytest.mark.parametrize("N, C, V", [(20_000, 16, 2), (20_000, 16, 8), (64, 1, 3)])
+def test_the_planes_of_fp32_probabilities(cuda, N, C, V):
+    """Norm of dX's error over its own, few classes and logits below 1 in magnitude, so that |t| < 4 in base 2: three
+    roundings of 2^-23 ln 2 in the exponent, ex2 2^-22, four truncations of an ulp of 2^-23 in the logits' and the
+    gradients' last products, three roundings.  1.1e-6 in all; without its third plane P alone would be off by
+    2^-18 / sqrt(3) = 2.2e-6."""
+    x, w, y, _ = _inputs(N, C, V, torch.float32, bias=False, ignore=0.0, seed=27, spread=0.0)
+    w *= 0.3
+    got = _run(x, w, y, None, "sum", torch.ones((), device=cuda))["grad_features"]
+    assert _off(got, _exact(x, w, y)[0]) <= 3 * 2 * U * 0.6931 + 4 * U + 4 * 2 * U + 3 * U
