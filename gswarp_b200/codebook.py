@@ -53,25 +53,35 @@ def _validate(table, codes, scale) -> None:
         raise ValueError("scale must be a number or a float32 tensor")
 
 
+# The small calls' time is the host's (10,000 x 3 in training: 10 us of kernels, 75 of a pass), and half of that is
+# autograd's; what runs once per call below is kept short.
+
+
 def _call(device, stage, name, a) -> None:
-    if _pipeline.TIMING_ENABLED:
-        with _pipeline._stage_timer(stage, {"rows": a.P}):
-            _lib.call_on(device, name, a)
-    else:
+    with _pipeline._stage_timer(stage, {"rows": a.P}):
         _lib.call_on(device, name, a)
 
 
 def _forward(table, codes, scale, gain, out):
     """The rows, and the argument block, of contiguous tensors."""
-    dev, shape, P = table.device, table.shape, codes.numel()
-    K, *row = shape
-    D = row[0] if len(row) == 1 else math.prod(row)
+    dev, dtype, shape = table.device, table.dtype, table.shape
+    P = codes.numel()
+    if len(shape) == 2:
+        K, D = shape
+    else:
+        K, D = shape[0], math.prod(shape[1:])
     if out is None:
-        out = table.new_empty((P, D) if codes.ndim == 1 and len(row) == 1 else codes.shape + shape[1:])
-    a = _lib.CodebookArgs(P, K, D, _lib.DTYPES[table.dtype], codes.dtype is torch.int64, scale, table.data_ptr(),
+        if len(shape) == 2 and codes.ndim == 1:
+            out = torch.empty_strided((P, D), (D, 1), dtype=dtype, device=dev)  # the quickest of torch's ways
+        else:
+            out = torch.empty(codes.shape + shape[1:], dtype=dtype, device=dev)
+    a = _lib.CodebookArgs(P, K, D, _lib.DTYPES[dtype], codes.dtype is torch.int64, scale, table.data_ptr(),
                           codes.data_ptr(), None if gain is None else gain.data_ptr(), out.data_ptr(), None, None, None,
                           _pipeline.sticky_error_word(dev).data_ptr())
-    _call(dev, "codebook_fwd", "gsb_codebook_fwd", a)
+    if _pipeline.TIMING_ENABLED:
+        _call(dev, "codebook_fwd", "gsb_codebook_fwd", a)
+    else:
+        _lib.call_on(dev, "gsb_codebook_fwd", a)
     return out, a
 
 
@@ -81,23 +91,32 @@ def lookup_forward(table: torch.Tensor, codes: torch.Tensor, scale: float = 1.0,
     return _forward(table, codes, scale, gain, out)[0]
 
 
-def _backward(a, shape, codes, gain, grad_out, want_table, want_gain, out=None):
+def _backward(a, shape, codes, gain, grad_out, want_table, want_gain, out):
     """Gradients for the argument block ``a``, whose table, codes and gains are set."""
+    dev = grad_out.device
     a.grad_out = grad_out.data_ptr()
     grad_table = grad_gain = None
     if want_table:
-        grad_table = grad_out.new_empty(shape) if out is None else out
+        if out is not None:
+            grad_table = out
+        elif len(shape) == 2:
+            grad_table = torch.empty_strided(shape, (shape[1], 1), dtype=grad_out.dtype, device=dev)
+        else:
+            grad_table = torch.empty(shape, dtype=grad_out.dtype, device=dev)
         a.grad_table = grad_table.data_ptr()
         n = _lib.load().gsb_codebook_bwd_workspace_bytes(a.P, a.K, a.D)
         if n:
-            ws = torch.empty(n, dtype=torch.uint8, device=grad_out.device)
+            ws = torch.empty(n, dtype=torch.uint8, device=dev)
             a.workspace, a.workspace_bytes = ws.data_ptr(), n
     if want_gain:
-        grad_gain = torch.empty(codes.shape, dtype=torch.float32, device=grad_out.device)
+        grad_gain = torch.empty(codes.shape, dtype=torch.float32, device=dev)
         a.grad_gain = grad_gain.data_ptr()
         if gain is None:
             a.gain = a.grad_gain  # there have to be gains, but their own gradient does not read them
-    _call(grad_out.device, "codebook_bwd", "gsb_codebook_bwd", a)
+    if _pipeline.TIMING_ENABLED:
+        _call(dev, "codebook_bwd", "gsb_codebook_bwd", a)
+    else:
+        _lib.call_on(dev, "gsb_codebook_bwd", a)
     return grad_table, grad_gain
 
 
@@ -113,19 +132,6 @@ def lookup_backward(shape, dtype, table: torch.Tensor | None, codes: torch.Tenso
     return _backward(a, shape, codes, gain, grad_out, want_table, want_gain, out)
 
 
-def _gradients(ctx, grad):
-    want_table, _, _, want_gain = ctx.needs_input_grad
-    if not (want_table or want_gain):
-        return None, None, None, None
-    a = _lib.CodebookArgs.from_buffer_copy(ctx.args)
-    c, g, t = ctx.saved_tensors
-    a.codes = c.data_ptr()
-    a.gain = None if g is None else g.data_ptr()
-    a.table = None if t is None else t.data_ptr()
-    grad_table, grad_gain = _backward(a, ctx.shape, c, g, grad.contiguous(), want_table, want_gain)
-    return grad_table, None, None, grad_gain
-
-
 class _CodebookLookup(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, codes, scale, gain):
@@ -139,16 +145,25 @@ class _CodebookLookup(torch.autograd.Function):
         ctx.save_for_backward(c, g if want_table else None, t if want_gain else None)
         return out
 
-    once = torch.autograd.function.once_differentiable(_gradients)
-
     @staticmethod
     def backward(ctx, grad):
-        # a second derivative is refused; without a graph of this pass there is nothing to refuse
-        return _CodebookLookup.once(ctx, grad) if torch.is_grad_enabled() else _gradients(ctx, grad)
+        if torch.is_grad_enabled():  # a graph of this pass is asked for: a second derivative is refused
+            return _once(ctx, grad)
+        want_table, _, _, want_gain = ctx.needs_input_grad
+        if not (want_table or want_gain):
+            return None, None, None, None
+        a = _lib.CodebookArgs.from_buffer_copy(ctx.args)
+        c, g, t = ctx.saved_tensors
+        a.codes = c.data_ptr()
+        a.gain = None if g is None else g.data_ptr()
+        a.table = None if t is None else t.data_ptr()
+        grad_table, grad_gain = _backward(a, ctx.shape, c, g, grad.contiguous(), want_table, want_gain, None)
+        return grad_table, None, None, grad_gain
 
 
-# The small calls' time is the host's (10,000 x 3 in training: 25 us of kernels).  Function.apply's part in Python takes
-# 4 us of their 80 and is there for functorch's transforms, which it refuses for this class.
+_once = torch.autograd.function.once_differentiable(_CodebookLookup.backward)
+
+# Function.apply's part in Python is there for functorch's transforms, which it refuses for this class.
 _apply = super(torch.autograd.Function, _CodebookLookup).apply
 
 
@@ -163,8 +178,11 @@ def codebook_lookup(table, codes, scale=1.0):
     Differentiable in ``table`` and in a tensor ``scale``.
     """
     _validate(table, codes, scale)
-    gain = scale if isinstance(scale, torch.Tensor) else None
-    scale = 1.0 if gain is not None else float(scale)
+    gain = None
+    if isinstance(scale, torch.Tensor):
+        gain, scale = scale, 1.0
+    else:
+        scale = float(scale)
     if not (torch.is_grad_enabled() and (table.requires_grad or (gain is not None and gain.requires_grad))):
         return lookup_forward(table.contiguous(), codes.contiguous(), scale,
                               None if gain is None else gain.contiguous())
