@@ -162,8 +162,9 @@ def class_cross_entropy(features, weight, labels, bias=None, ignore_index=-100, 
     Returns a float32 scalar ("mean" over the rows that count, "sum") or the rows' losses in ``labels``' shape
     ("none").  Rows labelled ``ignore_index`` have loss 0 and no gradient, whatever their features hold; with no
     row left the mean is 0.  Labels outside [0, V) count as ignored and are reported by the device error word (a
-    ``RuntimeError`` from ``raise_device_errors``, or from the next rasterizer call, which reads it too).  A class whose bias is -inf takes no part (its weight row is
-    not read); a row labelled with it has the loss +inf and no gradient.
+    ``RuntimeError`` from ``raise_device_errors``, or from the next rasterizer call, which reads it too).  A class
+    whose bias is -inf takes no part (its weight row is not read); a row labelled with it has the loss +inf and no
+    gradient.  Finite biases beyond 2e38 in magnitude count as 2e38.
 
     With ``train`` the loss is differentiable in ``features``, ``weight`` and ``bias``; the call then keeps a
     packed copy of the features and the classifier instead of the tensors themselves.  Where no gradient can be

@@ -20,8 +20,6 @@ from . import _lib, _pipeline
 __all__ = ["codebook_lookup"]
 
 _INDEX_TYPES = (torch.int32, torch.int64)
-
-
 MAX_COLS = 1 << 22
 MAX_ROWS = (1 << 31) - 4096
 
@@ -173,8 +171,8 @@ def codebook_lookup(table, codes, scale=1.0):
 
     ``scale`` is a number, or a float32 tensor of ``codes``' shape (one gain per row).  Products are taken in
     float32 and rounded once.  Code -1 gives a zero row and no gradient; any other code outside ``[0, K)`` does
-    the same and is reported by the device error word (a ``RuntimeError`` from
-    ``raise_device_errors``, or from the next rasterizer call, which reads it too).
+    the same and is reported by the device error word (a ``RuntimeError`` from ``raise_device_errors``, or from the
+    next rasterizer call, which reads it too).
     Differentiable in ``table`` and in a tensor ``scale``.
     """
     _validate(table, codes, scale)
