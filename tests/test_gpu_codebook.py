@@ -475,3 +475,13 @@ def test_nothing_to_differentiate_keeps_nothing(cuda):
         assert not gs.codebook_lookup(table.requires_grad_(True), codes, s).requires_grad
     assert gs.codebook_lookup(table, codes, s).requires_grad
     assert gs.codebook_lookup(table.detach(), codes, s.requires_grad_(True)).requires_grad
+
+
+@pytest.mark.parametrize("D, dtype", [(45, torch.float32), (48, torch.float32), (48, torch.bfloat16)])
+@pytest.mark.parametrize("hot", [False, True])
+def test_whole_rows_of_a_large_scene(cuda, D, dtype, hot):
+    # chunks of 128 rows; a run's 8,594 chunks in CTAs of at least 16 of them: below DEPTH additions
+    args = _inputs(1_100_003, 4096, D, dtype, torch.int32, True, seed=D)
+    if hot:
+        args[1][torch.rand(1_100_003, device="cuda") < 0.6] = 77
+    _check(*args, *_run(*args))
